@@ -5,16 +5,21 @@ This package is a thin ctypes mirror of ``include/fomoe_b200.h``; all work happe
 Python or CPU implementation of the path: if the shared library is missing or no CUDA
 device is present, construction fails loudly.
 
-The three classes follow the three groups of the C ABI:
+The classes follow the groups of the C ABI:
 
 * :class:`GpuOperator`   -- the reference's ``gpu.h`` surface (``gpu_init`` / ``gpu_expert_ffn``)
 * :class:`ExpertEngine`  -- CUDA twin of the reference's ``cpu_expert.h`` engine
 * :class:`MoeDecoder`    -- resident expert table + on-device routing + decode stack
+* :class:`BatchedMoe`    -- many tokens per call on the tensor cores
+* :class:`DeviceOps`     -- operators on device memory (torch tensors): routing, norms, FP8 products, FP8 experts
 """
 import ctypes as C
 import os
 
 import numpy as np
+
+from . import device_ops as _device_ops
+from .device_ops import DeviceOps  # noqa: F401
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("FOMOE_B200_LIB") or os.path.join(_HERE, "libfomoe_b200.so")  # override: a differently built library
@@ -152,6 +157,7 @@ _SIGS = {
     "fomoe_b200_synth_matrix": (None, [C.c_uint64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "fomoe_b200_synth_f32": (None, [C.c_uint64, C.c_int, C.c_int, C.c_float, C.c_float, C.c_uint64, _f32p]),
 }
+_SIGS.update(_device_ops.SIGS)
 
 _lib = None
 

@@ -1,0 +1,24 @@
+/*
+ * ops_quant.cuh -- one block of 128 values to e4m3 with an fp32 scale: scale = max(amax, 2^-100) / 448, q = e4m3(x / scale).
+ * Division and conversion are IEEE operations (round to nearest even), so any implementation of the formula gets the
+ * same bits.
+ */
+#pragma once
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+/* |b| joins the running amax; a NaN stays (max.NaN), so a block that holds one gets a NaN scale */
+__device__ __forceinline__ float ops_amax(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
+}
+
+__device__ __forceinline__ float ops_f8_scale(float amax) { return __fdiv_rn(ops_amax(amax, 0x1p-100f), 448.0f); }
+
+/* four numbers as e4m3, the first in the low byte */
+__device__ __forceinline__ uint32_t ops_f8_pack4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+}

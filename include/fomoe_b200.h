@@ -1,7 +1,7 @@
 /*
  * fomoe_b200.h -- C ABI of libfomoe_b200.so: fomoe's routed-expert FFN decode path on B200.
  *
- * Three groups of entry points:
+ * Groups of entry points:
  *   1. the reference's own GPU operator surface, same names and signatures
  *      (reference include/gpu.h:13-83), so a build of the reference can link this
  *      library in place of src/gpu_kernels.hip for the expert FFN;
@@ -9,7 +9,10 @@
  *      (reference include/cpu_expert.h:13-62) under the b200_expert_ prefix;
  *   3. extensions for what the reference has no call for: an HBM-resident expert table
  *      (instead of its VRAM/DRAM/NVMe tiers), the on-device router + cache-aware routing,
- *      and the multi-layer decode stack used by the benchmark.
+ *      and the multi-layer decode stack used by the benchmark;
+ *   4. the batched routed-expert FFN (many tokens per call);
+ *   5. operators on device memory for FP8 MoE layers: routing with scores, bias and groups, norms around a block,
+ *      FP8 products with block scales, FP8 experts.
  *
  * Conventions are the reference's: opaque contexts, constructors return NULL on failure,
  * int functions return 0 on success and -1 on failure, diagnostics go to stderr, nothing
@@ -376,6 +379,141 @@ int fomoe_b200_batch_get_routing(fomoe_b200_batch_t *b, int n_tokens, int *ids, 
 int fomoe_b200_batch_set_allreduce(fomoe_b200_batch_t *b, fomoe_b200_allreduce_fn fn, void *user);
 int fomoe_b200_batch_wait_profile(fomoe_b200_batch_t *b, int on, unsigned long long *out);
 void fomoe_b200_batch_synth_logits(uint64_t seed, int layer, int max_tokens, int n_experts, int n_tokens, float *out);
+
+/* ======================================================================================
+ * 5. Operators on device memory: the pieces of an FP8 MoE layer for callers that keep their tensors on the GPU.
+ *    Like fomoe_b200_matvec_noalloc they take DEVICE pointers, enqueue on the caller's stream (a cudaStream_t of the
+ *    handle's device; NULL = its default stream), allocate nothing and do not synchronise, so every call can be captured
+ *    into a CUDA graph; the device that is current on entry is current again on return.  Return 0, or -1 with the reason
+ *    in fomoe_b200_ops_last_error (and on stderr) and nothing enqueued.  A call with no rows returns 0.
+ *    A handle is used from one thread at a time; any number of streams may have its calls in flight.
+ *
+ *    FP8 here is e4m3 (OCP: 4 exponent bits, largest value 448) with fp32 scales: one for each block of 128 values of an
+ *    activation row (the last block may be shorter), one for each 128 x 128 block of a weight matrix (the last ones may
+ *    be smaller).  A value is its e4m3 number times its block's scale.  Products sum in fp32 inside a block of 128 and
+ *    across blocks.
+ * ====================================================================================== */
+typedef struct fomoe_b200_ops fomoe_b200_ops_t;
+
+#define FOMOE_B200_F32 0
+#define FOMOE_B200_BF16 1
+#define FOMOE_B200_F8 2
+
+fomoe_b200_ops_t *fomoe_b200_ops_create(int device);
+void fomoe_b200_ops_destroy(fomoe_b200_ops_t *ops); /* none of its calls may still be in flight */
+const char *fomoe_b200_ops_last_error(fomoe_b200_ops_t *ops);
+/* What went wrong on the device since the last call of this function (as far as the device has got: synchronise first
+ * for what is in flight): 0 nothing, 1 an expert id outside the table (its pair was left out), 2 a kernel gave a bounded
+ * wait up (what it wrote is incomplete).  Reading clears it. */
+int fomoe_b200_ops_status(fomoe_b200_ops_t *ops);
+uint64_t fomoe_b200_ops_kernel_launches(fomoe_b200_ops_t *ops);
+
+/* Routing.  For every token: p = softmax or sigmoid of its logits; choice c_e = p_e + bias_e; with n_group > 1 the
+ * experts fall into n_group equal runs, a run scores the sum of the group_best (1 or 2) best choices in it, and only the
+ * topk_group best runs stay (lower run first among equals); the top_k experts by choice, best first (lower id first among
+ * equals).  ids[t][j] and weights[t][j] = p_e (without the bias); renorm: divided by their sum + 1e-20; times scale.
+ * The order is the order of the exact values: near ties are decided in 64 bits, and without a bias by the logits.
+ * Closed experts are never chosen: a logit of -inf or NaN, or a bias of -inf or NaN.  A logit of +inf counts as FLT_MAX.
+ * valid (optional, one byte per token): a token whose byte is 0 (padding) has all experts closed.  A slot that no open
+ * expert fills gets id -1 and weight 0. */
+#define FOMOE_B200_SOFTMAX 0
+#define FOMOE_B200_SIGMOID 1
+typedef struct {
+    int n_experts;  /* <= 512 */
+    int top_k;      /* <= 16, <= n_experts */
+    int score;      /* FOMOE_B200_SOFTMAX or FOMOE_B200_SIGMOID */
+    int n_group;    /* divides n_experts, <= 32; 1 = no groups */
+    int topk_group; /* 1 .. n_group */
+    int group_best; /* 1 or 2 */
+    int renorm;
+    float scale;
+} fomoe_b200_route_config_t;
+int fomoe_b200_ops_route(fomoe_b200_ops_t *ops, const fomoe_b200_route_config_t *cfg, int n_tokens, const void *logits,
+                         int logits_type /* F32 or BF16 */, int64_t row_stride /* elements */,
+                         const float *bias /* [n_experts] or NULL */, const uint8_t *valid /* [n_tokens] or NULL */,
+                         int *ids /* [n_tokens][top_k] */, float *weights /* [n_tokens][top_k] */, void *stream);
+
+/* Norms around a block, with its gate and residual scale, in one pass over the row:
+ *     r  = block                                            or, with post, rms(block) * (post + offset)
+ *     x' = x + scale * gate * r                             (gate optional; without a block x' = x)
+ *     h  = rms(x') * (pre + offset),   rms(v) = v / sqrt(mean(v^2) + eps)
+ * x' goes to x_out (optional; may be x itself) in x's type, h to h in h_type.  All arithmetic is fp32; h is made from the
+ * unrounded x'.  h_type F8: e4m3 with scales (as fomoe_b200_ops_f8_quantize makes them).  Strides are in elements;
+ * x_out and h overlap no input except that x_out may be x with x's stride. */
+typedef struct {
+    int n_tokens, n; /* n <= 16384 */
+    float eps, offset, scale;
+    const void *x;
+    int x_type; /* F32 or BF16 */
+    int64_t x_stride;
+    const void *block; /* or NULL */
+    int block_type;
+    int64_t block_stride;
+    const float *post; /* [n] or NULL */
+    const void *gate;  /* of block's type: element (t, i) at gate[t * gate_stride + i * gate_step], step 0 or 1; or NULL */
+    int64_t gate_stride;
+    int gate_step;
+    void *x_out; /* or NULL */
+    int64_t x_out_stride;
+    const float *pre; /* [n]; NULL: no h */
+    void *h;
+    int h_type;
+    int64_t h_stride;
+    float *h_scales; /* F8 only: [n_tokens][ceil(n / 128)] */
+    int64_t h_scales_stride;
+} fomoe_b200_norm_args_t;
+int fomoe_b200_ops_norm(fomoe_b200_ops_t *ops, const fomoe_b200_norm_args_t *args, void *stream);
+
+/* Rows to FP8: per block of 128 columns scale = max(amax, 2^-100) / 448 and q = e4m3(x / scale), each operation rounded
+ * once in fp32 (to nearest even; e4m3 likewise).  A block that holds an infinity or a NaN comes back as NaN. */
+int fomoe_b200_ops_f8_quantize(fomoe_b200_ops_t *ops, int rows, int cols, const void *x, int x_type /* F32 or BF16 */,
+                               int64_t x_stride, uint8_t *q, int64_t q_stride, float *scales, int64_t scales_stride,
+                               void *stream);
+
+/* out[m][n] = sum_k a[m][k] b[n][k], a FP8 rows, b an FP8 weight matrix.  k a multiple of 16; a and b 16-byte aligned,
+ * their strides (bytes) multiples of 16; scale strides in elements. */
+typedef struct {
+    int m, n, k;
+    const uint8_t *a;
+    int64_t a_stride;
+    const float *a_scales; /* [m][ceil(k / 128)] */
+    int64_t a_scales_stride;
+    const uint8_t *b;
+    int64_t b_stride;
+    const float *b_scales; /* [ceil(n / 128)][ceil(k / 128)] */
+    int64_t b_scales_stride;
+    void *out; /* [m][n] */
+    int out_type; /* F32 or BF16 */
+    int64_t out_stride;
+} fomoe_b200_f8_matmul_args_t;
+int fomoe_b200_ops_f8_matmul(fomoe_b200_ops_t *ops, const fomoe_b200_f8_matmul_args_t *args, void *stream);
+
+/* The experts of one layer on FP8 rows, routing given:
+ *     z = gate_up_e x,  act = silu(z[0 .. I)) * z[I .. 2 I)  (to FP8 per 128),  y_e = down_e act
+ *     out[t] = sum_j weights[t][j] y_{ids[t][j]}  (in slot order)  + y_shared   (bf16)
+ * ids of -1 are left out (as fomoe_b200_ops_route writes them); other ids outside 0 .. n_experts - 1 too, with status 1.
+ * A token with no expert at all gets zeros.  The tables hold n_experts + has_shared contiguous records, the shared
+ * expert last.  workspace: fomoe_b200_ops_f8_experts_workspace bytes, 256-byte aligned; its contents do not matter
+ * before or after, and calls that may overlap on the GPU (two streams, two graphs) each need their own. */
+typedef struct {
+    int n_tokens, n_embd, n_inter; /* multiples of 128, <= 16384 */
+    int n_experts, top_k, has_shared; /* n_experts <= 512, top_k <= 16 */
+    const uint8_t *x; /* [n_tokens][n_embd] e4m3 */
+    int64_t x_stride; /* bytes, a multiple of 16 */
+    const float *x_scales; /* [n_tokens][n_embd / 128] */
+    int64_t x_scales_stride;
+    const int *ids;       /* [n_tokens][top_k] */
+    const float *weights; /* [n_tokens][top_k] */
+    const uint8_t *gate_up;      /* [records][2 n_inter][n_embd] e4m3: the gate rows, then the up rows */
+    const float *gate_up_scales; /* [records][2 n_inter / 128][n_embd / 128] */
+    const uint8_t *down;         /* [records][n_embd][n_inter] */
+    const float *down_scales;    /* [records][n_embd / 128][n_inter / 128] */
+    void *out; /* [n_tokens][n_embd] bf16 */
+    int64_t out_stride;
+} fomoe_b200_f8_experts_args_t;
+uint64_t fomoe_b200_ops_f8_experts_workspace(const fomoe_b200_f8_experts_args_t *args); /* 0: the sizes are refused */
+int fomoe_b200_ops_f8_experts(fomoe_b200_ops_t *ops, const fomoe_b200_f8_experts_args_t *args, void *workspace,
+                              uint64_t workspace_bytes, void *stream);
 
 /* Host-side synthetic generator (same bytes as fomoe_b200_table_generate puts on the device). */
 void fomoe_b200_synth_matrix(uint64_t seed, int layer, int expert, int matrix, int type, int rows, int cols,
