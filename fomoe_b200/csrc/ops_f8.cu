@@ -26,8 +26,8 @@
 #define BK_WARPS 32
 
 __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n_routed, int n_tokens, int n_experts,
-                                                          int has_shared, int *counts, int *pairs, int4 *items,
-                                                          int *status) {
+                                                          int has_shared, int tile, int *counts, int *pairs,
+                                                          int4 *items, int *status) {
     extern __shared__ int s_cnt[]; /* [n_experts][BK_WARPS] */
     __shared__ int s_tot[BK_WARPS], s_til[BK_WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -54,11 +54,11 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
         }
         if (pass == 1) break;
         __syncthreads();
-        /* thread e: the expert's total, then exclusive prefixes of pairs and of 128-row tiles over the experts */
+        /* thread e: the expert's total, then exclusive prefixes of pairs and of tiles (`tile` rows) over the experts */
         int tot = 0;
         if (tid < n_experts)
             for (int w = 0; w < BK_WARPS; w++) tot += s_cnt[tid * BK_WARPS + ((w + tid) & 31)];
-        const int til = (tot + 127) / 128;
+        const int til = (tot + tile - 1) / tile;
         int a = tot, c = til;
         for (int s = 1; s < 32; s <<= 1) {
             const int oa = __shfl_up_sync(FULL, a, s), oc = __shfl_up_sync(FULL, c, s);
@@ -84,12 +84,12 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
                 s_cnt[tid * BK_WARPS + w] = at;
                 at += n;
             }
-            for (int m = 0; m < til; m++) items[tbase + m] = make_int4(tid, base + 128 * m, min(128, tot - 128 * m), 0);
+            for (int m = 0; m < til; m++) items[tbase + m] = make_int4(tid, base + tile * m, min(tile, tot - tile * m), 0);
         }
         if (tid == BK_THREADS - 1) { /* no expert's thread: n_experts <= 512 */
-            const int sh = has_shared ? (n_tokens + 127) / 128 : 0;
+            const int sh = has_shared ? (n_tokens + tile - 1) / tile : 0;
             for (int m = 0; m < sh; m++)
-                items[tbase + m] = make_int4(n_experts, base + 128 * m, min(128, n_tokens - 128 * m), 0);
+                items[tbase + m] = make_int4(n_experts, base + tile * m, min(tile, n_tokens - tile * m), 0);
             counts[0] = tbase + sh; /* tiles */
             counts[1] = base;       /* routed pairs that are left */
         }
@@ -109,15 +109,18 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
  * acc = fma(sum, sa sb, acc).  A row is a lane of tensor memory and a weight tile has one scale a block, so a thread needs
  * one factor for all of its columns.
  *
- * One persistent block per SM, warp-specialised: warp 8 asks for the operand tiles (TMA, 128-byte swizzle, one block of
- * 128 k a stage), one thread of warp 9 issues the MMAs (M = 128 rows, N = NT columns), warps 0..7 are two warpgroups
- * that each join half of the columns.  Tensor memory holds NB buffers of NT columns, so the MMAs of the next block run
- * while this one's sums are joined: NT / 2 columns a thread are NT / 4 two-wide FMAs of 2 warps a scheduler, under the
- * 2 NT cycles that the MMAs of the block take.
+ * Persistent blocks, one per SM, warp-specialised: warp 8 asks for the operand tiles (TMA, 128-byte swizzle, one block of
+ * 128 k a stage), one thread of warp 9 issues the MMAs (NT columns), warps 0..7 are two warpgroups that each join half of
+ * the columns.  Tensor memory holds NB buffers of NT columns, so the MMAs of the next block run while this one's sums are
+ * joined.
  *
- *   dense    A: rows of a;                                 B: NT rows of b;                 D to out
- *   gate/up  A: the tokens of an expert's pairs (gather4); B: 128 gate rows, 128 up rows;   silu(g) u to FP8, 128 a block
- *   down     A: an expert's rows of the activations;       B: NT rows of its down matrix;   D to the pair's row of dots
+ * PAIR: two SMs work on one tile of 256 rows x 256 columns (cta_group::2).  Each loads its own 128 rows and half of the
+ * columns' weights, 32 KB a block of k instead of 48 KB for the same MMAs: with one SM a tile the kernel ran at the L2's
+ * bandwidth (4096 x 8192 x 4096: 11.8 TB/s, the tensor cores 45 % busy).
+ *
+ *   dense    A: rows of a;                               B: rows of b;                        D to out
+ *   gate/up  A: the tokens of an expert's pairs;         B: 128 gate rows, 128 up rows;       silu(g) u to FP8, 128 a block
+ *   down     A: the activations of an expert's pairs;    B: rows of its down matrix;          D to the pair's row of dots
  *
  * Every wait is bounded; when one runs out the status word is set, all roles stop waiting and the block drains, frees its
  * tensor memory and returns. */
@@ -128,6 +131,7 @@ enum { F8_DENSE = 0, F8_GATE_UP = 1, F8_DOWN = 2 };
 #define F8_WAIT_LIMIT (1u << 22)
 #define F8_A_BYTES 16384u /* 128 rows x 128 k */
 #define F8_MAX_STAGES 8
+#define F8_SC 4 /* blocks of k whose scales are handed over at once */
 
 typedef struct {
     CUtensorMap ta, tb;
@@ -144,15 +148,15 @@ typedef struct {
     float *act_scales;
     const int *counts, *pairs;
     const int4 *items;
-    int n_routed, top_k;
     int *status;
 } f8_args_t;
 
 typedef struct {
-    uint64_t full[F8_MAX_STAGES], empty[F8_MAX_STAGES], acc_full[4], acc_empty[4];
+    uint64_t full[F8_MAX_STAGES], empty[F8_MAX_STAGES], acc_full[4], acc_empty[4], sc_full[2], sc_empty[2];
     uint32_t tmem_base;
     volatile int abort_flag;
-    float amax[2][2][128]; /* tile parity, warpgroup, row */
+    float amax[2][2][128];              /* tile parity, warpgroup, row */
+    float scale[2][F8_SC][2][128];      /* group parity, block of k in the group, column half, row: sa sb */
 } f8_ctl_t;
 
 __device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, f8_ctl_t *C) {
@@ -170,49 +174,74 @@ __device__ __forceinline__ uint64_t f8_desc(uint32_t saddr) {
            ((uint64_t)2 << 61);
 }
 
+template <bool PAIR>
 __device__ __forceinline__ void f8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+            "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+            "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
 
+/* all MMAs so far, then an arrival at `bar`, in a pair at both SMs' */
+template <bool PAIR>
 __device__ __forceinline__ void f8_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+/* the same shared-memory address in the pair's first SM */
+__device__ __forceinline__ uint32_t f8_leader(uint32_t addr) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+
+/* a box of the map to this SM's shared memory; bar may be the pair's first SM's */
+template <bool PAIR>
 __device__ __forceinline__ void f8_tma2(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+            "[%4];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
 }
 
-/* four rows of the map, anywhere */
-__device__ __forceinline__ void f8_gather4(uint32_t dst, const CUtensorMap *map, int x, int4 y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
-        "%6}], [%7];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w), "r"(bar)
-        : "memory");
+__device__ __forceinline__ void f8_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void f8_tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
+__device__ __forceinline__ void f8_tmem_ld32(uint32_t taddr, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr));
 }
 
-/* the loads of r have landed (r passes through so that nothing reads it earlier) */
-__device__ __forceinline__ void f8_tmem_wait(uint32_t (&r)[16]) {
+/* the loads have landed (32 registers pass through so that nothing reads them earlier) */
+__device__ __forceinline__ void f8_tmem_wait(uint32_t *r) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
 /* acc += v s, two columns at once */
@@ -225,19 +254,33 @@ __device__ __forceinline__ void f8_fma2(float2 &acc, uint32_t v0, uint32_t v1, f
     asm("mov.b64 {%0, %1}, %2;" : "=f"(acc.x), "=f"(acc.y) : "l"(a));
 }
 
+__device__ __forceinline__ float f8_silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+
+template <int MODE, int NT, bool PAIR>
+struct f8_cfg {
+    static constexpr int ROWS = PAIR ? 256 : 128;                /* of a tile */
+    static constexpr int B_BYTES = (PAIR ? NT / 2 : NT) * 128;   /* of one SM's share */
+    static constexpr int STAGE = (int)F8_A_BYTES + B_BYTES;
+    static constexpr int STAGES = PAIR ? 6 : NT == 256 ? 4 : NT == 128 ? 6 : 8;
+    static constexpr int NB = NT == 256 ? 2 : 4;
+    static constexpr int OUT = F8_EPI_WARPS * 2048;              /* a warp's 32 rows x 64 bytes on their way out */
+    static constexpr int SMEM = STAGES * STAGE + OUT + 1024 + (int)sizeof(f8_ctl_t);
+};
+
 /* what tile `it` is */
 typedef struct {
     int e, r0, rows, n0;
 } f8_tile_t;
 
-template <int MODE, int NT>
+template <int MODE, int NT, bool PAIR>
 __device__ __forceinline__ f8_tile_t f8_tile(const f8_args_t &P, int it, int n_tiles) {
+    constexpr int ROWS = f8_cfg<MODE, NT, PAIR>::ROWS;
     f8_tile_t t;
     if (MODE == F8_DENSE) { /* rows first: tiles in flight at the same time share rows of b */
-        const int mt = (P.m + 127) / 128, nt = it / mt;
+        const int mt = (P.m + ROWS - 1) / ROWS, nt = it / mt;
         t.e = 0;
-        t.r0 = (it - nt * mt) * 128;
-        t.rows = min(128, P.m - t.r0);
+        t.r0 = (it - nt * mt) * ROWS;
+        t.rows = min(ROWS, P.m - t.r0);
         t.n0 = nt * NT;
     } else {
         const int g = it / n_tiles;
@@ -250,25 +293,60 @@ __device__ __forceinline__ f8_tile_t f8_tile(const f8_args_t &P, int it, int n_t
     return t;
 }
 
-template <int MODE, int NT>
-struct f8_cfg {
-    static constexpr int B_BYTES = NT * 128, STAGE = (int)F8_A_BYTES + B_BYTES;
-    static constexpr int STAGES = NT == 256 ? 4 : NT == 128 ? 6 : 8;
-    static constexpr int NB = NT == 256 ? 2 : 4;
-    static constexpr int SMEM = STAGES * STAGE + 1024 + (int)sizeof(f8_ctl_t);
-};
+/* Out of registers, coalesced: a warp's 32 rows x N8 x 8 bytes pass through shared memory 64 bytes of a row at a time (the
+ * 16-byte pieces of row r at piece ^ (r / 2) % 4, so that neither side has bank conflicts) and leave as runs of 64 bytes.
+ * rowp: where row 0 .. 31 of the warp begin (NULL: not stored); left: bytes of a row that are inside out. */
+template <int BYTES>
+__device__ __forceinline__ void f8_rows_out(uint32_t buf, const uint32_t *w, uint8_t *my_row, int left, int vec, int elem) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int c = 0; c < BYTES / 64; c++) {
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 64u + (uint32_t)((q ^ ((lane >> 1) & 3)) << 4)),
+                         "r"(w[16 * c + 4 * q]), "r"(w[16 * c + 4 * q + 1]), "r"(w[16 * c + 4 * q + 2]), "r"(w[16 * c + 4 * q + 3])
+                         : "memory");
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = 8 * i + (lane >> 2), q = lane & 3, at = 64 * c + 16 * q;
+            uint8_t *row = reinterpret_cast<uint8_t *>(__shfl_sync(FULL, (unsigned long long)my_row, r));
+            const uint4 v = fb_lds128(buf + r * 64u + (uint32_t)((q ^ ((r >> 1) & 3)) << 4));
+            if (row && at < left) {
+                if (vec && at + 16 <= left) {
+                    *reinterpret_cast<uint4 *>(row + at) = v;
+                } else {
+                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        if (elem == 4) {
+                            if (at + 4 * k < left) *reinterpret_cast<uint32_t *>(row + at + 4 * k) = x[k];
+                        } else {
+                            if (at + 4 * k < left) *reinterpret_cast<uint16_t *>(row + at + 4 * k) = (uint16_t)x[k];
+                            if (at + 4 * k + 2 < left) *reinterpret_cast<uint16_t *>(row + at + 4 * k + 2) = (uint16_t)(x[k] >> 16);
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
 
-template <int MODE, int NT>
+template <int MODE, int NT, bool PAIR>
 __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant__ f8_args_t P) {
-    typedef f8_cfg<MODE, NT> cfg;
+    typedef f8_cfg<MODE, NT, PAIR> cfg;
     constexpr int STAGES = cfg::STAGES, NB = cfg::NB;
     extern __shared__ uint8_t dyn_raw[];
     const uint32_t dyn_u = (fb_smem_u32(dyn_raw) + 1023u) & ~1023u;
-    f8_ctl_t *C = reinterpret_cast<f8_ctl_t *>(dyn_raw + (dyn_u - fb_smem_u32(dyn_raw)) + STAGES * cfg::STAGE);
+    const uint32_t out_u = dyn_u + STAGES * cfg::STAGE;
+    f8_ctl_t *C = reinterpret_cast<f8_ctl_t *>(dyn_raw + (dyn_u - fb_smem_u32(dyn_raw)) + STAGES * cfg::STAGE + cfg::OUT);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
+    const int first = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, stride = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
     const int per_n = MODE == F8_GATE_UP ? NT / 2 : NT;
     const int n_tiles = (P.n + per_n - 1) / per_n, kbs = (P.k + 127) / 128;
-    const int tiles = MODE == F8_DENSE ? ((P.m + 127) / 128) * n_tiles : P.counts[0] * n_tiles;
+    const int tiles = (MODE == F8_DENSE ? (P.m + cfg::ROWS - 1) / cfg::ROWS : P.counts[0]) * n_tiles;
 
     if (tid == 0) {
         for (int s = 0; s < STAGES; s++) {
@@ -277,19 +355,31 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
         }
         for (int b = 0; b < NB; b++) {
             fb_mbar_init(fb_smem_u32(&C->acc_full[b]), 1);
-            fb_mbar_init(fb_smem_u32(&C->acc_empty[b]), F8_EPI_WARPS);
+            fb_mbar_init(fb_smem_u32(&C->acc_empty[b]), PAIR ? 2 * F8_EPI_WARPS : F8_EPI_WARPS);
+        }
+        for (int g = 0; g < 2; g++) {
+            fb_mbar_init(fb_smem_u32(&C->sc_full[g]), 2);
+            fb_mbar_init(fb_smem_u32(&C->sc_empty[g]), F8_EPI_WARPS);
         }
         C->abort_flag = 0;
         fb_mbar_init_fence();
     }
     if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fb_smem_u32(&C->tmem_base)),
-                     "r"((uint32_t)(NB * NT))
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fb_smem_u32(&C->tmem_base)),
+                         "r"((uint32_t)(NB * NT))
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fb_smem_u32(&C->tmem_base)),
+                         "r"((uint32_t)(NB * NT))
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    if (PAIR) f8_cluster_sync();
+    else __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = C->tmem_base;
 
@@ -300,54 +390,38 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             /* ---------------- operand tiles */
             uint32_t step = 0;
             bool ok = true;
-            for (int it = blockIdx.x; it < tiles && ok; it += gridDim.x) {
-                const f8_tile_t t = f8_tile<MODE, NT>(P, it, n_tiles);
-                int4 rows = make_int4(0, 0, 0, 0); /* gate/up: this lane's four tokens; past the end, the last pair's again */
-                int groups = (t.rows + 31) / 32;
-                uint32_t a_bytes = (uint32_t)groups * 4096u;
-                if (MODE == F8_GATE_UP) {
-                    int v[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int p = P.pairs[t.r0 + min(4 * lane + i, t.rows - 1)];
-                        v[i] = p < P.n_routed ? p / P.top_k : p - P.n_routed;
-                    }
-                    rows = make_int4(v[0], v[1], v[2], v[3]);
-                    groups = (t.rows + 3) / 4;
-                    a_bytes = (uint32_t)groups * 512u;
-                }
+            for (int it = first; it < tiles && ok; it += stride) {
+                const f8_tile_t t = f8_tile<MODE, NT, PAIR>(P, it, n_tiles);
+                /* boxes of 32 rows, as many as this SM's rows need; what is behind the tile's rows is never stored */
+                const int groups = min(4, max(0, (t.rows - 128 * rank + 31) / 32));
+                const int y = t.e * P.b_rec_rows + (MODE == F8_GATE_UP && rank ? P.n + t.n0 : t.n0 + (PAIR ? NT / 2 * rank : 0));
+                const uint32_t bytes = (uint32_t)((t.rows + 31) / 32) * 4096u + (PAIR ? 2u : 1u) * cfg::B_BYTES; /* of both SMs */
                 for (int kb = 0; kb < kbs; kb++, step++) {
                     const int s = step % STAGES;
-                    const uint32_t bar = fb_smem_u32(&C->full[s]), a_u = dyn_u + s * cfg::STAGE, b_u = a_u + F8_A_BYTES;
+                    const uint32_t a_u = dyn_u + s * cfg::STAGE, b_u = a_u + F8_A_BYTES;
                     if (!__all_sync(FULL, f8_wait(fb_smem_u32(&C->empty[s]), ((step / STAGES) & 1) ^ 1, C))) {
                         ok = false;
                         break;
                     }
+                    const uint32_t own = fb_smem_u32(&C->full[s]), bar = PAIR ? f8_leader(own) : own;
                     if (lane == 0) {
-                        fb_mbar_expect_tx(bar, a_bytes + cfg::B_BYTES);
-                        if (MODE == F8_GATE_UP) {
-                            f8_tma2(b_u, &P.tb, kb * 128, t.e * P.b_rec_rows + t.n0, bar);
-                            f8_tma2(b_u + 16384u, &P.tb, kb * 128, t.e * P.b_rec_rows + P.n + t.n0, bar);
-                        } else {
-                            f8_tma2(b_u, &P.tb, kb * 128, t.e * P.b_rec_rows + t.n0, bar);
-                        }
+                        if (rank == 0) fb_mbar_expect_tx(own, bytes);
+                        f8_tma2<PAIR>(b_u, &P.tb, kb * 128, y, bar);
+                        if (MODE == F8_GATE_UP && !PAIR) f8_tma2<PAIR>(b_u + 16384u, &P.tb, kb * 128, y + P.n, bar);
                     }
                     __syncwarp();
-                    if (lane < groups) {
-                        if (MODE == F8_GATE_UP) f8_gather4(a_u + lane * 512u, &P.ta, kb * 128, rows, bar);
-                        else f8_tma2(a_u + lane * 4096u, &P.ta, kb * 128, t.r0 + 32 * lane, bar);
-                    }
+                    if (lane < groups) f8_tma2<PAIR>(a_u + lane * 4096u, &P.ta, kb * 128, t.r0 + 128 * rank + 32 * lane, bar);
                 }
             }
             /* every stage's last commit has arrived before the block, and with it the barriers' memory, goes away */
             for (int i = 0; i < STAGES && ok; i++, step++)
                 ok = __all_sync(FULL, f8_wait(fb_smem_u32(&C->empty[step % STAGES]), ((step / STAGES) & 1) ^ 1, C));
-        } else if (warp == 9 && lane == 0) {
-            /* ---------------- MMAs: one thread */
-            const uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        } else if (warp == 9 && lane == 0 && rank == 0) {
+            /* ---------------- MMAs: one thread, in a pair one for both SMs */
+            const uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(cfg::ROWS >> 4) << 24);
             uint32_t step = 0;
             bool ok = true;
-            for (int it = blockIdx.x; it < tiles && ok; it += gridDim.x)
+            for (int it = first; it < tiles && ok; it += stride)
                 for (int kb = 0; kb < kbs; kb++, step++) {
                     const int s = step % STAGES, b = step % NB;
                     if (!f8_wait(fb_smem_u32(&C->acc_empty[b]), ((step / NB) & 1) ^ 1, C) ||
@@ -359,128 +433,137 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     const uint32_t a_u = dyn_u + s * cfg::STAGE, b_u = a_u + F8_A_BYTES;
 #pragma unroll
                     for (int q = 0; q < 4; q++)
-                        f8_mma(tmem + (uint32_t)(b * NT), f8_desc(a_u + 32 * q), f8_desc(b_u + 32 * q), idesc, q > 0);
-                    f8_commit(fb_smem_u32(&C->empty[s]));
-                    f8_commit(fb_smem_u32(&C->acc_full[b]));
+                        f8_mma<PAIR>(tmem + (uint32_t)(b * NT), f8_desc(a_u + 32 * q), f8_desc(b_u + 32 * q), idesc, q > 0);
+                    f8_commit<PAIR>(fb_smem_u32(&C->empty[s]));
+                    f8_commit<PAIR>(fb_smem_u32(&C->acc_full[b]));
                 }
+        } else if (warp >= 10) {
+            /* ---------------- scales: 64 threads, rows i and i + 64; asked for a group of blocks ahead.  (Read by the joining
+             * threads themselves they missed the L1 beside 200 KB of shared memory and cost an L2 latency every block.) */
+            const int i = tid - 320;
+            uint32_t g = 0;
+            bool ok = true;
+            for (int it = first; it < tiles && ok; it += stride) {
+                const f8_tile_t t = f8_tile<MODE, NT, PAIR>(P, it, n_tiles);
+                const float *a0 = P.a_scales + (int64_t)(t.r0 + min(128 * rank + i, t.rows - 1)) * P.as_stride;
+                const float *a1 = P.a_scales + (int64_t)(t.r0 + min(128 * rank + i + 64, t.rows - 1)) * P.as_stride;
+                const float *rec = P.b_scales + (int64_t)t.e * P.bs_rec;
+                const float *b0 = rec + (int64_t)(min(t.n0, P.n - 1) >> 7) * P.bs_stride;
+                const float *b1 = rec + (int64_t)((MODE == F8_GATE_UP ? P.n + t.n0 : min(t.n0 + NT / 2, P.n - 1)) >> 7) * P.bs_stride;
+                for (int kb = 0; kb < kbs; kb += F8_SC, g++) {
+                    float va[2][F8_SC], vb[2][F8_SC];
+#pragma unroll
+                    for (int q = 0; q < F8_SC; q++) {
+                        const int k = min(kb + q, kbs - 1);
+                        va[0][q] = __ldg(a0 + k);
+                        va[1][q] = __ldg(a1 + k);
+                        vb[0][q] = __ldg(b0 + k);
+                        vb[1][q] = __ldg(b1 + k);
+                    }
+                    ok = __all_sync(FULL, f8_wait(fb_smem_u32(&C->sc_empty[g & 1]), ((g >> 1) & 1) ^ 1, C));
+                    if (!ok) break;
+#pragma unroll
+                    for (int q = 0; q < F8_SC; q++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            C->scale[g & 1][q][h][i] = va[0][q] * vb[h][q];
+                            C->scale[g & 1][q][h][i + 64] = va[1][q] * vb[h][q];
+                        }
+                    __syncwarp();
+                    if (lane == 0) fb_mbar_arrive(fb_smem_u32(&C->sc_full[g & 1]));
+                }
+            }
         }
         __syncwarp();
     } else {
         if (NT == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         /* ---------------- join the blocks' sums: warp w reads lanes 32 (w % 4) .., warpgroup wg its half of the columns */
-        constexpr int W = NT / 2, CH = W / 16;
+        constexpr int W = NT / 2, CW = W < 64 ? W : 64;
         const int wg = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t t_row = tmem + ((uint32_t)(warp & 3) << 21);
-        uint32_t step = 0, cnt = 0;
+        uint32_t step = 0, cnt = 0, grp = 0;
         bool ok = true;
-        for (int it = blockIdx.x; it < tiles; it += gridDim.x, cnt++) {
-            const f8_tile_t t = f8_tile<MODE, NT>(P, it, n_tiles);
-            int sr = t.r0 + min(row, t.rows - 1); /* the row of the scales */
-            if (MODE == F8_GATE_UP) {
-                const int p = P.pairs[sr];
-                sr = p < P.n_routed ? p / P.top_k : p - P.n_routed;
-            }
-            const float *sa_p = P.a_scales + (int64_t)sr * P.as_stride;
+        for (int it = first; it < tiles; it += stride, cnt++) {
+            const f8_tile_t t = f8_tile<MODE, NT, PAIR>(P, it, n_tiles);
+            const int r0 = t.r0 + 128 * rank, rows = min(128, t.rows - 128 * rank); /* of this SM; a pair's second may have none */
             const int c0 = t.n0 + (MODE == F8_GATE_UP ? 0 : wg * W); /* first row of b of this thread's columns */
-            const float *sb_p = P.b_scales + (int64_t)t.e * P.bs_rec + (int64_t)(min(c0, P.n - 1) >> 7) * P.bs_stride;
-            const float *su_p = sb_p + (int64_t)(P.n >> 7) * P.bs_stride; /* gate/up: the up rows' */
             float2 acc[W / 2];
 #pragma unroll
             for (int i = 0; i < W / 2; i++) acc[i] = make_float2(0.0f, 0.0f);
-            float sa = __ldg(sa_p), sb = __ldg(sb_p), su = MODE == F8_GATE_UP ? __ldg(su_p) : 0.0f;
             for (int kb = 0; kb < kbs; kb++, step++) {
-                const int b = step % NB;
-                const float f0 = sa * sb, f1 = MODE == F8_GATE_UP ? sa * su : f0;
-                if (kb + 1 < kbs) { /* asked for before the wait */
-                    sa = __ldg(sa_p + kb + 1);
-                    sb = __ldg(sb_p + kb + 1);
-                    if (MODE == F8_GATE_UP) su = __ldg(su_p + kb + 1);
+                const int b = step % NB, q = kb % F8_SC;
+                if (ok && q == 0) ok = __all_sync(FULL, f8_wait(fb_smem_u32(&C->sc_full[grp & 1]), (grp >> 1) & 1, C));
+                const float f0 = C->scale[grp & 1][q][MODE == F8_GATE_UP ? 0 : wg][row];
+                const float f1 = MODE == F8_GATE_UP ? C->scale[grp & 1][q][1][row] : f0;
+                if (q == F8_SC - 1 || kb == kbs - 1) {
+                    __syncwarp();
+                    if (ok && lane == 0) fb_mbar_arrive(fb_smem_u32(&C->sc_empty[grp & 1]));
+                    grp++;
                 }
                 if (ok) ok = __all_sync(FULL, f8_wait(fb_smem_u32(&C->acc_full[b]), (step / NB) & 1, C));
                 if (!ok) continue;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t r[2][16];
                 const uint32_t tc = t_row + (uint32_t)(b * NT);
-                /* chunk c of the thread's columns: gate/up takes half of them from the gate's columns, half from the up's */
-#define F8_COL(c) (uint32_t)(MODE == F8_GATE_UP ? ((c) < CH / 2 ? wg * (W / 2) + 16 * (c) : NT / 2 + wg * (W / 2) + 16 * ((c) - CH / 2)) : wg * W + 16 * (c))
-                f8_tmem_ld16(tc + F8_COL(0), r[0]);
+                /* chunk c of the thread's columns (gate/up: the gate's, then the up's) */
 #pragma unroll
-                for (int c = 0; c < CH; c++) {
-                    f8_tmem_wait(r[c & 1]);
-                    if (c + 1 < CH) {
-                        f8_tmem_ld16(tc + F8_COL(c + 1), r[(c + 1) & 1]);
-                    } else { /* the buffer has been read: the next block's MMAs may have it */
+                for (int c = 0; c < W / CW; c++) {
+                    uint32_t r[CW];
+                    const uint32_t col = tc + (uint32_t)(MODE == F8_GATE_UP ? c * (NT / 2) + wg * CW : wg * W + c * CW);
+                    f8_tmem_ld32(col, r);
+                    if (CW > 32) f8_tmem_ld32(col + 32, r + CW - 32);
+                    f8_tmem_wait(r);
+                    if (CW > 32) f8_tmem_wait(r + CW - 32);
+                    if (c == W / CW - 1) { /* the buffer has been read: the next block's MMAs may have it */
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) fb_mbar_arrive(fb_smem_u32(&C->acc_empty[b]));
+                        if (lane == 0) {
+                            const uint32_t bar = fb_smem_u32(&C->acc_empty[b]);
+                            if (PAIR)
+                                asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(f8_leader(bar)) : "memory");
+                            else
+                                fb_mbar_arrive(bar);
+                        }
                     }
-                    const float f = MODE == F8_GATE_UP && c >= CH / 2 ? f1 : f0;
+                    const float f = c ? f1 : f0;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) f8_fma2(acc[8 * c + i], r[c & 1][2 * i], r[c & 1][2 * i + 1], f);
+                    for (int i = 0; i < CW / 2; i++) f8_fma2(acc[c * (CW / 2) + i], r[2 * i], r[2 * i + 1], f);
                 }
             }
+            const uint32_t buf = out_u + warp * 2048u;
             if (MODE == F8_GATE_UP) {
                 /* silu(g) u of this thread's 64 columns, and the amax over the row's 128 with the other warpgroup's */
                 float amax = 0.0f;
 #pragma unroll
                 for (int i = 0; i < W / 4; i++) {
-                    const float2 g = acc[i], u = acc[W / 4 + i];
-                    acc[i].x = g.x / (1.0f + expf(-g.x)) * u.x;
-                    acc[i].y = g.y / (1.0f + expf(-g.y)) * u.y;
+                    acc[i].x = f8_silu_mul(acc[i].x, acc[W / 4 + i].x);
+                    acc[i].y = f8_silu_mul(acc[i].y, acc[W / 4 + i].y);
                     amax = ops_amax(ops_amax(amax, acc[i].x), acc[i].y);
                 }
                 C->amax[cnt & 1][wg][row] = amax;
                 asm volatile("bar.sync 1, 256;" ::: "memory"); /* the 8 warps meet once a tile, also after a wait that ran out */
                 const float sc = ops_f8_scale(ops_amax(amax, C->amax[cnt & 1][wg ^ 1][row]));
-                if (row < t.rows && ok) {
-                    uint4 *q = reinterpret_cast<uint4 *>(P.act_q + (int64_t)(t.r0 + row) * P.n + t.n0 + wg * 64);
+                const float inv = __frcp_rn(sc); /* (the values carry a few roundings already: one more, of the quotient, is theirs) */
+                const bool mine = row < rows && ok;
+                uint32_t w[16];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        uint32_t w[4];
+                for (int i = 0; i < 16; i++)
+                    w[i] = ops_f8_pack4(acc[2 * i].x * inv, acc[2 * i].y * inv, acc[2 * i + 1].x * inv, acc[2 * i + 1].y * inv);
+                f8_rows_out<64>(buf, w, mine ? P.act_q + (int64_t)(r0 + row) * P.n + t.n0 + wg * 64 : nullptr, 64, 1, 4);
+                if (mine && wg == 0) P.act_scales[(int64_t)(r0 + row) * (P.n >> 7) + (t.n0 >> 7)] = sc;
+            } else {
+                const bool mine = row < rows && ok;
+                const int64_t o = mine ? (int64_t)(MODE == F8_DOWN ? P.pairs[r0 + row] : r0 + row) * P.out_stride + c0 : 0;
+                if (MODE == F8_DENSE && P.out_bf16) {
+                    uint32_t w[W / 2];
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            w[i] = ops_f8_pack4(__fdiv_rn(acc[8 * j + 2 * i].x, sc), __fdiv_rn(acc[8 * j + 2 * i].y, sc),
-                                                __fdiv_rn(acc[8 * j + 2 * i + 1].x, sc), __fdiv_rn(acc[8 * j + 2 * i + 1].y, sc));
-                        q[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int i = 0; i < W / 2; i++) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(acc[i].x, acc[i].y);
+                        w[i] = *reinterpret_cast<const uint32_t *>(&h);
                     }
-                    if (wg == 0) P.act_scales[(int64_t)(t.r0 + row) * (P.n >> 7) + (t.n0 >> 7)] = sc;
-                }
-            } else if (row < t.rows && ok) {
-                const int64_t o = (int64_t)(MODE == F8_DOWN ? P.pairs[t.r0 + row] : t.r0 + row) * P.out_stride + c0;
-                const int left = P.n - c0;
-                if (P.out_bf16) {
-                    __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(P.out) + o;
-#pragma unroll
-                    for (int j = 0; j < W / 8; j++) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const __nv_bfloat162 h = __floats2bfloat162_rn(acc[4 * j + i].x, acc[4 * j + i].y);
-                            w[i] = *reinterpret_cast<const uint32_t *>(&h);
-                        }
-                        if (P.out_vec && 8 * j + 8 <= left) {
-                            *reinterpret_cast<uint4 *>(out + 8 * j) = make_uint4(w[0], w[1], w[2], w[3]);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 8; i++)
-                                if (8 * j + i < left)
-                                    reinterpret_cast<uint16_t *>(out)[8 * j + i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-                        }
-                    }
+                    f8_rows_out<W * 2>(buf, w, mine ? reinterpret_cast<uint8_t *>(P.out) + 2 * o : nullptr, 2 * (P.n - c0), P.out_vec, 2);
                 } else {
-                    float *out = reinterpret_cast<float *>(P.out) + o;
-#pragma unroll
-                    for (int j = 0; j < W / 4; j++) {
-                        const float4 v = make_float4(acc[2 * j].x, acc[2 * j].y, acc[2 * j + 1].x, acc[2 * j + 1].y);
-                        if (P.out_vec && 4 * j + 4 <= left) {
-                            *reinterpret_cast<float4 *>(out + 4 * j) = v;
-                        } else {
-                            if (4 * j < left) out[4 * j] = v.x;
-                            if (4 * j + 1 < left) out[4 * j + 1] = v.y;
-                            if (4 * j + 2 < left) out[4 * j + 2] = v.z;
-                            if (4 * j + 3 < left) out[4 * j + 3] = v.w;
-                        }
-                    }
+                    f8_rows_out<W * 4>(buf, reinterpret_cast<const uint32_t *>(acc),
+                                       mine ? reinterpret_cast<uint8_t *>(P.out) + 4 * o : nullptr, 4 * (P.n - c0), P.out_vec, 4);
                 }
             }
         }
@@ -491,10 +574,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
     if (C->abort_flag) {
         if (tid == 0) *P.status = FB_ST_WAIT_TIMEOUT;
         for (int i = 0; i < 100; i++) __nanosleep(1000); /* copies and MMAs under way land before their memory is released */
-        __syncthreads();
     }
-    if (warp == 9)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(NB * NT)) : "memory");
+    if (PAIR) f8_cluster_sync(); /* neither SM goes while the other's MMAs or arrivals may reach it */
+    if (warp == 9) {
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(NB * NT)) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(NB * NT)) : "memory");
+    }
 }
 
 /* ------------------------------------------------------------------ tensor maps */
@@ -514,12 +599,23 @@ static int f8_map(CUtensorMap *m, const void *p, uint64_t k, uint64_t rows, uint
                : (int)cudaErrorInvalidValue;
 }
 
-template <int MODE, int NT>
+template <int MODE, int NT, bool PAIR>
 static int f8_launch(f8_args_t &p, int64_t most_tiles, int n_sm, int *launches, cudaStream_t st) {
-    const int grid = (int)(most_tiles < n_sm ? most_tiles : n_sm);
-    k_f8_mma<MODE, NT><<<grid, F8_THREADS, f8_cfg<MODE, NT>::SMEM, st>>>(p);
+    cudaLaunchConfig_t c = {};
+    cudaLaunchAttribute at[1];
+    const int64_t want = PAIR ? 2 * most_tiles : most_tiles;
+    c.gridDim = dim3((unsigned)(want < n_sm ? want : PAIR ? n_sm & ~1 : n_sm));
+    c.blockDim = dim3(F8_THREADS);
+    c.dynamicSmemBytes = f8_cfg<MODE, NT, PAIR>::SMEM;
+    c.stream = st;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = PAIR ? 2 : 1;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    c.attrs = at;
+    c.numAttrs = 1;
     *launches += 1;
-    return (int)cudaGetLastError();
+    const cudaError_t rc = cudaLaunchKernelEx(&c, k_f8_mma<MODE, NT, PAIR>, p);
+    return (int)(rc != cudaSuccess ? rc : cudaGetLastError());
 }
 
 extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *status, int n_sm, int *launches,
@@ -531,16 +627,32 @@ extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *s
     p.out = a->out, p.out_bf16 = a->out_type == FOMOE_B200_BF16, p.out_stride = a->out_stride;
     p.out_vec = ((uintptr_t)a->out & 15) == 0 && (a->out_stride * (p.out_bf16 ? 2 : 4)) % 16 == 0;
     p.status = status;
-    /* columns of a tile: 256 keep the tensor cores' operand traffic lowest; fewer when that would leave SMs without one */
-    const int64_t mt = (a->m + 127) / 128;
-    const int nt = mt * ((a->n + 255) / 256) >= n_sm ? 256 : mt * ((a->n + 127) / 128) >= n_sm ? 128 : 64;
-    int rc = f8_map(&p.ta, a->a, a->k, a->m, a->a_stride, 32) | f8_map(&p.tb, a->b, a->k, a->n, a->b_stride, nt);
-    if (rc) return rc;
-    const int64_t tiles = mt * ((a->n + nt - 1) / nt);
     cudaStream_t st = (cudaStream_t)stream;
-    return nt == 256   ? f8_launch<F8_DENSE, 256>(p, tiles, n_sm, launches, st)
-           : nt == 128 ? f8_launch<F8_DENSE, 128>(p, tiles, n_sm, launches, st)
-                       : f8_launch<F8_DENSE, 64>(p, tiles, n_sm, launches, st);
+    const int64_t m = a->m, n = a->n, mt = (m + 127) / 128;
+    /* the largest tile that still gives every SM one: two SMs a tile of 256 x 256 read least, then fewer columns */
+    const int64_t pairs = ((m + 255) / 256) * ((n + 255) / 256);
+    const bool pair = 2 * pairs >= n_sm;
+    const int nt = pair ? 256 : mt * ((n + 127) / 128) >= n_sm ? 128 : 64;
+    const int rc = f8_map(&p.ta, a->a, a->k, a->m, a->a_stride, 32) | f8_map(&p.tb, a->b, a->k, a->n, a->b_stride, pair ? 128 : nt);
+    if (rc) return rc;
+    return pair        ? f8_launch<F8_DENSE, 256, true>(p, pairs, n_sm, launches, st)
+           : nt == 128 ? f8_launch<F8_DENSE, 128, false>(p, mt * ((n + 127) / 128), n_sm, launches, st)
+                       : f8_launch<F8_DENSE, 64, false>(p, mt * ((n + 63) / 64), n_sm, launches, st);
+}
+
+/* ------------------------------------------------------------------ the pairs' rows of x side by side: one warp a row
+ * so that the products' operand tiles are plain boxes (fetching 128 scattered rows as 32 gathers a stage took 2.7
+ * thousand cycles a stage, five times the MMAs). */
+__global__ void __launch_bounds__(256) k_ops_permute(const uint8_t *x, int64_t x_stride, const float *xs, int64_t xs_stride, int H,
+                                                     const int *counts, const int *pairs, int n_routed, int top_k, int n_shared,
+                                                     uint8_t *xp, float *xps) {
+    const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (r >= counts[1] + n_shared) return;
+    const int p = pairs[r], t = p < n_routed ? p / top_k : p - n_routed;
+    const uint4 *src = reinterpret_cast<const uint4 *>(x + t * x_stride);
+    uint4 *dst = reinterpret_cast<uint4 *>(xp + (int64_t)r * H);
+    for (int i = lane; i < H / 16; i += 32) dst[i] = __ldg(src + i);
+    for (int i = lane; i < H / 128; i += 32) xps[(int64_t)r * (H / 128) + i] = __ldg(xs + t * xs_stride + i);
 }
 
 /* ------------------------------------------------------------------ out[t] = sum over the slots, in slot order */
@@ -565,8 +677,10 @@ extern "C" void ops_experts_layout(const fomoe_b200_f8_experts_args_t *a, ops_ex
     uint64_t at = 0;
 #define PART(name, n) w->name = at, at += ((uint64_t)(n) + 255) & ~255ull
     w->n_pairs = (int)np;
-    PART(counts, 256 + 16 * items); /* {tiles, pairs}, then the tiles */
+    PART(counts, 256 + 16 * items); /* {tiles, routed pairs}, then the tiles */
     PART(pairs, 4 * np);
+    PART(xp, np * a->n_embd);
+    PART(xp_scales, np * (a->n_embd / 128) * 4);
     PART(act_q, np * a->n_inter);
     PART(act_scales, np * (a->n_inter / 128) * 4);
     PART(dots, np * a->n_embd * 4);
@@ -579,31 +693,41 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     cudaStream_t st = (cudaStream_t)stream;
     ops_experts_ws_t w;
     ops_experts_layout(a, &w);
-    const int n_routed = a->n_tokens * a->top_k, H = a->n_embd, I = a->n_inter;
+    const int n_routed = a->n_tokens * a->top_k, n_shared = a->has_shared ? a->n_tokens : 0, H = a->n_embd, I = a->n_inter;
     int *counts = (int *)(ws + w.counts), *pairs = (int *)(ws + w.pairs);
     int4 *items = (int4 *)(ws + w.counts + 256);
-    k_ops_bucket<<<1, BK_THREADS, (size_t)a->n_experts * BK_WARPS * 4, st>>>(a->ids, n_routed, a->n_tokens, a->n_experts,
-                                                                            a->has_shared, counts, pairs, items, status);
-    *launches += 1;
+    /* two SMs a tile of 256 rows once the experts have that many rows to fill it; until then the weights' bytes decide */
+    const int64_t recs = a->n_experts + (a->has_shared ? 1 : 0);
+    const bool pair = w.n_pairs >= 192 * recs;
+    const int tile = pair ? 256 : 128;
+    k_ops_bucket<<<1, BK_THREADS, (size_t)a->n_experts * BK_WARPS * 4, st>>>(
+        a->ids, n_routed, a->n_tokens, a->n_experts, a->has_shared, tile, counts, pairs, items, status);
+    k_ops_permute<<<(w.n_pairs + 7) / 8, 256, 0, st>>>(a->x, a->x_stride, a->x_scales, a->x_scales_stride, H, counts, pairs,
+                                                      n_routed, a->top_k, n_shared, ws + w.xp, (float *)(ws + w.xp_scales));
+    *launches += 2;
     int rc = (int)cudaGetLastError();
     if (rc) return rc;
-    /* a tile of pairs holds at most 128 of one expert: no more tiles than this (the device knows how many there are) */
-    const int64_t tiles = w.n_pairs / 128 + a->n_experts + 1, recs = a->n_experts + (a->has_shared ? 1 : 0);
+    /* no more tiles than this (the device knows how many there are) */
+    const int64_t tiles = w.n_pairs / tile + recs;
     f8_args_t p = {};
-    p.counts = counts, p.pairs = pairs, p.items = items, p.n_routed = n_routed, p.top_k = a->top_k, p.status = status;
+    p.counts = counts, p.pairs = pairs, p.items = items, p.status = status;
     p.n = I, p.k = H;
-    p.a_scales = a->x_scales, p.as_stride = a->x_scales_stride;
+    p.a_scales = (const float *)(ws + w.xp_scales), p.as_stride = H / 128;
     p.b_scales = a->gate_up_scales, p.bs_stride = H / 128, p.bs_rec = (int64_t)(2 * I / 128) * (H / 128), p.b_rec_rows = 2 * I;
     p.act_q = ws + w.act_q, p.act_scales = (float *)(ws + w.act_scales);
-    rc = f8_map(&p.ta, a->x, H, a->n_tokens, a->x_stride, 1) | f8_map(&p.tb, a->gate_up, H, recs * 2 * I, H, 128);
-    if (!rc) rc = f8_launch<F8_GATE_UP, 256>(p, tiles * (I / 128), n_sm, launches, st);
+    rc = f8_map(&p.ta, ws + w.xp, H, w.n_pairs, H, 32) | f8_map(&p.tb, a->gate_up, H, recs * 2 * I, H, 128);
+    if (!rc)
+        rc = pair ? f8_launch<F8_GATE_UP, 256, true>(p, tiles * (I / 128), n_sm, launches, st)
+                  : f8_launch<F8_GATE_UP, 256, false>(p, tiles * (I / 128), n_sm, launches, st);
     if (rc) return rc;
     p.n = H, p.k = I;
     p.a_scales = p.act_scales, p.as_stride = I / 128;
     p.b_scales = a->down_scales, p.bs_stride = I / 128, p.bs_rec = (int64_t)(H / 128) * (I / 128), p.b_rec_rows = H;
     p.out = ws + w.dots, p.out_stride = H, p.out_vec = 1;
-    rc = f8_map(&p.ta, ws + w.act_q, I, w.n_pairs, I, 32) | f8_map(&p.tb, a->down, I, recs * H, I, 256);
-    if (!rc) rc = f8_launch<F8_DOWN, 256>(p, tiles * ((H + 255) / 256), n_sm, launches, st);
+    rc = f8_map(&p.ta, ws + w.act_q, I, w.n_pairs, I, 32) | f8_map(&p.tb, a->down, I, recs * H, I, pair ? 128 : 256);
+    if (!rc)
+        rc = pair ? f8_launch<F8_DOWN, 256, true>(p, tiles * ((H + 255) / 256), n_sm, launches, st)
+                  : f8_launch<F8_DOWN, 256, false>(p, tiles * ((H + 255) / 256), n_sm, launches, st);
     if (rc) return rc;
     k_ops_combine<<<a->n_tokens, 256, 0, st>>>((const float *)(ws + w.dots), a->ids, a->weights, H, a->n_experts, a->top_k,
                                               n_routed, a->has_shared, (__nv_bfloat16 *)a->out, a->out_stride);
@@ -623,10 +747,12 @@ extern "C" int ops_f8_init(void) {
         f8_encode = (f8_encode_t)fn;
     }
 #define RK(k) rc |= (int)cudaFuncGetAttributes(&f, (k))
-#define RM(MODE, NT) \
-    rc |= (int)cudaFuncSetAttribute(k_f8_mma<MODE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, f8_cfg<MODE, NT>::SMEM)
-    RK(k_ops_combine); RK(k_ops_bucket);
-    RM(F8_DENSE, 256); RM(F8_DENSE, 128); RM(F8_DENSE, 64); RM(F8_GATE_UP, 256); RM(F8_DOWN, 256);
+#define RM(MODE, NT, PAIR)                                                                                        \
+    rc |= (int)cudaFuncSetAttribute(k_f8_mma<MODE, NT, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
+                                    f8_cfg<MODE, NT, PAIR>::SMEM)
+    RK(k_ops_combine); RK(k_ops_bucket); RK(k_ops_permute);
+    RM(F8_DENSE, 256, true); RM(F8_DENSE, 128, false); RM(F8_DENSE, 64, false);
+    RM(F8_GATE_UP, 256, true); RM(F8_GATE_UP, 256, false); RM(F8_DOWN, 256, true); RM(F8_DOWN, 256, false);
 #undef RM
 #undef RK
     rc |= (int)cudaFuncSetAttribute(k_ops_bucket, cudaFuncAttributeMaxDynamicSharedMemorySize, OPS_MAX_E * BK_WARPS * 4);
