@@ -168,6 +168,39 @@ __device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, f8_ctl_t 
     return false;
 }
 
+/* one look, whose answer may be used later: on a busy SM it takes a quarter of a thousand cycles to come back */
+__device__ __forceinline__ uint32_t f8_look(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok;
+}
+
+__device__ __forceinline__ bool f8_wait_all(uint32_t bar, uint32_t parity, f8_ctl_t *C) {
+    return __all_sync(FULL, f8_wait(bar, parity, C));
+}
+
+/* one lane of a converged warp: the instructions that take warp-uniform operands (tcgen05, TMA) are issued under it; under
+ * `lane == 0` the compiler does not know them to be uniform, and the issue of a block's MMAs took 460 cycles */
+__device__ __forceinline__ bool f8_elect() {
+    uint32_t p;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "elect.sync _|p, 0xffffffff;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(p));
+    return p != 0;
+}
+
 /* shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row groups 1024 bytes apart */
 __device__ __forceinline__ uint64_t f8_desc(uint32_t saddr) {
     return (uint64_t)((saddr & 0x3ffffu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1 << 46) |
@@ -388,54 +421,74 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
         if (NT == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 8) {
             /* ---------------- operand tiles */
-            uint32_t step = 0;
+            uint32_t st = 0, ph = 0; /* stage, and the parity of its phase */
             bool ok = true;
             for (int it = first; it < tiles && ok; it += stride) {
                 const f8_tile_t t = f8_tile<MODE, NT, PAIR>(P, it, n_tiles);
                 /* boxes of 32 rows, as many as this SM's rows need; what is behind the tile's rows is never stored */
-                const int groups = min(4, max(0, (t.rows - 128 * rank + 31) / 32));
+                const int groups = min(4, max(0, (t.rows - 128 * rank + 31) / 32)), y0 = t.r0 + 128 * rank;
                 const int y = t.e * P.b_rec_rows + (MODE == F8_GATE_UP && rank ? P.n + t.n0 : t.n0 + (PAIR ? NT / 2 * rank : 0));
                 const uint32_t bytes = (uint32_t)((t.rows + 31) / 32) * 4096u + (PAIR ? 2u : 1u) * cfg::B_BYTES; /* of both SMs */
-                for (int kb = 0; kb < kbs; kb++, step++) {
-                    const int s = step % STAGES;
-                    const uint32_t a_u = dyn_u + s * cfg::STAGE, b_u = a_u + F8_A_BYTES;
-                    if (!__all_sync(FULL, f8_wait(fb_smem_u32(&C->empty[s]), ((step / STAGES) & 1) ^ 1, C))) {
+                for (int kb = 0; kb < kbs; kb++) {
+                    const uint32_t a_u = dyn_u + st * cfg::STAGE, b_u = a_u + F8_A_BYTES;
+                    if (!f8_wait_all(fb_smem_u32(&C->empty[st]), ph ^ 1, C)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t own = fb_smem_u32(&C->full[s]), bar = PAIR ? f8_leader(own) : own;
-                    if (lane == 0) {
+                    if (f8_elect()) {
+                        const uint32_t own = fb_smem_u32(&C->full[st]), bar = PAIR ? f8_leader(own) : own;
                         if (rank == 0) fb_mbar_expect_tx(own, bytes);
                         f8_tma2<PAIR>(b_u, &P.tb, kb * 128, y, bar);
                         if (MODE == F8_GATE_UP && !PAIR) f8_tma2<PAIR>(b_u + 16384u, &P.tb, kb * 128, y + P.n, bar);
+                        for (int g = 0; g < groups; g++) f8_tma2<PAIR>(a_u + g * 4096u, &P.ta, kb * 128, y0 + 32 * g, bar);
                     }
                     __syncwarp();
-                    if (lane < groups) f8_tma2<PAIR>(a_u + lane * 4096u, &P.ta, kb * 128, t.r0 + 128 * rank + 32 * lane, bar);
+                    if (++st == STAGES) {
+                        st = 0;
+                        ph ^= 1;
+                    }
                 }
             }
             /* every stage's last commit has arrived before the block, and with it the barriers' memory, goes away */
-            for (int i = 0; i < STAGES && ok; i++, step++)
-                ok = __all_sync(FULL, f8_wait(fb_smem_u32(&C->empty[step % STAGES]), ((step / STAGES) & 1) ^ 1, C));
-        } else if (warp == 9 && lane == 0 && rank == 0) {
+            for (int i = 0; i < STAGES && ok; i++) {
+                ok = f8_wait_all(fb_smem_u32(&C->empty[st]), ph ^ 1, C);
+                if (++st == STAGES) {
+                    st = 0;
+                    ph ^= 1;
+                }
+            }
+        } else if (warp == 9 && rank == 0) {
             /* ---------------- MMAs: one thread, in a pair one for both SMs */
             const uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(cfg::ROWS >> 4) << 24);
-            uint32_t step = 0;
+            uint32_t st = 0, ph = 0, b = 0, bph = 0, have_ab = 0, have_acc = 0;
             bool ok = true;
             for (int it = first; it < tiles && ok; it += stride)
-                for (int kb = 0; kb < kbs; kb++, step++) {
-                    const int s = step % STAGES, b = step % NB;
-                    if (!f8_wait(fb_smem_u32(&C->acc_empty[b]), ((step / NB) & 1) ^ 1, C) ||
-                        !f8_wait(fb_smem_u32(&C->full[s]), (step / STAGES) & 1, C)) {
+                for (int kb = 0; kb < kbs; kb++) {
+                    if ((!__all_sync(FULL, have_ab) && !f8_wait_all(fb_smem_u32(&C->full[st]), ph, C)) ||
+                        (!__all_sync(FULL, have_acc) && !f8_wait_all(fb_smem_u32(&C->acc_empty[b]), bph ^ 1, C))) {
                         ok = false;
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t a_u = dyn_u + s * cfg::STAGE, b_u = a_u + F8_A_BYTES;
+                    const uint32_t a_u = dyn_u + st * cfg::STAGE, b_u = a_u + F8_A_BYTES;
+                    if (f8_elect()) {
 #pragma unroll
-                    for (int q = 0; q < 4; q++)
-                        f8_mma<PAIR>(tmem + (uint32_t)(b * NT), f8_desc(a_u + 32 * q), f8_desc(b_u + 32 * q), idesc, q > 0);
-                    f8_commit<PAIR>(fb_smem_u32(&C->empty[s]));
-                    f8_commit<PAIR>(fb_smem_u32(&C->acc_full[b]));
+                        for (int q = 0; q < 4; q++)
+                            f8_mma<PAIR>(tmem + b * NT, f8_desc(a_u + 32 * q), f8_desc(b_u + 32 * q), idesc, q > 0);
+                        f8_commit<PAIR>(fb_smem_u32(&C->acc_full[b]));
+                        f8_commit<PAIR>(fb_smem_u32(&C->empty[st]));
+                    }
+                    __syncwarp();
+                    if (++st == STAGES) {
+                        st = 0;
+                        ph ^= 1;
+                    }
+                    if (++b == NB) {
+                        b = 0;
+                        bph ^= 1;
+                    }
+                    have_ab = f8_look(fb_smem_u32(&C->full[st]), ph);
+                    have_acc = f8_look(fb_smem_u32(&C->acc_empty[b]), bph ^ 1);
                 }
         } else if (warp >= 10) {
             /* ---------------- scales: 64 threads, rows i and i + 64; asked for a group of blocks ahead.  (Read by the joining
@@ -460,7 +513,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                         vb[0][q] = __ldg(b0 + k);
                         vb[1][q] = __ldg(b1 + k);
                     }
-                    ok = __all_sync(FULL, f8_wait(fb_smem_u32(&C->sc_empty[g & 1]), ((g >> 1) & 1) ^ 1, C));
+                    ok = f8_wait_all(fb_smem_u32(&C->sc_empty[g & 1]), ((g >> 1) & 1) ^ 1, C);
                     if (!ok) break;
 #pragma unroll
                     for (int q = 0; q < F8_SC; q++)
@@ -481,7 +534,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
         constexpr int W = NT / 2, CW = W < 64 ? W : 64;
         const int wg = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t t_row = tmem + ((uint32_t)(warp & 3) << 21);
-        uint32_t step = 0, cnt = 0, grp = 0;
+        uint32_t step = 0, cnt = 0, grp = 0, have = 0;
         bool ok = true;
         for (int it = first; it < tiles; it += stride, cnt++) {
             const f8_tile_t t = f8_tile<MODE, NT, PAIR>(P, it, n_tiles);
@@ -490,17 +543,25 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             float2 acc[W / 2];
 #pragma unroll
             for (int i = 0; i < W / 2; i++) acc[i] = make_float2(0.0f, 0.0f);
+            /* the group's scales have come: this block's factors; the last block of a group gives the group back */
+#define F8_FACTORS(kb)                                                                               \
+    do {                                                                                             \
+        const int q_ = (kb) % F8_SC;                                                                 \
+        if (ok && q_ == 0) ok = f8_wait_all(fb_smem_u32(&C->sc_full[grp & 1]), (grp >> 1) & 1, C);   \
+        n0 = C->scale[grp & 1][q_][MODE == F8_GATE_UP ? 0 : wg][row];                                \
+        if (MODE == F8_GATE_UP) n1 = C->scale[grp & 1][q_][1][row];                                  \
+        if (q_ == F8_SC - 1 || (kb) == kbs - 1) {                                                    \
+            __syncwarp();                                                                            \
+            if (ok && lane == 0) fb_mbar_arrive(fb_smem_u32(&C->sc_empty[grp & 1]));                 \
+            grp++;                                                                                   \
+        }                                                                                            \
+    } while (0)
+            float n0, n1 = 0.0f;
+            F8_FACTORS(0);
             for (int kb = 0; kb < kbs; kb++, step++) {
-                const int b = step % NB, q = kb % F8_SC;
-                if (ok && q == 0) ok = __all_sync(FULL, f8_wait(fb_smem_u32(&C->sc_full[grp & 1]), (grp >> 1) & 1, C));
-                const float f0 = C->scale[grp & 1][q][MODE == F8_GATE_UP ? 0 : wg][row];
-                const float f1 = MODE == F8_GATE_UP ? C->scale[grp & 1][q][1][row] : f0;
-                if (q == F8_SC - 1 || kb == kbs - 1) {
-                    __syncwarp();
-                    if (ok && lane == 0) fb_mbar_arrive(fb_smem_u32(&C->sc_empty[grp & 1]));
-                    grp++;
-                }
-                if (ok) ok = __all_sync(FULL, f8_wait(fb_smem_u32(&C->acc_full[b]), (step / NB) & 1, C));
+                const int b = step % NB;
+                const float f0 = n0, f1 = MODE == F8_GATE_UP ? n1 : n0;
+                if (ok && !__all_sync(FULL, have)) ok = f8_wait_all(fb_smem_u32(&C->acc_full[b]), (step / NB) & 1, C);
                 if (!ok) continue;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t tc = t_row + (uint32_t)(b * NT);
@@ -523,6 +584,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                             else
                                 fb_mbar_arrive(bar);
                         }
+                        /* the next block's barrier and factors are asked for before this block's products */
+                        have = f8_look(fb_smem_u32(&C->acc_full[(step + 1) % NB]), ((step + 1) / NB) & 1);
+                        if (kb + 1 < kbs) F8_FACTORS(kb + 1);
                     }
                     const float f = c ? f1 : f0;
 #pragma unroll
