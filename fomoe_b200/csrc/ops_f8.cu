@@ -26,8 +26,8 @@
 #define BK_WARPS 32
 
 __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n_routed, int n_tokens, int n_experts,
-                                                          int has_shared, int tile, int *counts, int *pairs,
-                                                          int4 *items, int *status) {
+                                                          int has_shared, int *counts, int *pairs, int4 *items,
+                                                          int *status) {
     extern __shared__ int s_cnt[]; /* [n_experts][BK_WARPS] */
     __shared__ int s_tot[BK_WARPS], s_til[BK_WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -54,11 +54,11 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
         }
         if (pass == 1) break;
         __syncthreads();
-        /* thread e: the expert's total, then exclusive prefixes of pairs and of tiles (`tile` rows) over the experts */
+        /* thread e: the expert's total, then exclusive prefixes of pairs and of 128-row tiles over the experts */
         int tot = 0;
         if (tid < n_experts)
             for (int w = 0; w < BK_WARPS; w++) tot += s_cnt[tid * BK_WARPS + ((w + tid) & 31)];
-        const int til = (tot + tile - 1) / tile;
+        const int til = (tot + 127) / 128;
         int a = tot, c = til;
         for (int s = 1; s < 32; s <<= 1) {
             const int oa = __shfl_up_sync(FULL, a, s), oc = __shfl_up_sync(FULL, c, s);
@@ -84,12 +84,12 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
                 s_cnt[tid * BK_WARPS + w] = at;
                 at += n;
             }
-            for (int m = 0; m < til; m++) items[tbase + m] = make_int4(tid, base + tile * m, min(tile, tot - tile * m), 0);
+            for (int m = 0; m < til; m++) items[tbase + m] = make_int4(tid, base + 128 * m, min(128, tot - 128 * m), 0);
         }
         if (tid == BK_THREADS - 1) { /* no expert's thread: n_experts <= 512 */
-            const int sh = has_shared ? (n_tokens + tile - 1) / tile : 0;
+            const int sh = has_shared ? (n_tokens + 127) / 128 : 0;
             for (int m = 0; m < sh; m++)
-                items[tbase + m] = make_int4(n_experts, base + tile * m, min(tile, n_tokens - tile * m), 0);
+                items[tbase + m] = make_int4(n_experts, base + 128 * m, min(128, n_tokens - 128 * m), 0);
             counts[0] = tbase + sh; /* tiles */
             counts[1] = base;       /* routed pairs that are left */
         }
@@ -110,13 +110,16 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
  * one factor for all of its columns.
  *
  * Persistent blocks, one per SM, warp-specialised: warp 8 asks for the operand tiles (TMA, 128-byte swizzle, one block of
- * 128 k a stage), one thread of warp 9 issues the MMAs (NT columns), warps 0..7 are two warpgroups that each join half of
- * the columns.  Tensor memory holds NB buffers of NT columns, so the MMAs of the next block run while this one's sums are
- * joined.
+ * 128 k a stage), one thread of warp 9 issues the MMAs (M = 128 rows, NT columns), warps 10 and 11 bring the scales, and
+ * warps 0..7 are two warpgroups that each join half of the columns.  Tensor memory holds NB buffers of NT columns, so the
+ * MMAs of the next block run while this one's sums are joined.
  *
- * PAIR: two SMs work on one tile of 256 rows x 256 columns (cta_group::2).  Each loads its own 128 rows and half of the
- * columns' weights, 32 KB a block of k instead of 48 KB for the same MMAs: with one SM a tile the kernel ran at the L2's
- * bandwidth (4096 x 8192 x 4096: 11.8 TB/s, the tensor cores 45 % busy).
+ * What bounds it (4096 x 8192 x 4096, 148 us, 1.85 PFLOP/s): the MMAs with nothing but their barriers take 121 us -- the
+ * operands of 128 x 256 tiles pass shared memory twice, 192 bytes a cycle at the tensor cores' full rate --, the joining
+ * FMAs 13 us more and the way out 14 us.  Two SMs a tile of 256 x 256 (cta_group::2: two thirds of the operand bytes) came
+ * to 147 us, with more padding for the experts (1.81 against 1.76 ms): its hand-overs between the SMs cost what the bytes
+ * saved.  Handing the columns over in two halves (180 us) and 16 joining warps (158 us) were slower: every barrier is
+ * shared-memory traffic too.
  *
  *   dense    A: rows of a;                               B: rows of b;                        D to out
  *   gate/up  A: the tokens of an expert's pairs;         B: 128 gate rows, 128 up rows;       silu(g) u to FP8, 128 a block
@@ -207,62 +210,27 @@ __device__ __forceinline__ uint64_t f8_desc(uint32_t saddr) {
            ((uint64_t)2 << 61);
 }
 
-template <bool PAIR>
 __device__ __forceinline__ void f8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    if (PAIR)
-        asm volatile(
-            "{\n"
-            ".reg .pred p;\n"
-            "setp.ne.b32 p, %4, 0;\n"
-            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-            "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n"
-            ".reg .pred p;\n"
-            "setp.ne.b32 p, %4, 0;\n"
-            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-            "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-            : "memory");
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
 
-/* all MMAs so far, then an arrival at `bar`, in a pair at both SMs' */
-template <bool PAIR>
+/* all MMAs so far, then an arrival at `bar` */
 __device__ __forceinline__ void f8_commit(uint32_t bar) {
-    if (PAIR)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-                     "h"((uint16_t)3)
-                     : "memory");
-    else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-/* the same shared-memory address in the pair's first SM */
-__device__ __forceinline__ uint32_t f8_leader(uint32_t addr) {
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
-    return r;
-}
-
-/* a box of the map to this SM's shared memory; bar may be the pair's first SM's */
-template <bool PAIR>
+/* a box of the map to shared memory */
 __device__ __forceinline__ void f8_tma2(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
-    if (PAIR)
-        asm volatile(
-            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-            "[%4];" ::"r"(dst),
-            "l"(map), "r"(x), "r"(y), "r"(bar)
-            : "memory");
-    else
-        asm volatile(
-            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-            "l"(map), "r"(x), "r"(y), "r"(bar)
-            : "memory");
-}
-
-__device__ __forceinline__ void f8_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
 }
 
 __device__ __forceinline__ void f8_tmem_ld32(uint32_t taddr, uint32_t *r) {
@@ -289,12 +257,11 @@ __device__ __forceinline__ void f8_fma2(float2 &acc, uint32_t v0, uint32_t v1, f
 
 __device__ __forceinline__ float f8_silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
-template <int MODE, int NT, bool PAIR>
+template <int MODE, int NT>
 struct f8_cfg {
-    static constexpr int ROWS = PAIR ? 256 : 128;                /* of a tile */
-    static constexpr int B_BYTES = (PAIR ? NT / 2 : NT) * 128;   /* of one SM's share */
+    static constexpr int B_BYTES = NT * 128;
     static constexpr int STAGE = (int)F8_A_BYTES + B_BYTES;
-    static constexpr int STAGES = PAIR ? 6 : NT == 256 ? 4 : NT == 128 ? 6 : 8;
+    static constexpr int STAGES = NT == 256 ? 4 : NT == 128 ? 6 : 8;
     static constexpr int NB = NT == 256 ? 2 : 4;
     static constexpr int OUT = F8_EPI_WARPS * 2048;              /* a warp's 32 rows x 64 bytes on their way out */
     static constexpr int SMEM = STAGES * STAGE + OUT + 1024 + (int)sizeof(f8_ctl_t);
@@ -305,15 +272,14 @@ typedef struct {
     int e, r0, rows, n0;
 } f8_tile_t;
 
-template <int MODE, int NT, bool PAIR>
+template <int MODE, int NT>
 __device__ __forceinline__ f8_tile_t f8_tile(const f8_args_t &P, int it, int n_tiles) {
-    constexpr int ROWS = f8_cfg<MODE, NT, PAIR>::ROWS;
     f8_tile_t t;
     if (MODE == F8_DENSE) { /* rows first: tiles in flight at the same time share rows of b */
-        const int mt = (P.m + ROWS - 1) / ROWS, nt = it / mt;
+        const int mt = (P.m + 127) / 128, nt = it / mt;
         t.e = 0;
-        t.r0 = (it - nt * mt) * ROWS;
-        t.rows = min(ROWS, P.m - t.r0);
+        t.r0 = (it - nt * mt) * 128;
+        t.rows = min(128, P.m - t.r0);
         t.n0 = nt * NT;
     } else {
         const int g = it / n_tiles;
@@ -366,20 +332,18 @@ __device__ __forceinline__ void f8_rows_out(uint32_t buf, const uint32_t *w, uin
     }
 }
 
-template <int MODE, int NT, bool PAIR>
+template <int MODE, int NT>
 __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant__ f8_args_t P) {
-    typedef f8_cfg<MODE, NT, PAIR> cfg;
+    typedef f8_cfg<MODE, NT> cfg;
     constexpr int STAGES = cfg::STAGES, NB = cfg::NB;
     extern __shared__ uint8_t dyn_raw[];
     const uint32_t dyn_u = (fb_smem_u32(dyn_raw) + 1023u) & ~1023u;
     const uint32_t out_u = dyn_u + STAGES * cfg::STAGE;
     f8_ctl_t *C = reinterpret_cast<f8_ctl_t *>(dyn_raw + (dyn_u - fb_smem_u32(dyn_raw)) + STAGES * cfg::STAGE + cfg::OUT);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
-    const int first = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, stride = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
     const int per_n = MODE == F8_GATE_UP ? NT / 2 : NT;
     const int n_tiles = (P.n + per_n - 1) / per_n, kbs = (P.k + 127) / 128;
-    const int tiles = (MODE == F8_DENSE ? (P.m + cfg::ROWS - 1) / cfg::ROWS : P.counts[0]) * n_tiles;
+    const int tiles = (MODE == F8_DENSE ? (P.m + 127) / 128 : P.counts[0]) * n_tiles;
 
     if (tid == 0) {
         for (int s = 0; s < STAGES; s++) {
@@ -388,7 +352,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
         }
         for (int b = 0; b < NB; b++) {
             fb_mbar_init(fb_smem_u32(&C->acc_full[b]), 1);
-            fb_mbar_init(fb_smem_u32(&C->acc_empty[b]), PAIR ? 2 * F8_EPI_WARPS : F8_EPI_WARPS);
+            fb_mbar_init(fb_smem_u32(&C->acc_empty[b]), F8_EPI_WARPS);
         }
         for (int g = 0; g < 2; g++) {
             fb_mbar_init(fb_smem_u32(&C->sc_full[g]), 2);
@@ -398,21 +362,13 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
         fb_mbar_init_fence();
     }
     if (warp == 9) {
-        if (PAIR) {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fb_smem_u32(&C->tmem_base)),
-                         "r"((uint32_t)(NB * NT))
-                         : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-        } else {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fb_smem_u32(&C->tmem_base)),
-                         "r"((uint32_t)(NB * NT))
-                         : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        }
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fb_smem_u32(&C->tmem_base)),
+                     "r"((uint32_t)(NB * NT))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    if (PAIR) f8_cluster_sync();
-    else __syncthreads();
+    __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = C->tmem_base;
 
@@ -423,12 +379,11 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             /* ---------------- operand tiles */
             uint32_t st = 0, ph = 0; /* stage, and the parity of its phase */
             bool ok = true;
-            for (int it = first; it < tiles && ok; it += stride) {
-                const f8_tile_t t = f8_tile<MODE, NT, PAIR>(P, it, n_tiles);
-                /* boxes of 32 rows, as many as this SM's rows need; what is behind the tile's rows is never stored */
-                const int groups = min(4, max(0, (t.rows - 128 * rank + 31) / 32)), y0 = t.r0 + 128 * rank;
-                const int y = t.e * P.b_rec_rows + (MODE == F8_GATE_UP && rank ? P.n + t.n0 : t.n0 + (PAIR ? NT / 2 * rank : 0));
-                const uint32_t bytes = (uint32_t)((t.rows + 31) / 32) * 4096u + (PAIR ? 2u : 1u) * cfg::B_BYTES; /* of both SMs */
+            for (int it = blockIdx.x; it < tiles && ok; it += gridDim.x) {
+                const f8_tile_t t = f8_tile<MODE, NT>(P, it, n_tiles);
+                /* boxes of 32 rows, as many as the rows need; what is behind the tile's rows is never stored */
+                const int groups = (t.rows + 31) / 32, y = t.e * P.b_rec_rows + t.n0;
+                const uint32_t bytes = (uint32_t)groups * 4096u + cfg::B_BYTES;
                 for (int kb = 0; kb < kbs; kb++) {
                     const uint32_t a_u = dyn_u + st * cfg::STAGE, b_u = a_u + F8_A_BYTES;
                     if (!f8_wait_all(fb_smem_u32(&C->empty[st]), ph ^ 1, C)) {
@@ -436,11 +391,11 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                         break;
                     }
                     if (f8_elect()) {
-                        const uint32_t own = fb_smem_u32(&C->full[st]), bar = PAIR ? f8_leader(own) : own;
-                        if (rank == 0) fb_mbar_expect_tx(own, bytes);
-                        f8_tma2<PAIR>(b_u, &P.tb, kb * 128, y, bar);
-                        if (MODE == F8_GATE_UP && !PAIR) f8_tma2<PAIR>(b_u + 16384u, &P.tb, kb * 128, y + P.n, bar);
-                        for (int g = 0; g < groups; g++) f8_tma2<PAIR>(a_u + g * 4096u, &P.ta, kb * 128, y0 + 32 * g, bar);
+                        const uint32_t bar = fb_smem_u32(&C->full[st]);
+                        fb_mbar_expect_tx(bar, bytes);
+                        f8_tma2(b_u, &P.tb, kb * 128, y, bar);
+                        if (MODE == F8_GATE_UP) f8_tma2(b_u + 16384u, &P.tb, kb * 128, y + P.n, bar);
+                        for (int g = 0; g < groups; g++) f8_tma2(a_u + g * 4096u, &P.ta, kb * 128, t.r0 + 32 * g, bar);
                     }
                     __syncwarp();
                     if (++st == STAGES) {
@@ -457,12 +412,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     ph ^= 1;
                 }
             }
-        } else if (warp == 9 && rank == 0) {
-            /* ---------------- MMAs: one thread, in a pair one for both SMs */
-            const uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(cfg::ROWS >> 4) << 24);
+        } else if (warp == 9) {
+            /* ---------------- MMAs: one thread */
+            const uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             uint32_t st = 0, ph = 0, b = 0, bph = 0, have_ab = 0, have_acc = 0;
             bool ok = true;
-            for (int it = first; it < tiles && ok; it += stride)
+            for (int it = blockIdx.x; it < tiles && ok; it += gridDim.x)
                 for (int kb = 0; kb < kbs; kb++) {
                     if ((!__all_sync(FULL, have_ab) && !f8_wait_all(fb_smem_u32(&C->full[st]), ph, C)) ||
                         (!__all_sync(FULL, have_acc) && !f8_wait_all(fb_smem_u32(&C->acc_empty[b]), bph ^ 1, C))) {
@@ -474,9 +429,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     if (f8_elect()) {
 #pragma unroll
                         for (int q = 0; q < 4; q++)
-                            f8_mma<PAIR>(tmem + b * NT, f8_desc(a_u + 32 * q), f8_desc(b_u + 32 * q), idesc, q > 0);
-                        f8_commit<PAIR>(fb_smem_u32(&C->acc_full[b]));
-                        f8_commit<PAIR>(fb_smem_u32(&C->empty[st]));
+                            f8_mma(tmem + b * NT, f8_desc(a_u + 32 * q), f8_desc(b_u + 32 * q), idesc, q > 0);
+                        f8_commit(fb_smem_u32(&C->acc_full[b]));
+                        f8_commit(fb_smem_u32(&C->empty[st]));
                     }
                     __syncwarp();
                     if (++st == STAGES) {
@@ -496,10 +451,10 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             const int i = tid - 320;
             uint32_t g = 0;
             bool ok = true;
-            for (int it = first; it < tiles && ok; it += stride) {
-                const f8_tile_t t = f8_tile<MODE, NT, PAIR>(P, it, n_tiles);
-                const float *a0 = P.a_scales + (int64_t)(t.r0 + min(128 * rank + i, t.rows - 1)) * P.as_stride;
-                const float *a1 = P.a_scales + (int64_t)(t.r0 + min(128 * rank + i + 64, t.rows - 1)) * P.as_stride;
+            for (int it = blockIdx.x; it < tiles && ok; it += gridDim.x) {
+                const f8_tile_t t = f8_tile<MODE, NT>(P, it, n_tiles);
+                const float *a0 = P.a_scales + (int64_t)(t.r0 + min(i, t.rows - 1)) * P.as_stride;
+                const float *a1 = P.a_scales + (int64_t)(t.r0 + min(i + 64, t.rows - 1)) * P.as_stride;
                 const float *rec = P.b_scales + (int64_t)t.e * P.bs_rec;
                 const float *b0 = rec + (int64_t)(min(t.n0, P.n - 1) >> 7) * P.bs_stride;
                 const float *b1 = rec + (int64_t)((MODE == F8_GATE_UP ? P.n + t.n0 : min(t.n0 + NT / 2, P.n - 1)) >> 7) * P.bs_stride;
@@ -531,14 +486,13 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
     } else {
         if (NT == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         /* ---------------- join the blocks' sums: warp w reads lanes 32 (w % 4) .., warpgroup wg its half of the columns */
-        constexpr int W = NT / 2, CW = W < 64 ? W : 64;
+        constexpr int W = NT / 2;
         const int wg = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t t_row = tmem + ((uint32_t)(warp & 3) << 21);
         uint32_t step = 0, cnt = 0, grp = 0, have = 0;
         bool ok = true;
-        for (int it = first; it < tiles; it += stride, cnt++) {
-            const f8_tile_t t = f8_tile<MODE, NT, PAIR>(P, it, n_tiles);
-            const int r0 = t.r0 + 128 * rank, rows = min(128, t.rows - 128 * rank); /* of this SM; a pair's second may have none */
+        for (int it = blockIdx.x; it < tiles; it += gridDim.x, cnt++) {
+            const f8_tile_t t = f8_tile<MODE, NT>(P, it, n_tiles);
             const int c0 = t.n0 + (MODE == F8_GATE_UP ? 0 : wg * W); /* first row of b of this thread's columns */
             float2 acc[W / 2];
 #pragma unroll
@@ -558,39 +512,51 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
     } while (0)
             float n0, n1 = 0.0f;
             F8_FACTORS(0);
+            /* Chunks of 32 columns through two register buffers: while one is joined the next is on its way, also across
+             * blocks.  (gate/up: the first half of a thread's columns are the gate's, the second the up's) */
+#define F8_COL(buffer, c) \
+    (t_row + (uint32_t)((buffer) * NT + (MODE == F8_GATE_UP ? (c) / (CH / 2) * (NT / 2) + wg * (W / 2) + (c) % (CH / 2) * 32 : wg * W + (c) * 32)))
+            constexpr int CH = W / 32;
+            uint32_t r[2][32];
+            if (ok && !__all_sync(FULL, have)) ok = f8_wait_all(fb_smem_u32(&C->acc_full[step % NB]), (step / NB) & 1, C);
+            if (ok) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                f8_tmem_ld32(F8_COL(step % NB, 0), r[0]);
+            }
             for (int kb = 0; kb < kbs; kb++, step++) {
                 const int b = step % NB;
                 const float f0 = n0, f1 = MODE == F8_GATE_UP ? n1 : n0;
-                if (ok && !__all_sync(FULL, have)) ok = f8_wait_all(fb_smem_u32(&C->acc_full[b]), (step / NB) & 1, C);
                 if (!ok) continue;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t tc = t_row + (uint32_t)(b * NT);
-                /* chunk c of the thread's columns (gate/up: the gate's, then the up's) */
 #pragma unroll
-                for (int c = 0; c < W / CW; c++) {
-                    uint32_t r[CW];
-                    const uint32_t col = tc + (uint32_t)(MODE == F8_GATE_UP ? c * (NT / 2) + wg * CW : wg * W + c * CW);
-                    f8_tmem_ld32(col, r);
-                    if (CW > 32) f8_tmem_ld32(col + 32, r + CW - 32);
-                    f8_tmem_wait(r);
-                    if (CW > 32) f8_tmem_wait(r + CW - 32);
-                    if (c == W / CW - 1) { /* the buffer has been read: the next block's MMAs may have it */
+                for (int c = 0; c < CH; c++) {
+                    const int w = CH == 1 ? 0 : c & 1; /* (a single chunk has no second buffer to go to) */
+                    f8_tmem_wait(r[w]);
+                    if (c + 1 < CH) {
+                        f8_tmem_ld32(F8_COL(b, c + 1), r[w ^ 1]);
+                    } else { /* the buffer has been read: the next block's MMAs may have it */
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) {
-                            const uint32_t bar = fb_smem_u32(&C->acc_empty[b]);
-                            if (PAIR)
-                                asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(f8_leader(bar)) : "memory");
-                            else
-                                fb_mbar_arrive(bar);
+                        if (lane == 0) fb_mbar_arrive(fb_smem_u32(&C->acc_empty[b]));
+                        if (kb + 1 < kbs) {
+                            if (CH == 1 || !__all_sync(FULL, have)) ok = f8_wait_all(fb_smem_u32(&C->acc_full[(step + 1) % NB]), ((step + 1) / NB) & 1, C);
+                            if (ok && CH > 1) {
+                                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                                f8_tmem_ld32(F8_COL((step + 1) % NB, 0), r[w ^ 1]);
+                            }
+                            F8_FACTORS(kb + 1);
+                        } else {
+                            have = f8_look(fb_smem_u32(&C->acc_full[(step + 1) % NB]), ((step + 1) / NB) & 1);
                         }
-                        /* the next block's barrier and factors are asked for before this block's products */
-                        have = f8_look(fb_smem_u32(&C->acc_full[(step + 1) % NB]), ((step + 1) / NB) & 1);
-                        if (kb + 1 < kbs) F8_FACTORS(kb + 1);
                     }
-                    const float f = c ? f1 : f0;
+                    const float f = c >= CH / 2 ? f1 : f0;
 #pragma unroll
-                    for (int i = 0; i < CW / 2; i++) f8_fma2(acc[c * (CW / 2) + i], r[2 * i], r[2 * i + 1], f);
+                    for (int i = 0; i < 16; i++) f8_fma2(acc[16 * c + i], r[w][2 * i], r[w][2 * i + 1], f);
+                    /* the next block's barrier is asked for a chunk ahead of its use */
+                    if (CH > 1 && c == CH - 2) have = f8_look(fb_smem_u32(&C->acc_full[(step + 1) % NB]), ((step + 1) / NB) & 1);
+                    if (CH == 1 && kb + 1 < kbs && ok) {
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        f8_tmem_ld32(F8_COL((step + 1) % NB, 0), r[0]);
+                    }
                 }
             }
             const uint32_t buf = out_u + warp * 2048u;
@@ -607,16 +573,16 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                 asm volatile("bar.sync 1, 256;" ::: "memory"); /* the 8 warps meet once a tile, also after a wait that ran out */
                 const float sc = ops_f8_scale(ops_amax(amax, C->amax[cnt & 1][wg ^ 1][row]));
                 const float inv = __frcp_rn(sc); /* (the values carry a few roundings already: one more, of the quotient, is theirs) */
-                const bool mine = row < rows && ok;
+                const bool mine = row < t.rows && ok;
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++)
                     w[i] = ops_f8_pack4(acc[2 * i].x * inv, acc[2 * i].y * inv, acc[2 * i + 1].x * inv, acc[2 * i + 1].y * inv);
-                f8_rows_out<64>(buf, w, mine ? P.act_q + (int64_t)(r0 + row) * P.n + t.n0 + wg * 64 : nullptr, 64, 1, 4);
-                if (mine && wg == 0) P.act_scales[(int64_t)(r0 + row) * (P.n >> 7) + (t.n0 >> 7)] = sc;
+                f8_rows_out<64>(buf, w, mine ? P.act_q + (int64_t)(t.r0 + row) * P.n + t.n0 + wg * 64 : nullptr, 64, 1, 4);
+                if (mine && wg == 0) P.act_scales[(int64_t)(t.r0 + row) * (P.n >> 7) + (t.n0 >> 7)] = sc;
             } else {
-                const bool mine = row < rows && ok;
-                const int64_t o = mine ? (int64_t)(MODE == F8_DOWN ? P.pairs[r0 + row] : r0 + row) * P.out_stride + c0 : 0;
+                const bool mine = row < t.rows && ok;
+                const int64_t o = mine ? (int64_t)(MODE == F8_DOWN ? P.pairs[t.r0 + row] : t.r0 + row) * P.out_stride + c0 : 0;
                 if (MODE == F8_DENSE && P.out_bf16) {
                     uint32_t w[W / 2];
 #pragma unroll
@@ -639,11 +605,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
         if (tid == 0) *P.status = FB_ST_WAIT_TIMEOUT;
         for (int i = 0; i < 100; i++) __nanosleep(1000); /* copies and MMAs under way land before their memory is released */
     }
-    if (PAIR) f8_cluster_sync(); /* neither SM goes while the other's MMAs or arrivals may reach it */
-    if (warp == 9) {
-        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(NB * NT)) : "memory");
-        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(NB * NT)) : "memory");
-    }
+    __syncthreads();
+    if (warp == 9)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(NB * NT)) : "memory");
 }
 
 /* ------------------------------------------------------------------ tensor maps */
@@ -663,23 +627,12 @@ static int f8_map(CUtensorMap *m, const void *p, uint64_t k, uint64_t rows, uint
                : (int)cudaErrorInvalidValue;
 }
 
-template <int MODE, int NT, bool PAIR>
+template <int MODE, int NT>
 static int f8_launch(f8_args_t &p, int64_t most_tiles, int n_sm, int *launches, cudaStream_t st) {
-    cudaLaunchConfig_t c = {};
-    cudaLaunchAttribute at[1];
-    const int64_t want = PAIR ? 2 * most_tiles : most_tiles;
-    c.gridDim = dim3((unsigned)(want < n_sm ? want : PAIR ? n_sm & ~1 : n_sm));
-    c.blockDim = dim3(F8_THREADS);
-    c.dynamicSmemBytes = f8_cfg<MODE, NT, PAIR>::SMEM;
-    c.stream = st;
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = PAIR ? 2 : 1;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    c.attrs = at;
-    c.numAttrs = 1;
+    const int grid = (int)(most_tiles < n_sm ? most_tiles : n_sm);
+    k_f8_mma<MODE, NT><<<grid, F8_THREADS, f8_cfg<MODE, NT>::SMEM, st>>>(p);
     *launches += 1;
-    const cudaError_t rc = cudaLaunchKernelEx(&c, k_f8_mma<MODE, NT, PAIR>, p);
-    return (int)(rc != cudaSuccess ? rc : cudaGetLastError());
+    return (int)cudaGetLastError();
 }
 
 extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *status, int n_sm, int *launches,
@@ -693,15 +646,14 @@ extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *s
     p.status = status;
     cudaStream_t st = (cudaStream_t)stream;
     const int64_t m = a->m, n = a->n, mt = (m + 127) / 128;
-    /* the largest tile that still gives every SM one: two SMs a tile of 256 x 256 read least, then fewer columns */
-    const int64_t pairs = ((m + 255) / 256) * ((n + 255) / 256);
-    const bool pair = 2 * pairs >= n_sm;
-    const int nt = pair ? 256 : mt * ((n + 127) / 128) >= n_sm ? 128 : 64;
-    const int rc = f8_map(&p.ta, a->a, a->k, a->m, a->a_stride, 32) | f8_map(&p.tb, a->b, a->k, a->n, a->b_stride, pair ? 128 : nt);
+    /* the widest tile that still gives every SM one: wide tiles read the least (4096 x 8192 x 4096: 148 us with 256 columns) */
+    const int nt = mt * ((n + 255) / 256) >= n_sm ? 256 : mt * ((n + 127) / 128) >= n_sm ? 128 : 64;
+    const int rc = f8_map(&p.ta, a->a, a->k, a->m, a->a_stride, 32) | f8_map(&p.tb, a->b, a->k, a->n, a->b_stride, nt);
     if (rc) return rc;
-    return pair        ? f8_launch<F8_DENSE, 256, true>(p, pairs, n_sm, launches, st)
-           : nt == 128 ? f8_launch<F8_DENSE, 128, false>(p, mt * ((n + 127) / 128), n_sm, launches, st)
-                       : f8_launch<F8_DENSE, 64, false>(p, mt * ((n + 63) / 64), n_sm, launches, st);
+    const int64_t tiles = mt * ((n + nt - 1) / nt);
+    return nt == 256   ? f8_launch<F8_DENSE, 256>(p, tiles, n_sm, launches, st)
+           : nt == 128 ? f8_launch<F8_DENSE, 128>(p, tiles, n_sm, launches, st)
+                       : f8_launch<F8_DENSE, 64>(p, tiles, n_sm, launches, st);
 }
 
 /* ------------------------------------------------------------------ the pairs' rows of x side by side: one warp a row
@@ -760,19 +712,16 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     const int n_routed = a->n_tokens * a->top_k, n_shared = a->has_shared ? a->n_tokens : 0, H = a->n_embd, I = a->n_inter;
     int *counts = (int *)(ws + w.counts), *pairs = (int *)(ws + w.pairs);
     int4 *items = (int4 *)(ws + w.counts + 256);
-    /* two SMs a tile of 256 rows once the experts have that many rows to fill it; until then the weights' bytes decide */
     const int64_t recs = a->n_experts + (a->has_shared ? 1 : 0);
-    const bool pair = w.n_pairs >= 192 * recs;
-    const int tile = pair ? 256 : 128;
     k_ops_bucket<<<1, BK_THREADS, (size_t)a->n_experts * BK_WARPS * 4, st>>>(
-        a->ids, n_routed, a->n_tokens, a->n_experts, a->has_shared, tile, counts, pairs, items, status);
+        a->ids, n_routed, a->n_tokens, a->n_experts, a->has_shared, counts, pairs, items, status);
     k_ops_permute<<<(w.n_pairs + 7) / 8, 256, 0, st>>>(a->x, a->x_stride, a->x_scales, a->x_scales_stride, H, counts, pairs,
                                                       n_routed, a->top_k, n_shared, ws + w.xp, (float *)(ws + w.xp_scales));
     *launches += 2;
     int rc = (int)cudaGetLastError();
     if (rc) return rc;
     /* no more tiles than this (the device knows how many there are) */
-    const int64_t tiles = w.n_pairs / tile + recs;
+    const int64_t tiles = w.n_pairs / 128 + recs;
     f8_args_t p = {};
     p.counts = counts, p.pairs = pairs, p.items = items, p.status = status;
     p.n = I, p.k = H;
@@ -780,18 +729,14 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     p.b_scales = a->gate_up_scales, p.bs_stride = H / 128, p.bs_rec = (int64_t)(2 * I / 128) * (H / 128), p.b_rec_rows = 2 * I;
     p.act_q = ws + w.act_q, p.act_scales = (float *)(ws + w.act_scales);
     rc = f8_map(&p.ta, ws + w.xp, H, w.n_pairs, H, 32) | f8_map(&p.tb, a->gate_up, H, recs * 2 * I, H, 128);
-    if (!rc)
-        rc = pair ? f8_launch<F8_GATE_UP, 256, true>(p, tiles * (I / 128), n_sm, launches, st)
-                  : f8_launch<F8_GATE_UP, 256, false>(p, tiles * (I / 128), n_sm, launches, st);
+    if (!rc) rc = f8_launch<F8_GATE_UP, 256>(p, tiles * (I / 128), n_sm, launches, st);
     if (rc) return rc;
     p.n = H, p.k = I;
     p.a_scales = p.act_scales, p.as_stride = I / 128;
     p.b_scales = a->down_scales, p.bs_stride = I / 128, p.bs_rec = (int64_t)(H / 128) * (I / 128), p.b_rec_rows = H;
     p.out = ws + w.dots, p.out_stride = H, p.out_vec = 1;
-    rc = f8_map(&p.ta, ws + w.act_q, I, w.n_pairs, I, 32) | f8_map(&p.tb, a->down, I, recs * H, I, pair ? 128 : 256);
-    if (!rc)
-        rc = pair ? f8_launch<F8_DOWN, 256, true>(p, tiles * ((H + 255) / 256), n_sm, launches, st)
-                  : f8_launch<F8_DOWN, 256, false>(p, tiles * ((H + 255) / 256), n_sm, launches, st);
+    rc = f8_map(&p.ta, ws + w.act_q, I, w.n_pairs, I, 32) | f8_map(&p.tb, a->down, I, recs * H, I, 256);
+    if (!rc) rc = f8_launch<F8_DOWN, 256>(p, tiles * ((H + 255) / 256), n_sm, launches, st);
     if (rc) return rc;
     k_ops_combine<<<a->n_tokens, 256, 0, st>>>((const float *)(ws + w.dots), a->ids, a->weights, H, a->n_experts, a->top_k,
                                               n_routed, a->has_shared, (__nv_bfloat16 *)a->out, a->out_stride);
@@ -811,12 +756,10 @@ extern "C" int ops_f8_init(void) {
         f8_encode = (f8_encode_t)fn;
     }
 #define RK(k) rc |= (int)cudaFuncGetAttributes(&f, (k))
-#define RM(MODE, NT, PAIR)                                                                                        \
-    rc |= (int)cudaFuncSetAttribute(k_f8_mma<MODE, NT, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
-                                    f8_cfg<MODE, NT, PAIR>::SMEM)
+#define RM(MODE, NT)                                                                                             \
+    rc |= (int)cudaFuncSetAttribute(k_f8_mma<MODE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, f8_cfg<MODE, NT>::SMEM)
     RK(k_ops_combine); RK(k_ops_bucket); RK(k_ops_permute);
-    RM(F8_DENSE, 256, true); RM(F8_DENSE, 128, false); RM(F8_DENSE, 64, false);
-    RM(F8_GATE_UP, 256, true); RM(F8_GATE_UP, 256, false); RM(F8_DOWN, 256, true); RM(F8_DOWN, 256, false);
+    RM(F8_DENSE, 256); RM(F8_DENSE, 128); RM(F8_DENSE, 64); RM(F8_GATE_UP, 256); RM(F8_DOWN, 256);
 #undef RM
 #undef RK
     rc |= (int)cudaFuncSetAttribute(k_ops_bucket, cudaFuncAttributeMaxDynamicSharedMemorySize, OPS_MAX_E * BK_WARPS * 4);

@@ -320,7 +320,8 @@ def mat64(q, s):
 
 MNK = [(1, 1, 16), (1, 128, 128), (2, 130, 144), (3, 64, 2064), (7, 1000, 272), (8, 4096, 512), (9, 31, 128), (15, 513, 400),
        (16, 256, 1024), (17, 300, 640), (31, 128, 4096), (33, 257, 256), (64, 2048, 1040), (67, 1000, 2064), (127, 255, 384),
-       (128, 256, 128), (129, 129, 160), (200, 1, 512), (255, 640, 2048), (513, 1152, 896), (1025, 520, 256)]
+       (128, 256, 128), (129, 129, 160), (200, 1, 512), (255, 640, 2048), (513, 1152, 896), (1025, 520, 256),
+       (640, 4001, 144), (1100, 4488, 176), (1281, 4096, 272)]
 
 
 @pytest.mark.parametrize("M,N,K", MNK)
