@@ -4,6 +4,7 @@
  */
 #include <cuda.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -19,87 +20,127 @@
 #endif
 
 /* ------------------------------------------------------------------ bucket: the pairs of every expert, in pair order
- * One block.  Warp w owns a contiguous run of pairs; a first walk counts each warp's pairs of every expert, a prefix over
- * (expert, warp) gives every warp its first place, a second walk places the pairs.  The order inside an expert is the
- * order of the pairs, so results do not depend on timing.  The shared expert's pairs (n_routed + t) come last. */
+ * Block b owns a run of pairs, warp w a run of the block's.  A first walk counts each warp's pairs of every expert, prefixes
+ * over (expert, block, warp) give every warp its first place, a second walk places the pairs.  The order inside an expert is
+ * the order of the pairs, so results do not depend on timing.  The shared expert's pairs (n_routed + t) come last.  With more
+ * than one block a first launch (COUNT) leaves each block's counts in `block_counts`.  Eight ids a lane are in flight at
+ * once.  (65,536 pairs: one block, one id a lane 150 us; eight ids 100 us, bound by one SM's scattered stores.) */
 #define BK_THREADS 1024
 #define BK_WARPS 32
+#define BK_AHEAD 8
+#define BK_RUN 4096   /* pairs of a block, unless that makes more than ... */
+#define BK_BLOCKS 64  /* ... this many blocks */
 
-__global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n_routed, int n_tokens, int n_experts,
-                                                          int has_shared, int *counts, int *pairs, int4 *items,
-                                                          int *status) {
-    extern __shared__ int s_cnt[]; /* [n_experts][BK_WARPS] */
+template <bool COUNT>
+__global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n_routed, int block_run, int n_tokens,
+                                                          int n_experts, int has_shared, int *block_counts, int *counts,
+                                                          int *pairs, int *pos, int4 *items, int *status) {
+    extern __shared__ int s_cnt[]; /* [n_experts][BK_WARPS], then [n_experts]: the block's first place */
     __shared__ int s_tot[BK_WARPS], s_til[BK_WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int i = tid; i < n_experts * BK_WARPS; i += BK_THREADS) s_cnt[i] = 0;
     __syncthreads();
-    const int run = ((n_routed + BK_THREADS - 1) / BK_THREADS) * 32; /* pairs of a warp */
-    const int p0 = warp * run, p1 = min(n_routed, p0 + run);
-    for (int pass = 0; pass < 2; pass++) {
-        for (int b = p0; b < p1; b += 32) {
-            const int p = b + lane;
-            int e = p < p1 ? ids[p] : -1;
-            if (e < -1 || e >= n_experts) {
-                if (pass == 0) *status = FB_ST_BAD_ID;
-                e = -1;
-            }
-            const unsigned same = __match_any_sync(FULL, e);
-            if (e >= 0) {
-                const int rank = __popc(same & ((1u << lane) - 1u)), at = s_cnt[e * BK_WARPS + warp];
-                if (pass == 1) pairs[at + rank] = p;
-            }
-            __syncwarp();
-            if (e >= 0 && lane == __ffs(same) - 1) s_cnt[e * BK_WARPS + warp] += __popc(same);
-            __syncwarp();
+    const int run = ((block_run + BK_THREADS - 1) / BK_THREADS) * 32; /* pairs of a warp */
+    const int q1 = min(n_routed, ((int)blockIdx.x + 1) * block_run);
+    const int p0 = min(q1, (int)blockIdx.x * block_run + warp * run), p1 = min(q1, p0 + run);
+    for (int b0 = p0; b0 < p1; b0 += 32 * BK_AHEAD) {
+        int e[BK_AHEAD];
+#pragma unroll
+        for (int u = 0; u < BK_AHEAD; u++) e[u] = b0 + 32 * u + lane < p1 ? ids[b0 + 32 * u + lane] : -1;
+#pragma unroll
+        for (int u = 0; u < BK_AHEAD; u++) {
+            if ((unsigned)e[u] < (unsigned)n_experts) atomicAdd(&s_cnt[e[u] * BK_WARPS + warp], 1);
+            else if (e[u] != -1) *status = FB_ST_BAD_ID;
         }
-        if (pass == 1) break;
-        __syncthreads();
-        /* thread e: the expert's total, then exclusive prefixes of pairs and of 128-row tiles over the experts */
-        int tot = 0;
-        if (tid < n_experts)
+    }
+    __syncthreads();
+    /* thread e: the expert's total and what the blocks before this one have of it */
+    int tot = 0, before = 0;
+    if (tid < n_experts) {
+        if (COUNT || gridDim.x == 1)
             for (int w = 0; w < BK_WARPS; w++) tot += s_cnt[tid * BK_WARPS + ((w + tid) & 31)];
-        const int til = (tot + 127) / 128;
-        int a = tot, c = til;
-        for (int s = 1; s < 32; s <<= 1) {
-            const int oa = __shfl_up_sync(FULL, a, s), oc = __shfl_up_sync(FULL, c, s);
-            if (lane >= s) {
-                a += oa;
-                c += oc;
+        else
+            for (int b = 0; b < (int)gridDim.x; b++) {
+                const int n = block_counts[b * n_experts + tid];
+                tot += n;
+                before += b < (int)blockIdx.x ? n : 0;
             }
+    }
+    if (COUNT) {
+        if (tid < n_experts) block_counts[blockIdx.x * n_experts + tid] = tot;
+        return;
+    }
+    /* exclusive prefixes of pairs and of 128-row tiles over the experts */
+    const int til = (tot + 127) / 128;
+    int a = tot, c = til;
+    for (int s = 1; s < 32; s <<= 1) {
+        const int oa = __shfl_up_sync(FULL, a, s), oc = __shfl_up_sync(FULL, c, s);
+        if (lane >= s) {
+            a += oa;
+            c += oc;
         }
-        if (lane == 31) {
-            s_tot[warp] = a;
-            s_til[warp] = c;
-        }
-        __syncthreads();
-        int base = a - tot, tbase = c - til;
-        for (int w = 0; w < warp; w++) {
+    }
+    if (lane == 31) {
+        s_tot[warp] = a;
+        s_til[warp] = c;
+    }
+    __syncthreads();
+    int base = a - tot, tbase = c - til, all = 0;
+    for (int w = 0; w < BK_WARPS; w++) {
+        all += s_tot[w];
+        if (w < warp) {
             base += s_tot[w];
             tbase += s_til[w];
         }
+    }
+    if (blockIdx.x == 0) {
         if (tid < n_experts) {
-            int at = base;
-            for (int w = 0; w < BK_WARPS; w++) {
-                const int n = s_cnt[tid * BK_WARPS + w];
-                s_cnt[tid * BK_WARPS + w] = at;
-                at += n;
-            }
             for (int m = 0; m < til; m++) items[tbase + m] = make_int4(tid, base + 128 * m, min(128, tot - 128 * m), 0);
-        }
-        if (tid == BK_THREADS - 1) { /* no expert's thread: n_experts <= 512 */
+        } else if (tid == BK_THREADS - 1) { /* no expert's thread: n_experts <= 512 */
             const int sh = has_shared ? (n_tokens + 127) / 128 : 0;
             for (int m = 0; m < sh; m++)
                 items[tbase + m] = make_int4(n_experts, base + 128 * m, min(128, n_tokens - 128 * m), 0);
             counts[0] = tbase + sh; /* tiles */
             counts[1] = base;       /* routed pairs that are left */
         }
-        __syncthreads();
     }
-    if (has_shared) {
-        int base = 0;
-        for (int w = 0; w < BK_WARPS; w++) base += s_tot[w];
-        for (int t = tid; t < n_tokens; t += BK_THREADS) pairs[base + t] = n_routed + t;
+    /* the first place of every (expert, warp): a warp to an expert, a lane to a warp's count */
+    if (tid < n_experts) s_cnt[n_experts * BK_WARPS + tid] = base + before;
+    __syncthreads();
+    for (int e = warp; e < n_experts; e += BK_WARPS) {
+        const int n = s_cnt[e * BK_WARPS + lane];
+        int x = n;
+        for (int s = 1; s < 32; s <<= 1) {
+            const int o = __shfl_up_sync(FULL, x, s);
+            if (lane >= s) x += o;
+        }
+        s_cnt[e * BK_WARPS + lane] = s_cnt[n_experts * BK_WARPS + e] + x - n;
     }
+    __syncthreads();
+    for (int b0 = p0; b0 < p1; b0 += 32 * BK_AHEAD) {
+        int e[BK_AHEAD];
+#pragma unroll
+        for (int u = 0; u < BK_AHEAD; u++) e[u] = b0 + 32 * u + lane < p1 ? ids[b0 + 32 * u + lane] : -1;
+#pragma unroll
+        for (int u = 0; u < BK_AHEAD; u++) {
+            const bool in = (unsigned)e[u] < (unsigned)n_experts;
+            const unsigned same = __match_any_sync(FULL, in ? e[u] : -1);
+            int at = 0;
+            if (in) {
+                at = s_cnt[e[u] * BK_WARPS + warp] + __popc(same & ((1u << lane) - 1u));
+                pairs[at] = b0 + 32 * u + lane;
+                pos[b0 + 32 * u + lane] = at;
+            }
+            __syncwarp();
+            if (in && lane == 31 - __clz(same)) s_cnt[e[u] * BK_WARPS + warp] = at + 1;
+            __syncwarp();
+        }
+    }
+    if (has_shared)
+        for (int t = blockIdx.x * BK_THREADS + tid; t < n_tokens; t += gridDim.x * BK_THREADS) {
+            pairs[all + t] = n_routed + t;
+            pos[n_routed + t] = all + t;
+        }
 }
 
 /* ------------------------------------------------------------------ products on the 5th-generation tensor cores
@@ -123,7 +164,7 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
  *
  *   dense    A: rows of a;                               B: rows of b;                        D to out
  *   gate/up  A: the tokens of an expert's pairs;         B: 128 gate rows, 128 up rows;       silu(g) u to FP8, 128 a block
- *   down     A: the activations of an expert's pairs;    B: rows of its down matrix;          D to the pair's row of dots
+ *   down     A: the activations of an expert's pairs;    B: rows of its down matrix;          D as fp16 with a scale
  *
  * Every wait is bounded; when one runs out the status word is set, all roles stop waiting and the block drains, frees its
  * tensor memory and returns. */
@@ -137,7 +178,7 @@ enum { F8_DENSE = 0, F8_GATE_UP = 1, F8_DOWN = 2 };
 #define F8_SC 4 /* blocks of k whose scales are handed over at once */
 
 typedef struct {
-    CUtensorMap ta, tb;
+    CUtensorMap ta, tb, to; /* to: where D goes, boxes of 128 bytes x 32 rows (out_tma) */
     int m, n, k; /* n: rows of b, of one half (gate or up) for F8_GATE_UP */
     const float *a_scales;
     int64_t as_stride;
@@ -145,8 +186,9 @@ typedef struct {
     int64_t bs_stride, bs_rec; /* elements of a row of blocks, of a record */
     int b_rec_rows;            /* rows of b of a record */
     void *out;
-    int out_bf16, out_vec; /* out_vec: rows of out are 16-byte aligned */
+    int out_bf16, out_tma; /* out_tma: rows of out are 16-byte aligned, D leaves as boxes */
     int64_t out_stride;
+    float *out_scales; /* F8_DOWN: [pairs][n / 128] */
     uint8_t *act_q; /* F8_GATE_UP: [pairs][n] */
     float *act_scales;
     const int *counts, *pairs;
@@ -261,9 +303,10 @@ template <int MODE, int NT>
 struct f8_cfg {
     static constexpr int B_BYTES = NT * 128;
     static constexpr int STAGE = (int)F8_A_BYTES + B_BYTES;
-    static constexpr int STAGES = NT == 256 ? 4 : NT == 128 ? 6 : 8;
+    static constexpr int STAGES = NT == 256 ? (MODE == F8_GATE_UP ? 4 : 3) : NT == 128 ? 5 : 7;
     static constexpr int NB = NT == 256 ? 2 : 4;
-    static constexpr int OUT = F8_EPI_WARPS * 2048;              /* a warp's 32 rows x 64 bytes on their way out */
+    static constexpr int BUFS = MODE == F8_GATE_UP ? 0 : NT == 256 ? 2 : 1; /* a warp's staging buffers of 32 rows x 128 bytes */
+    static constexpr int OUT = F8_EPI_WARPS * BUFS * 4096;
     static constexpr int SMEM = STAGES * STAGE + OUT + 1024 + (int)sizeof(f8_ctl_t);
 };
 
@@ -292,44 +335,57 @@ __device__ __forceinline__ f8_tile_t f8_tile(const f8_args_t &P, int it, int n_t
     return t;
 }
 
-/* Out of registers, coalesced: a warp's 32 rows x N8 x 8 bytes pass through shared memory 64 bytes of a row at a time (the
- * 16-byte pieces of row r at piece ^ (r / 2) % 4, so that neither side has bank conflicts) and leave as runs of 64 bytes.
- * rowp: where row 0 .. 31 of the warp begin (NULL: not stored); left: bytes of a row that are inside out. */
-template <int BYTES>
-__device__ __forceinline__ void f8_rows_out(uint32_t buf, const uint32_t *w, uint8_t *my_row, int left, int vec, int elem) {
+/* 128 bytes of each of a warp's 32 rows to its staging buffer, as a TMA box with 128-byte swizzle has them: the 16-byte piece
+ * q of row r at q ^ r % 8, so that a warp's stores have no bank conflicts either */
+__device__ __forceinline__ void f8_stage(uint32_t buf, const uint32_t *w) {
+    const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+    for (uint32_t q = 0; q < 8; q++)
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 128u + ((q ^ (lane & 7u)) << 4)), "r"(w[4 * q]),
+                     "r"(w[4 * q + 1]), "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
+                     : "memory");
+}
+
+/* the staged box to global memory: all of it by TMA, or the first `rows` rows by the warp.  row0: where the first row's
+ * 128 bytes go, stride: bytes from row to row, left: bytes of a row that are inside out, elem: bytes of a value */
+__device__ __forceinline__ void f8_box_out(uint32_t buf, const CUtensorMap *map, int x, int y, bool tma, uint8_t *row0,
+                                           int64_t stride, int rows, int left, int elem) {
     const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int c = 0; c < BYTES / 64; c++) {
+    if (tma) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 64u + (uint32_t)((q ^ ((lane >> 1) & 3)) << 4)),
-                         "r"(w[16 * c + 4 * q]), "r"(w[16 * c + 4 * q + 1]), "r"(w[16 * c + 4 * q + 2]), "r"(w[16 * c + 4 * q + 3])
+        if (f8_elect()) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x),
+                         "r"(y), "r"(buf)
                          : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
         __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = 8 * i + (lane >> 2), q = lane & 3, at = 64 * c + 16 * q;
-            uint8_t *row = reinterpret_cast<uint8_t *>(__shfl_sync(FULL, (unsigned long long)my_row, r));
-            const uint4 v = fb_lds128(buf + r * 64u + (uint32_t)((q ^ ((r >> 1) & 3)) << 4));
-            if (row && at < left) {
-                if (vec && at + 16 <= left) {
-                    *reinterpret_cast<uint4 *>(row + at) = v;
-                } else {
-                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        if (elem == 4) {
-                            if (at + 4 * k < left) *reinterpret_cast<uint32_t *>(row + at + 4 * k) = x[k];
-                        } else {
-                            if (at + 4 * k < left) *reinterpret_cast<uint16_t *>(row + at + 4 * k) = (uint16_t)x[k];
-                            if (at + 4 * k + 2 < left) *reinterpret_cast<uint16_t *>(row + at + 4 * k + 2) = (uint16_t)(x[k] >> 16);
-                        }
-                    }
-                }
-            }
+        return;
+    }
+    __syncwarp();
+    const int per = 128 / elem;
+    for (int i = lane; i < rows * per; i += 32) {
+        const int r = i / per, c = i - r * per;
+        if (c * elem >= left) continue;
+        const uint32_t at = buf + r * 128u + (uint32_t)((((c * elem) >> 4) ^ (r & 7)) << 4) + ((c * elem) & 15);
+        if (elem == 4) {
+            uint32_t v;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+            *reinterpret_cast<uint32_t *>(row0 + r * stride + c * 4) = v;
+        } else {
+            uint16_t v;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+            *reinterpret_cast<uint16_t *>(row0 + r * stride + c * 2) = v;
         }
     }
+    __syncwarp();
+}
+
+/* the warp's boxes have left its staging buffers */
+__device__ __forceinline__ void f8_box_wait() {
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
 }
 
 template <int MODE, int NT>
@@ -559,7 +615,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     }
                 }
             }
-            const uint32_t buf = out_u + warp * 2048u;
+            const uint32_t buf = out_u + warp * (uint32_t)(cfg::BUFS * 4096);
             if (MODE == F8_GATE_UP) {
                 /* silu(g) u of this thread's 64 columns, and the amax over the row's 128 with the other warpgroup's */
                 float amax = 0.0f;
@@ -574,29 +630,90 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                 const float sc = ops_f8_scale(ops_amax(amax, C->amax[cnt & 1][wg ^ 1][row]));
                 const float inv = __frcp_rn(sc); /* (the values carry a few roundings already: one more, of the quotient, is theirs) */
                 const bool mine = row < t.rows && ok;
-                uint32_t w[16];
+                if (mine) {
+                    uint4 *q = reinterpret_cast<uint4 *>(P.act_q + (int64_t)(t.r0 + row) * P.n + t.n0 + wg * 64);
 #pragma unroll
-                for (int i = 0; i < 16; i++)
-                    w[i] = ops_f8_pack4(acc[2 * i].x * inv, acc[2 * i].y * inv, acc[2 * i + 1].x * inv, acc[2 * i + 1].y * inv);
-                f8_rows_out<64>(buf, w, mine ? P.act_q + (int64_t)(t.r0 + row) * P.n + t.n0 + wg * 64 : nullptr, 64, 1, 4);
-                if (mine && wg == 0) P.act_scales[(int64_t)(t.r0 + row) * (P.n >> 7) + (t.n0 >> 7)] = sc;
-            } else {
-                const bool mine = row < t.rows && ok;
-                const int64_t o = mine ? (int64_t)(MODE == F8_DOWN ? P.pairs[t.r0 + row] : t.r0 + row) * P.out_stride + c0 : 0;
-                if (MODE == F8_DENSE && P.out_bf16) {
-                    uint32_t w[W / 2];
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t w[4];
 #pragma unroll
-                    for (int i = 0; i < W / 2; i++) {
-                        const __nv_bfloat162 h = __floats2bfloat162_rn(acc[i].x, acc[i].y);
-                        w[i] = *reinterpret_cast<const uint32_t *>(&h);
+                        for (int k = 0; k < 4; k++)
+                            w[k] = ops_f8_pack4(acc[8 * i + 2 * k].x * inv, acc[8 * i + 2 * k].y * inv, acc[8 * i + 2 * k + 1].x * inv,
+                                                acc[8 * i + 2 * k + 1].y * inv);
+                        q[i] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                    f8_rows_out<W * 2>(buf, w, mine ? reinterpret_cast<uint8_t *>(P.out) + 2 * o : nullptr, 2 * (P.n - c0), P.out_vec, 2);
+                    if (wg == 0) P.act_scales[(int64_t)(t.r0 + row) * (P.n >> 7) + (t.n0 >> 7)] = sc;
+                }
+            } else {
+                /* rows of this warp that are the tile's; a box may only leave whole if none of its rows is another expert's */
+                const int w0 = (warp & 3) * 32, rows = ok ? max(0, min(32, t.rows - w0)) : 0, c0 = t.n0 + wg * W;
+                const bool tma = P.out_tma && (MODE == F8_DENSE ? rows > 0 : rows == 32);
+                uint32_t w[W / 2];
+                if (MODE == F8_DOWN || P.out_bf16) {
+                    if constexpr (MODE == F8_DOWN) {
+                        /* fp16 relative to a power of two above the row's 128 values: 2^-12 of the largest, a sixteenth of the
+                         * rounding to bf16 that the sum over the experts ends with, at half of fp32's bytes both ways */
+                        float top = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < W / 2; i++) {
+                            const float x = fabsf(acc[i].x), y = fabsf(acc[i].y);
+                            top = fmaxf(top, fmaxf(x < INFINITY ? x : 0.0f, y < INFINITY ? y : 0.0f));
+                        }
+                        const uint32_t e = min((__float_as_uint(top) >> 23) + 1u, 253u);
+                        const float down = __uint_as_float((254u - e) << 23);
+#pragma unroll
+                        for (int i = 0; i < W / 2; i++) {
+                            const __half2 v = __floats2half2_rn(acc[i].x * down, acc[i].y * down);
+                            w[i] = *reinterpret_cast<const uint32_t *>(&v);
+                        }
+                        if (lane < rows && c0 < P.n)
+                            P.out_scales[(int64_t)(t.r0 + row) * (P.n >> 7) + (c0 >> 7)] = __uint_as_float(e << 23);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < W / 2; i++) {
+                            const __nv_bfloat162 v = __floats2bfloat162_rn(acc[i].x, acc[i].y);
+                            w[i] = *reinterpret_cast<const uint32_t *>(&v);
+                        }
+                    }
+                    if constexpr (W >= 64) {
+                        f8_box_wait();
+#pragma unroll
+                        for (int c = 0; c < W / 64; c++) { /* boxes of 64 columns */
+                            const int x = c0 + 64 * c;
+                            f8_stage(buf + c * 4096u, w + 32 * c);
+                            if (x < P.n)
+                                f8_box_out(buf + c * 4096u, &P.to, 2 * x, t.r0 + w0, tma,
+                                           reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + w0) * P.out_stride + x),
+                                           2 * P.out_stride, rows, 2 * (P.n - x), 2);
+                        }
+                    } else if (lane < rows) { /* 64 bytes a row: straight from the registers */
+                        uint8_t *o = reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + row) * P.out_stride + c0);
+#pragma unroll
+                        for (int i = 0; i < W / 8; i++) {
+                            if (P.out_tma && c0 + 8 * i + 8 <= P.n) {
+                                *reinterpret_cast<uint4 *>(o + 16 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < 8; k++)
+                                    if (c0 + 8 * i + k < P.n)
+                                        *reinterpret_cast<uint16_t *>(o + 16 * i + 2 * k) = (uint16_t)(w[4 * i + k / 2] >> (16 * (k & 1)));
+                            }
+                        }
+                    }
                 } else {
-                    f8_rows_out<W * 4>(buf, reinterpret_cast<const uint32_t *>(acc),
-                                       mine ? reinterpret_cast<uint8_t *>(P.out) + 4 * o : nullptr, 4 * (P.n - c0), P.out_vec, 4);
+#pragma unroll
+                    for (int c = 0; c < W / 32; c++) { /* boxes of 32 columns, through the buffers there are */
+                        const int x = c0 + 32 * c;
+                        if (c % cfg::BUFS == 0) f8_box_wait();
+                        f8_stage(buf + c % cfg::BUFS * 4096u, reinterpret_cast<const uint32_t *>(acc) + 32 * c);
+                        if (x < P.n)
+                            f8_box_out(buf + c % cfg::BUFS * 4096u, &P.to, 4 * x, t.r0 + w0, tma,
+                                       reinterpret_cast<uint8_t *>(P.out) + 4 * ((int64_t)(t.r0 + w0) * P.out_stride + x),
+                                       4 * P.out_stride, rows, 4 * (P.n - x), 4);
+                    }
                 }
             }
         }
+        if (MODE != F8_GATE_UP) f8_box_wait(); /* the staging buffers go away with the block */
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -608,6 +725,289 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
     __syncthreads();
     if (warp == 9)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(NB * NT)) : "memory");
+}
+
+/* ------------------------------------------------------------------ few rows: the weights' bytes are all that counts
+ * Up to 16 rows of a, or single pairs of an expert.  A block of 8 warps takes 16 weight rows; warp w takes the units
+ * (blocks of k; of all slots of a token for the down product) w, w + 8, ..., and the eight partial sums meet in shared
+ * memory, in warp order.  A unit, 16 rows x 128 k, goes to the registers of mma.sync (m16n8k32, e4m3: the weight rows are
+ * its 16 rows, the activations its columns) through a ring of FR_RING units a warp: each lane copies (cp.async) exactly the
+ * four 16-byte pieces that it will read, so no lane waits for another, and 192 KB an SM are in flight all the time.  The k
+ * inside a block come in the order that this gives: lane (g, t) holds bytes 16 t .. of rows g and g + 8, the activations
+ * likewise.  16 weight rows a block spread small matrices over all SMs, and nothing has to be set up first. */
+#define FR_WARPS 8
+#define FR_RING 2
+#define FR_SMEM (FR_WARPS * FR_RING * 2048)
+
+__device__ __forceinline__ void fr_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+/* asks for a unit: the lane's four 16-byte pieces {row g, row g + 8} x {first, second 64 bytes} into its places of the slot;
+ * nothing behind k is read (zeros) */
+__device__ __forceinline__ void fr_ask(uint32_t slot, const uint8_t *r0, const uint8_t *r1, int at, int k) {
+    const uint32_t dst = slot + (threadIdx.x & 31) * 16u;
+    const uint32_t in0 = at < k ? 16u : 0u, in1 = at + 64 < k ? 16u : 0u;
+    const int a0 = at < k ? at : 0, a1 = at + 64 < k ? at + 64 : 0;
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(r0 + a0), "r"(in0) : "memory");
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst + 512u), "l"(r1 + a0), "r"(in0) : "memory");
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst + 1024u), "l"(r0 + a1), "r"(in1) : "memory");
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst + 1536u), "l"(r1 + a1), "r"(in1) : "memory");
+}
+
+__device__ __forceinline__ void fr_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+/* the oldest unit in flight has landed: the lane's pieces */
+__device__ __forceinline__ void fr_take(uint4 (&w)[4], uint32_t slot) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(FR_RING - 1) : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = fb_lds128(slot + (threadIdx.x & 31) * 16u + 512u * i);
+}
+
+/* the block's sum of products for 8 columns */
+__device__ __forceinline__ void fr_block(float (&c)[4], const uint4 (&w)[4], uint4 x0, uint4 x1) {
+    c[0] = c[1] = c[2] = c[3] = 0.0f;
+    fr_mma(c, w[0].x, w[1].x, w[0].y, w[1].y, x0.x, x0.y);
+    fr_mma(c, w[0].z, w[1].z, w[0].w, w[1].w, x0.z, x0.w);
+    fr_mma(c, w[2].x, w[3].x, w[2].y, w[3].y, x1.x, x1.y);
+    fr_mma(c, w[2].z, w[3].z, w[2].w, w[3].w, x1.z, x1.w);
+}
+
+typedef struct {
+    int m, n, k;
+    const uint8_t *a;
+    int64_t a_stride;
+    const float *a_scales;
+    int64_t as_stride;
+    const uint8_t *b;
+    int64_t b_stride;
+    const float *b_scales;
+    int64_t bs_stride;
+    void *out;
+    int out_bf16;
+    int64_t out_stride;
+} fr_args_t;
+
+/* out = a b^T, m <= 8 C8 */
+template <int C8>
+__global__ void __launch_bounds__(32 * FR_WARPS) k_f8_few(const fr_args_t P) {
+    __shared__ float s_part[FR_WARPS][16][8 * C8 + 1];
+    extern __shared__ __align__(16) uint8_t ring[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const uint32_t ring_u = fb_smem_u32(ring) + warp * (FR_RING * 2048u);
+    const int n0 = blockIdx.x * 16, kbs = (P.k + 127) / 128;
+    const uint8_t *r0 = P.b + (int64_t)min(n0 + g, P.n - 1) * P.b_stride, *r1 = P.b + (int64_t)min(n0 + g + 8, P.n - 1) * P.b_stride;
+    const float *bs = P.b_scales + (int64_t)(n0 >> 7) * P.bs_stride;
+#pragma unroll
+    for (int i = 0; i < FR_RING; i++) {
+        const int kb = warp + FR_WARPS * i;
+        if (kb < kbs) fr_ask(ring_u + i * 2048u, r0, r1, kb * 128 + 16 * t, P.k);
+        fr_commit();
+    }
+    float acc[C8][4] = {};
+    int slot = 0;
+    for (int kb = warp; kb < kbs; kb += FR_WARPS) {
+        const int at = kb * 128 + 16 * t;
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        uint4 x[C8][2];
+        float s0[C8], s1[C8];
+        const float sb = __ldg(bs + kb);
+#pragma unroll
+        for (int h = 0; h < C8; h++) {
+            const uint8_t *xp = P.a + (int64_t)min(8 * h + g, P.m - 1) * P.a_stride + at;
+            x[h][0] = at < P.k ? __ldg(reinterpret_cast<const uint4 *>(xp)) : z;
+            x[h][1] = at + 64 < P.k ? __ldg(reinterpret_cast<const uint4 *>(xp + 64)) : z;
+            s0[h] = __ldg(P.a_scales + (int64_t)min(8 * h + 2 * t, P.m - 1) * P.as_stride + kb);
+            s1[h] = __ldg(P.a_scales + (int64_t)min(8 * h + 2 * t + 1, P.m - 1) * P.as_stride + kb);
+        }
+        uint4 w[4];
+        fr_take(w, ring_u + slot * 2048u);
+#pragma unroll
+        for (int h = 0; h < C8; h++) {
+            float c[4];
+            fr_block(c, w, x[h][0], x[h][1]);
+            acc[h][0] = fmaf(c[0], sb * s0[h], acc[h][0]);
+            acc[h][1] = fmaf(c[1], sb * s1[h], acc[h][1]);
+            acc[h][2] = fmaf(c[2], sb * s0[h], acc[h][2]);
+            acc[h][3] = fmaf(c[3], sb * s1[h], acc[h][3]);
+        }
+        const int next = kb + FR_WARPS * FR_RING;
+        if (next < kbs) fr_ask(ring_u + slot * 2048u, r0, r1, next * 128 + 16 * t, P.k);
+        fr_commit();
+        slot = (slot + 1) % FR_RING;
+    }
+#pragma unroll
+    for (int h = 0; h < C8; h++) {
+        s_part[warp][g][8 * h + 2 * t] = acc[h][0];
+        s_part[warp][g][8 * h + 2 * t + 1] = acc[h][1];
+        s_part[warp][g + 8][8 * h + 2 * t] = acc[h][2];
+        s_part[warp][g + 8][8 * h + 2 * t + 1] = acc[h][3];
+    }
+    __syncthreads();
+    const int n = threadIdx.x & 15, row = threadIdx.x >> 4;
+    if (row < P.m && n0 + n < P.n) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < FR_WARPS; w++) v += s_part[w][n][row];
+        const int64_t o = row * P.out_stride + n0 + n;
+        if (P.out_bf16) reinterpret_cast<__nv_bfloat16 *>(P.out)[o] = __float2bfloat16_rn(v);
+        else reinterpret_cast<float *>(P.out)[o] = v;
+    }
+}
+
+typedef struct {
+    int n_embd, n_inter, n_experts, top_k, has_shared, n_routed;
+    const uint8_t *x;
+    int64_t x_stride;
+    const float *x_scales;
+    int64_t xs_stride;
+    const int *ids;
+    const float *weights;
+    const uint8_t *gate_up, *down;
+    const float *gu_scales, *dn_scales;
+    float *act; /* [pairs][n_inter] */
+    __nv_bfloat16 *out;
+    int64_t out_stride;
+    int *status;
+} fr_experts_t;
+
+/* pair slot j of token t: its expert, or -1 */
+__device__ __forceinline__ int fr_expert(const fr_experts_t &P, int t, int j) {
+    if (j == P.top_k) return P.n_experts;
+    const int e = P.ids[t * P.top_k + j];
+    return (unsigned)e < (unsigned)P.n_experts ? e : -1;
+}
+
+/* act[pair][16 rows] = silu(gate x) (up x); block (rows, slot, token) */
+__global__ void __launch_bounds__(32 * FR_WARPS) k_f8_few_gate_up(const fr_experts_t P) {
+    __shared__ float s_part[FR_WARPS][2][16];
+    extern __shared__ __align__(16) uint8_t ring[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+    const uint32_t ring_u = fb_smem_u32(ring) + warp * (FR_RING * 2048u);
+    const int t = blockIdx.z, j = blockIdx.y, n0 = blockIdx.x * 16, H = P.n_embd, I = P.n_inter, kbs = H / 128;
+    const int e = fr_expert(P, t, j);
+    if (e < 0) {
+        if (threadIdx.x == 0 && P.ids[t * P.top_k + j] != -1) *P.status = FB_ST_BAD_ID;
+        return;
+    }
+    const uint8_t *r0 = P.gate_up + ((int64_t)e * 2 * I + n0 + g) * H;
+    const int64_t up = (int64_t)I * H, low = (int64_t)8 * H;
+    const float *gs = P.gu_scales + ((int64_t)e * 2 * (I / 128) + (n0 >> 7)) * kbs, *us = gs + (int64_t)(I / 128) * kbs;
+    const uint8_t *x = P.x + t * P.x_stride + 16 * t4;
+    const float *xs = P.x_scales + t * P.xs_stride;
+    /* units in turn: gate and up of a block of k */
+#pragma unroll
+    for (int i = 0; i < FR_RING; i++) {
+        const int kb = warp + FR_WARPS * (i / 2);
+        const uint8_t *r = r0 + (i & 1 ? up : 0);
+        if (kb < kbs) fr_ask(ring_u + i * 2048u, r, r + low, kb * 128 + 16 * t4, H);
+        fr_commit();
+    }
+    float acc[2][2] = {}; /* {gate, up} x {row g, row g + 8} (every column holds the same token) */
+    int slot = 0;
+    for (int kb = warp; kb < kbs; kb += FR_WARPS) {
+        const uint4 x0 = __ldg(reinterpret_cast<const uint4 *>(x + kb * 128)), x1 = __ldg(reinterpret_cast<const uint4 *>(x + kb * 128 + 64));
+        const float sx = __ldg(xs + kb), f[2] = {sx * __ldg(gs + kb), sx * __ldg(us + kb)};
+        const int next = kb + FR_WARPS * (FR_RING / 2);
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            uint4 w[4];
+            float c[4];
+            fr_take(w, ring_u + slot * 2048u);
+            fr_block(c, w, x0, x1);
+            acc[m][0] = fmaf(c[0], f[m], acc[m][0]);
+            acc[m][1] = fmaf(c[2], f[m], acc[m][1]);
+            const uint8_t *r = r0 + (m ? up : 0);
+            if (next < kbs) fr_ask(ring_u + slot * 2048u, r, r + low, next * 128 + 16 * t4, H);
+            fr_commit();
+            slot = (slot + 1) % FR_RING;
+        }
+    }
+    if (t4 == 0) {
+        s_part[warp][0][g] = acc[0][0];
+        s_part[warp][0][g + 8] = acc[0][1];
+        s_part[warp][1][g] = acc[1][0];
+        s_part[warp][1][g + 8] = acc[1][1];
+    }
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        float vg = 0.0f, vu = 0.0f;
+#pragma unroll
+        for (int w = 0; w < FR_WARPS; w++) {
+            vg += s_part[w][0][threadIdx.x];
+            vu += s_part[w][1][threadIdx.x];
+        }
+        P.act[(int64_t)(t * (P.top_k + P.has_shared) + j) * I + n0 + threadIdx.x] = f8_silu_mul(vg, vu);
+    }
+}
+
+/* out[t][16 rows] = sum over the slots of weight (down act), the activations brought to FP8 on the way; block (rows, token).
+ * The warps share the (slot, block of k) units of the token. */
+__global__ void __launch_bounds__(32 * FR_WARPS) k_f8_few_down(const fr_experts_t P) {
+    __shared__ float s_part[FR_WARPS][16];
+    extern __shared__ __align__(16) uint8_t ring[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+    const uint32_t ring_u = fb_smem_u32(ring) + warp * (FR_RING * 2048u);
+    const int t = blockIdx.y, n0 = blockIdx.x * 16, H = P.n_embd, I = P.n_inter, kbs = I / 128;
+    const int slots = P.top_k + P.has_shared, units = slots * kbs;
+    auto ask = [&](int un, int slot) {
+        if (un < units) {
+            const int j = un / kbs, kb = un - j * kbs, e = fr_expert(P, t, j);
+            const uint8_t *r0 = P.down + ((int64_t)max(e, 0) * H + n0 + g) * I;
+            if (e >= 0) fr_ask(ring_u + slot * 2048u, r0, r0 + (int64_t)8 * I, kb * 128 + 16 * t4, I);
+        }
+        fr_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < FR_RING; i++) ask(warp + FR_WARPS * i, i);
+    float acc[2] = {};
+    int slot = 0;
+    for (int un = warp; un < units; un += FR_WARPS) {
+        const int j = un / kbs, kb = un - j * kbs, e = fr_expert(P, t, j);
+        if (e >= 0) { /* the same for the whole warp */
+            const float4 a = *reinterpret_cast<const float4 *>(P.act + (int64_t)(t * slots + j) * I + kb * 128 + 4 * lane);
+            const float f = (j < P.top_k ? P.weights[t * P.top_k + j] : 1.0f) *
+                            __ldg(P.dn_scales + ((int64_t)e * (H / 128) + (n0 >> 7)) * kbs + kb);
+            float amax = ops_amax(ops_amax(ops_amax(ops_amax(0.0f, a.x), a.y), a.z), a.w);
+#pragma unroll
+            for (int s = 16; s > 0; s >>= 1) amax = ops_amax(amax, __shfl_xor_sync(FULL, amax, s));
+            const float sc = ops_f8_scale(amax), inv = __frcp_rn(sc);
+            const uint32_t q = ops_f8_pack4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+            uint4 x0, x1;
+            x0.x = __shfl_sync(FULL, q, 4 * t4);
+            x0.y = __shfl_sync(FULL, q, 4 * t4 + 1);
+            x0.z = __shfl_sync(FULL, q, 4 * t4 + 2);
+            x0.w = __shfl_sync(FULL, q, 4 * t4 + 3);
+            x1.x = __shfl_sync(FULL, q, 16 + 4 * t4);
+            x1.y = __shfl_sync(FULL, q, 16 + 4 * t4 + 1);
+            x1.z = __shfl_sync(FULL, q, 16 + 4 * t4 + 2);
+            x1.w = __shfl_sync(FULL, q, 16 + 4 * t4 + 3);
+            uint4 w[4];
+            float c[4];
+            fr_take(w, ring_u + slot * 2048u);
+            fr_block(c, w, x0, x1);
+            acc[0] = fmaf(c[0], f * sc, acc[0]);
+            acc[1] = fmaf(c[2], f * sc, acc[1]);
+        } else {
+            asm volatile("cp.async.wait_group %0;" ::"n"(FR_RING - 1) : "memory");
+        }
+        ask(un + FR_WARPS * FR_RING, slot);
+        slot = (slot + 1) % FR_RING;
+    }
+    if (t4 == 0) {
+        s_part[warp][g] = acc[0];
+        s_part[warp][g + 8] = acc[1];
+    }
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < FR_WARPS; w++) v += s_part[w][threadIdx.x];
+        P.out[t * P.out_stride + n0 + threadIdx.x] = __float2bfloat16_rn(v);
+    }
 }
 
 /* ------------------------------------------------------------------ tensor maps */
@@ -637,18 +1037,30 @@ static int f8_launch(f8_args_t &p, int64_t most_tiles, int n_sm, int *launches, 
 
 extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *status, int n_sm, int *launches,
                                     void *stream) {
+    if (a->m <= 16) {
+        const fr_args_t f = {a->m, a->n, a->k, a->a, a->a_stride, a->a_scales, a->a_scales_stride, a->b, a->b_stride, a->b_scales,
+                             a->b_scales_stride, a->out, a->out_type == FOMOE_B200_BF16, a->out_stride};
+        const int grid = (a->n + 15) / 16;
+        if (a->m <= 8) k_f8_few<1><<<grid, 32 * FR_WARPS, FR_SMEM, (cudaStream_t)stream>>>(f);
+        else k_f8_few<2><<<grid, 32 * FR_WARPS, FR_SMEM, (cudaStream_t)stream>>>(f);
+        *launches += 1;
+        return (int)cudaGetLastError();
+    }
     f8_args_t p = {};
     p.m = a->m, p.n = a->n, p.k = a->k;
     p.a_scales = a->a_scales, p.as_stride = a->a_scales_stride;
     p.b_scales = a->b_scales, p.bs_stride = a->b_scales_stride;
     p.out = a->out, p.out_bf16 = a->out_type == FOMOE_B200_BF16, p.out_stride = a->out_stride;
-    p.out_vec = ((uintptr_t)a->out & 15) == 0 && (a->out_stride * (p.out_bf16 ? 2 : 4)) % 16 == 0;
+    const int eb = p.out_bf16 ? 2 : 4;
+    const int64_t os = a->m == 1 ? (int64_t)a->n * eb : a->out_stride * eb;
+    p.out_tma = ((uintptr_t)a->out & 15) == 0 && (a->m == 1 ? 1 : os % 16 == 0);
     p.status = status;
     cudaStream_t st = (cudaStream_t)stream;
     const int64_t m = a->m, n = a->n, mt = (m + 127) / 128;
     /* the widest tile that still gives every SM one: wide tiles read the least (4096 x 8192 x 4096: 148 us with 256 columns) */
     const int nt = mt * ((n + 255) / 256) >= n_sm ? 256 : mt * ((n + 127) / 128) >= n_sm ? 128 : 64;
-    const int rc = f8_map(&p.ta, a->a, a->k, a->m, a->a_stride, 32) | f8_map(&p.tb, a->b, a->k, a->n, a->b_stride, nt);
+    int rc = f8_map(&p.ta, a->a, a->k, a->m, a->a_stride, 32) | f8_map(&p.tb, a->b, a->k, a->n, a->b_stride, nt);
+    if (p.out_tma) rc |= f8_map(&p.to, a->out, (uint64_t)a->n * eb, a->m, (os + 15) & ~15ull, 32);
     if (rc) return rc;
     const int64_t tiles = mt * ((n + nt - 1) / nt);
     return nt == 256   ? f8_launch<F8_DENSE, 256>(p, tiles, n_sm, launches, st)
@@ -671,21 +1083,47 @@ __global__ void __launch_bounds__(256) k_ops_permute(const uint8_t *x, int64_t x
     for (int i = lane; i < H / 128; i += 32) xps[(int64_t)r * (H / 128) + i] = __ldg(xs + t * xs_stride + i);
 }
 
-/* ------------------------------------------------------------------ out[t] = sum over the slots, in slot order */
-__global__ void __launch_bounds__(256) k_ops_combine(const float *dots, const int *ids, const float *weights, int n_embd,
-                                                    int n_experts, int top_k, int n_routed, int has_shared,
-                                                    __nv_bfloat16 *out, int64_t out_stride) {
-    const int t = blockIdx.x;
-    for (int c = threadIdx.x; c < n_embd; c += 256) {
-        float v = 0.0f;
-        for (int j = 0; j < top_k; j++) {
-            const int p = t * top_k + j;
-            if ((unsigned)ids[p] < (unsigned)n_experts) v = fmaf(weights[p], dots[(int64_t)p * n_embd + c], v);
+/* ------------------------------------------------------------------ out[t] = sum over the slots, in slot order
+ * A thread has 8 columns; a token's rows of dots lie where its pairs were bucketed. */
+__global__ void __launch_bounds__(256) k_ops_combine(const __half *dots, const float *dot_scales, const int *pos, const int *ids,
+                                                    const float *weights, int n_embd, int n_experts, int top_k, int n_routed,
+                                                    int has_shared, __nv_bfloat16 *out, int64_t out_stride, int vec) {
+    const int t = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 8;
+    if (c >= n_embd) return;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int j = 0; j < top_k + has_shared; j++) {
+        const int p = j < top_k ? t * top_k + j : n_routed + t;
+        if (j < top_k && (unsigned)ids[p] >= (unsigned)n_experts) continue;
+        const int64_t r = pos[p];
+        const float w = (j < top_k ? weights[p] : 1.0f) * dot_scales[r * (n_embd >> 7) + (c >> 7)];
+        const uint4 u = *reinterpret_cast<const uint4 *>(dots + r * n_embd + c);
+        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x[i]));
+            v[2 * i] = fmaf(w, f.x, v[2 * i]);
+            v[2 * i + 1] = fmaf(w, f.y, v[2 * i + 1]);
         }
-        if (has_shared) v += dots[(int64_t)(n_routed + t) * n_embd + c];
-        out[t * out_stride + c] = __float2bfloat16_rn(v);
+    }
+    __nv_bfloat16 *o = out + t * out_stride + c;
+    if (vec) {
+        uint32_t x[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            x[i] = *reinterpret_cast<const uint32_t *>(&b);
+        }
+        *reinterpret_cast<uint4 *>(o) = make_uint4(x[0], x[1], x[2], x[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = __float2bfloat16_rn(v[i]);
     }
 }
+
+/* up to this many pairs each pair reads its own expert's weights */
+#ifndef EXPERTS_FEW
+#define EXPERTS_FEW 32
+#endif
 
 extern "C" void ops_experts_layout(const fomoe_b200_f8_experts_args_t *a, ops_experts_ws_t *w) {
     const uint64_t np = (uint64_t)a->n_tokens * (a->top_k + (a->has_shared ? 1 : 0));
@@ -694,12 +1132,16 @@ extern "C" void ops_experts_layout(const fomoe_b200_f8_experts_args_t *a, ops_ex
 #define PART(name, n) w->name = at, at += ((uint64_t)(n) + 255) & ~255ull
     w->n_pairs = (int)np;
     PART(counts, 256 + 16 * items); /* {tiles, routed pairs}, then the tiles */
+    PART(block_counts, 4ull * BK_BLOCKS * a->n_experts);
     PART(pairs, 4 * np);
+    PART(pos, 4 * np);
     PART(xp, np * a->n_embd);
     PART(xp_scales, np * (a->n_embd / 128) * 4);
     PART(act_q, np * a->n_inter);
     PART(act_scales, np * (a->n_inter / 128) * 4);
-    PART(dots, np * a->n_embd * 4);
+    /* (the activations in fp32 where there are few pairs) */
+    PART(dots, np * (a->n_embd > 2 * a->n_inter ? a->n_embd * 2ull : a->n_inter * 4ull));
+    PART(dot_scales, np * (a->n_embd / 128) * 4);
 #undef PART
     w->bytes = at;
 }
@@ -709,12 +1151,31 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     cudaStream_t st = (cudaStream_t)stream;
     ops_experts_ws_t w;
     ops_experts_layout(a, &w);
+    const int few_slots = a->top_k + (a->has_shared ? 1 : 0);
+    if (w.n_pairs <= EXPERTS_FEW) {
+        const fr_experts_t f = {a->n_embd, a->n_inter, a->n_experts, a->top_k, a->has_shared ? 1 : 0, a->n_tokens * a->top_k, a->x,
+                                a->x_stride, a->x_scales, a->x_scales_stride, a->ids, a->weights, a->gate_up, a->down,
+                                a->gate_up_scales, a->down_scales, (float *)(ws + w.dots), (__nv_bfloat16 *)a->out, a->out_stride, status};
+        k_f8_few_gate_up<<<dim3(a->n_inter / 16, few_slots, a->n_tokens), 32 * FR_WARPS, FR_SMEM, st>>>(f);
+        k_f8_few_down<<<dim3(a->n_embd / 16, a->n_tokens), 32 * FR_WARPS, FR_SMEM, st>>>(f);
+        *launches += 2;
+        return (int)cudaGetLastError();
+    }
     const int n_routed = a->n_tokens * a->top_k, n_shared = a->has_shared ? a->n_tokens : 0, H = a->n_embd, I = a->n_inter;
-    int *counts = (int *)(ws + w.counts), *pairs = (int *)(ws + w.pairs);
+    int *counts = (int *)(ws + w.counts), *pairs = (int *)(ws + w.pairs), *pos = (int *)(ws + w.pos);
     int4 *items = (int4 *)(ws + w.counts + 256);
     const int64_t recs = a->n_experts + (a->has_shared ? 1 : 0);
-    k_ops_bucket<<<1, BK_THREADS, (size_t)a->n_experts * BK_WARPS * 4, st>>>(
-        a->ids, n_routed, a->n_tokens, a->n_experts, a->has_shared, counts, pairs, items, status);
+    int run = (n_routed + BK_BLOCKS - 1) / BK_BLOCKS;
+    run = run < BK_RUN ? BK_RUN : run;
+    const int nb = (n_routed + run - 1) / run, bk_smem = a->n_experts * (BK_WARPS + 1) * 4;
+    int *block_counts = (int *)(ws + w.block_counts);
+    if (nb > 1) {
+        k_ops_bucket<true><<<nb, BK_THREADS, bk_smem, st>>>(a->ids, n_routed, run, a->n_tokens, a->n_experts, a->has_shared,
+                                                          block_counts, counts, pairs, pos, items, status);
+        *launches += 1;
+    }
+    k_ops_bucket<false><<<nb, BK_THREADS, bk_smem, st>>>(a->ids, n_routed, run, a->n_tokens, a->n_experts, a->has_shared,
+                                                       block_counts, counts, pairs, pos, items, status);
     k_ops_permute<<<(w.n_pairs + 7) / 8, 256, 0, st>>>(a->x, a->x_stride, a->x_scales, a->x_scales_stride, H, counts, pairs,
                                                       n_routed, a->top_k, n_shared, ws + w.xp, (float *)(ws + w.xp_scales));
     *launches += 2;
@@ -734,13 +1195,20 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     p.n = H, p.k = I;
     p.a_scales = p.act_scales, p.as_stride = I / 128;
     p.b_scales = a->down_scales, p.bs_stride = I / 128, p.bs_rec = (int64_t)(H / 128) * (I / 128), p.b_rec_rows = H;
-    p.out = ws + w.dots, p.out_stride = H, p.out_vec = 1;
-    rc = f8_map(&p.ta, ws + w.act_q, I, w.n_pairs, I, 32) | f8_map(&p.tb, a->down, I, recs * H, I, 256);
+    p.out = ws + w.dots, p.out_stride = H, p.out_tma = 1, p.out_scales = (float *)(ws + w.dot_scales);
+    rc = f8_map(&p.ta, ws + w.act_q, I, w.n_pairs, I, 32) | f8_map(&p.tb, a->down, I, recs * H, I, 256) |
+         f8_map(&p.to, ws + w.dots, 2ull * H, w.n_pairs, 2ull * H, 32);
     if (!rc) rc = f8_launch<F8_DOWN, 256>(p, tiles * ((H + 255) / 256), n_sm, launches, st);
     if (rc) return rc;
-    k_ops_combine<<<a->n_tokens, 256, 0, st>>>((const float *)(ws + w.dots), a->ids, a->weights, H, a->n_experts, a->top_k,
-                                              n_routed, a->has_shared, (__nv_bfloat16 *)a->out, a->out_stride);
-    *launches += 1;
+    const int vec = ((uintptr_t)a->out & 15) == 0 && (a->n_tokens == 1 || a->out_stride % 8 == 0);
+    /* (the grid's y goes to 65535) */
+    for (int t0 = 0; t0 < a->n_tokens; t0 += 65535) {
+        const int nt = a->n_tokens - t0 < 65535 ? a->n_tokens - t0 : 65535, p0 = t0 * a->top_k;
+        k_ops_combine<<<dim3((H / 8 + 255) / 256, nt), 256, 0, st>>>(
+            (const __half *)(ws + w.dots), (const float *)(ws + w.dot_scales), pos + p0, a->ids + p0, a->weights + p0, H, a->n_experts,
+            a->top_k, n_routed + t0 - p0, a->has_shared, (__nv_bfloat16 *)a->out + t0 * a->out_stride, a->out_stride, vec);
+        *launches += 1;
+    }
     return (int)cudaGetLastError();
 }
 
@@ -758,10 +1226,14 @@ extern "C" int ops_f8_init(void) {
 #define RK(k) rc |= (int)cudaFuncGetAttributes(&f, (k))
 #define RM(MODE, NT)                                                                                             \
     rc |= (int)cudaFuncSetAttribute(k_f8_mma<MODE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, f8_cfg<MODE, NT>::SMEM)
-    RK(k_ops_combine); RK(k_ops_bucket); RK(k_ops_permute);
+    RK(k_ops_combine); RK(k_ops_permute);
+#define RF(k) rc |= (int)cudaFuncSetAttribute((k), cudaFuncAttributeMaxDynamicSharedMemorySize, FR_SMEM)
+    RF(k_f8_few<1>); RF(k_f8_few<2>); RF(k_f8_few_gate_up); RF(k_f8_few_down);
+#undef RF
     RM(F8_DENSE, 256); RM(F8_DENSE, 128); RM(F8_DENSE, 64); RM(F8_GATE_UP, 256); RM(F8_DOWN, 256);
 #undef RM
 #undef RK
-    rc |= (int)cudaFuncSetAttribute(k_ops_bucket, cudaFuncAttributeMaxDynamicSharedMemorySize, OPS_MAX_E * BK_WARPS * 4);
+    rc |= (int)cudaFuncSetAttribute(k_ops_bucket<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, OPS_MAX_E * (BK_WARPS + 1) * 4);
+    rc |= (int)cudaFuncSetAttribute(k_ops_bucket<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, OPS_MAX_E * (BK_WARPS + 1) * 4);
     return rc;
 }

@@ -18,152 +18,329 @@
 #endif
 
 /* ------------------------------------------------------------------ routing: one warp per token
- * Lane l holds experts l, l + 32, ... .  Everything that decides an order is computed in 64 bits. */
+ * Lane l holds experts l, l + 32, ... .  The order is the order of exact values.  Without a bias that is the logits' order,
+ * which fp32 holds exactly; choices p + bias and scores of groups are computed in fp32, and where two that a decision hangs on
+ * are closer than their errors allow (RT_NEAR) the warp repeats that decision in 64 bits.
+ *
+ * Error of a choice: p is an exp of an argument d rounded to |d| U (U = 2^-24; |d| e^-d < 0.4) by way of 2^x (3 U), a sum
+ * and a quotient, 1e-6 of at most 1; the addition of the bias half a step of the choice, 6e-8 |c|.  Twice that for a
+ * difference, four times for sums of two: RT_NEAR covers both with a factor of two to spare.
+ *
+ * The best K + 1 keys: each lane's best key first; the (K + 1)-th best of those is a bound that every one of the best K + 1
+ * keys reaches, and few others do.  The keys that reach it are put side by side in shared memory, one to a lane, and each
+ * counts how many are better.  (16,384 tokens x 384 experts, sigmoid + bias, top 8: 87 us in 64 bits with a round over all
+ * keys for every slot) */
 #define RT_WARPS 4
+#define RT_NEAR(a, b) (8e-6f + 1e-6f * (fabsf(a) + fabsf(b)))
 
-__device__ __forceinline__ bool rt_better(double v, int i, double w, int j) { return v > w || (v == w && i < j); }
+/* floats as unsigned numbers in the same order; 0 stands for "closed" (below -inf) */
+__device__ __forceinline__ uint32_t rt_key(float v) {
+    const uint32_t u = __float_as_uint(v == 0.0f ? 0.0f : v); /* (-0 is 0) */
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float rt_val(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 
-__device__ __forceinline__ void rt_warp_best(double &v, int &i) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const double ov = __shfl_xor_sync(FULL, v, o);
-        const int oi = __shfl_xor_sync(FULL, i, o);
-        if (rt_better(ov, oi, v, i)) {
-            v = ov;
-            i = oi;
+/* The best and the second best of every group, by the 32 / 2^ceil(log2 G) lanes that share a group; the group's first lane
+ * (g << shift) has them.  c: the choices, -inf where closed. */
+template <typename T>
+__device__ __forceinline__ T rt_group_score(const T *c, int G, int per, int best, int shift) {
+    const int lane = threadIdx.x & 31, g = lane >> shift, L = 1 << shift;
+    const T NINF = -INFINITY;
+    T a = NINF, b = NINF;
+    if (g < G)
+        for (int i = lane & (L - 1); i < per; i += L) {
+            const T v = c[g * per + i];
+            b = v > a ? a : v > b ? v : b;
+            a = v > a ? v : a;
+        }
+    for (int s = L >> 1; s > 0; s >>= 1) {
+        const T oa = __shfl_xor_sync(FULL, a, s), ob = __shfl_xor_sync(FULL, b, s);
+        b = a > oa ? (oa > b ? oa : b) : (a > ob ? a : ob);
+        a = a > oa ? a : oa;
+    }
+    return best == 2 && b > NINF ? a + b : a;
+}
+
+/* mask of the groups that stay: those with fewer than topk better ones (lower group first among equals) */
+template <typename T>
+__device__ __forceinline__ uint32_t rt_groups_stay(T gs, int G, int topk, int shift) {
+    const int lane = threadIdx.x & 31, g = lane >> shift;
+    int rank = 0;
+    for (int h = 0; h < G; h++) {
+        const T o = __shfl_sync(FULL, gs, h << shift);
+        rank += o > gs || (o == gs && h < g);
+    }
+    const uint32_t m = __ballot_sync(FULL, (lane & ((1 << shift) - 1)) == 0 && g < G && rank < topk);
+    uint32_t keep = 0;
+    for (int h = 0; h < G; h++) keep |= ((m >> (h << shift)) & 1u) << h;
+    return keep;
+}
+
+__device__ __forceinline__ float rt_logit(const ops_route_t &A, int t, int e) {
+    const int64_t at = (int64_t)t * A.row_stride + e;
+    return A.logits_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(A.logits)[at])
+                         : reinterpret_cast<const float *>(A.logits)[at];
+}
+
+/* The choices in 64 bits, to c[0 .. E) (-inf where closed).  Rare: written for size. */
+__device__ __noinline__ void rt_exact_choices(const ops_route_t &A, int t, bool shut, float mx, double *c) {
+    const int lane = threadIdx.x & 31, E = A.cfg.n_experts;
+    double sum = 0.0;
+    for (int e = lane; e < E; e += 32) {
+        const float v = rt_logit(A, t, e);
+        const bool open = !shut && v > -INFINITY;
+        const double x = fmin((double)v, (double)FLT_MAX);
+        double p = 0.0;
+        if (open) p = A.cfg.score == FOMOE_B200_SOFTMAX ? exp(x - (double)mx) : 1.0 / (1.0 + exp(-x));
+        sum += p;
+        c[e] = open ? p : -INFINITY;
+    }
+    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(FULL, sum, s);
+    for (int e = lane; e < E; e += 32) {
+        double v = c[e];
+        if (v > -INFINITY) {
+            if (A.cfg.score == FOMOE_B200_SOFTMAX) v /= sum;
+            if (A.bias) v += (double)A.bias[e];
+            c[e] = v > -INFINITY ? v : -INFINITY;
         }
     }
+    __syncwarp();
+}
+
+/* The choice of expert e in 64 bits (the whole warp calls it: softmax needs the sum over all experts). */
+__device__ __noinline__ double rt_exact_choice(const ops_route_t &A, int t, bool shut, float mx, int e) {
+    const int lane = threadIdx.x & 31, E = A.cfg.n_experts;
+    const bool softmax = A.cfg.score == FOMOE_B200_SOFTMAX;
+    double sum = 0.0;
+    if (softmax) {
+        for (int i = lane; i < E; i += 32) {
+            const float v = rt_logit(A, t, i);
+            if (!shut && v > -INFINITY) sum += exp(fmin((double)v, (double)FLT_MAX) - (double)mx);
+        }
+        for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(FULL, sum, s);
+    }
+    if (e < 0) return -INFINITY;
+    const double x = fmin((double)rt_logit(A, t, e), (double)FLT_MAX);
+    return (softmax ? exp(x - (double)mx) / sum : 1.0 / (1.0 + exp(-x))) + (double)A.bias[e];
+}
+
+/* the top_k of c by rounds over all of it; closed: what is never chosen; lane r gets the id of slot r */
+template <typename T>
+__device__ __noinline__ int rt_top(T *c, T closed, int E, int K, uint32_t keep, int per) {
+    const int lane = threadIdx.x & 31;
+    int my_id = -1;
+    for (int r = 0; r < K; r++) {
+        T v = closed;
+        int i = OPS_MAX_E;
+        for (int e = lane; e < E; e += 32)
+            if (c[e] > v && ((keep >> (e / per)) & 1u)) {
+                v = c[e];
+                i = e;
+            }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const T ov = __shfl_xor_sync(FULL, v, o);
+            const int oi = __shfl_xor_sync(FULL, i, o);
+            if (ov > v || (ov == v && oi < i)) {
+                v = ov;
+                i = oi;
+            }
+        }
+        if (i == OPS_MAX_E) break;
+        if (lane == r) my_id = i;
+        __syncwarp();
+        if (lane == 0) c[i] = closed;
+        __syncwarp();
+    }
+    return my_id;
+}
+
+__device__ __forceinline__ float rt_sigmoid(float x) { /* (x = -inf: 0) */
+    const float e = __expf(-fabsf(x)), q = __fdividef(1.0f, 1.0f + e);
+    return x >= 0.0f ? q : e * q;
 }
 
 template <int NPL>
-__global__ void __launch_bounds__(32 * RT_WARPS) k_ops_route(ops_route_t A) {
+__global__ void __launch_bounds__(32 * RT_WARPS) k_ops_route(const __grid_constant__ ops_route_t A) {
     __shared__ double s_c[RT_WARPS][OPS_MAX_E];
+    __shared__ uint2 s_best[RT_WARPS][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int t = blockIdx.x * RT_WARPS + warp;
     if (t >= A.n_tokens) return;
     const int E = A.cfg.n_experts, K = A.cfg.top_k, G = A.cfg.n_group;
-    const bool shut = A.valid && A.valid[t] == 0;
-    const double NINF = -INFINITY;
+    const bool shut = A.valid && A.valid[t] == 0, softmax = A.cfg.score == FOMOE_B200_SOFTMAX;
     float x[NPL];
+    if (A.logits_bf16) { /* (all loads first) */
+        const uint16_t *p = reinterpret_cast<const uint16_t *>(A.logits) + (int64_t)t * A.row_stride;
+#pragma unroll
+        for (int j = 0; j < NPL; j++) x[j] = __uint_as_float((uint32_t)__ldg(p + min(j * 32 + lane, E - 1)) << 16);
+    } else {
+        const float *p = reinterpret_cast<const float *>(A.logits) + (int64_t)t * A.row_stride;
+#pragma unroll
+        for (int j = 0; j < NPL; j++) x[j] = __ldg(p + min(j * 32 + lane, E - 1));
+    }
+    float mx = -INFINITY, inv = 1.0f;
 #pragma unroll
     for (int j = 0; j < NPL; j++) {
-        const int e = j * 32 + lane;
-        x[j] = -INFINITY;
-        if (e < E && !shut) {
-            const int64_t at = (int64_t)t * A.row_stride + e;
-            const float v = A.logits_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(A.logits)[at])
-                                          : reinterpret_cast<const float *>(A.logits)[at];
-            if (v > -INFINITY) x[j] = fminf(v, FLT_MAX);
-        }
+        x[j] = j * 32 + lane < E && !shut && x[j] > -INFINITY ? fminf(x[j], FLT_MAX) : -INFINITY;
+        mx = fmaxf(mx, x[j]);
     }
-    /* p, and the order key o: the choice, or without a bias the logit itself */
-    double p[NPL], o[NPL];
-    if (A.cfg.score == FOMOE_B200_SOFTMAX) {
-        float mx = -INFINITY;
+    uint32_t key[NPL]; /* the choice, or without a bias the logit itself */
+    const bool need_p = A.bias || G > 1;
+    if (softmax) {
 #pragma unroll
-        for (int j = 0; j < NPL; j++) mx = fmaxf(mx, x[j]);
         for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, s));
-        double sum = 0.0;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NPL; j++) sum += x[j] > -INFINITY ? __expf(x[j] - mx) : 0.0f;
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(FULL, sum, s);
+        inv = sum > 0.0f ? __fdiv_rn(1.0f, sum) : 0.0f;
+    }
+    if (need_p) {
 #pragma unroll
         for (int j = 0; j < NPL; j++) {
-            p[j] = x[j] > -INFINITY ? exp((double)x[j] - (double)mx) : 0.0;
-            sum += p[j];
+            const int e = j * 32 + lane;
+            const bool open = x[j] > -INFINITY;
+            float c = softmax ? __expf(x[j] - mx) * inv : rt_sigmoid(x[j]);
+            if (A.bias) c += __ldg(A.bias + min(e, E - 1));
+            c = open && c > -INFINITY ? c : -INFINITY;
+            key[j] = A.bias ? (c > -INFINITY ? rt_key(c) : 0u) : (open ? rt_key(x[j]) : 0u);
+            if (G > 1 && e < E) reinterpret_cast<float *>(s_c[warp])[e] = c;
         }
-        for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(FULL, sum, s);
-#pragma unroll
-        for (int j = 0; j < NPL; j++) p[j] = sum > 0.0 ? p[j] / sum : 0.0;
     } else {
 #pragma unroll
-        for (int j = 0; j < NPL; j++) p[j] = x[j] > -INFINITY ? 1.0 / (1.0 + exp(-(double)x[j])) : 0.0;
+        for (int j = 0; j < NPL; j++) key[j] = x[j] > -INFINITY ? rt_key(x[j]) : 0u;
     }
-#pragma unroll
-    for (int j = 0; j < NPL; j++) {
-        const int e = j * 32 + lane;
-        o[j] = NINF;
-        if (x[j] > -INFINITY) {
-            const double c = A.bias ? p[j] + (double)A.bias[e] : p[j];
-            if (c > NINF) o[j] = A.bias ? c : (double)x[j];
-            if (G > 1) s_c[warp][e] = c > NINF ? c : NINF;
-        } else if (G > 1 && e < E) {
-            s_c[warp][e] = NINF;
-        }
-    }
-    if (G > 1) { /* lane g scores group g; then the topk_group best stay */
+    const int per = E / G;
+    uint32_t keep = 0xffffffffu;
+    if (G > 1) {
         __syncwarp();
-        const int per = E / G;
-        double g1 = NINF, g2 = NINF;
-        if (lane < G)
-            for (int i = 0; i < per; i++) {
-                const double c = s_c[warp][lane * per + i];
-                if (c > g1) {
-                    g2 = g1;
-                    g1 = c;
-                } else if (c > g2) {
-                    g2 = c;
-                }
-            }
-        double gs = A.cfg.group_best == 2 && g2 > NINF ? g1 + g2 : g1;
-        bool taken = lane >= G;
-        uint32_t keep = 0;
-        for (int r = 0; r < A.cfg.topk_group; r++) {
-            double v = taken ? NINF : gs;
-            int i = taken ? 64 : lane;
-            rt_warp_best(v, i);
-            if (lane == i) taken = true;
-            if (i < 32) keep |= 1u << i;
+        const int shift = 5 - (32 - __clz(G - 1)); /* lanes of a group, as a power of two */
+        const float gs = rt_group_score(reinterpret_cast<const float *>(s_c[warp]), G, per, A.cfg.group_best, shift);
+        keep = rt_groups_stay(gs, G, A.cfg.topk_group, shift);
+        /* does the cut pass between two scores that are too close? */
+        const bool mine = (keep >> min(lane >> shift, 31)) & 1u;
+        bool near = false;
+        for (int h = 0; h < G; h++) {
+            const float o = __shfl_sync(FULL, gs, h << shift);
+            near |= (lane >> shift) < G && mine && !((keep >> h) & 1u) && o > -INFINITY && !(gs - o > 2.0f * RT_NEAR(gs, o));
+        }
+        if (__any_sync(FULL, near)) {
+            rt_exact_choices(A, t, shut, mx, s_c[warp]);
+            keep = rt_groups_stay(rt_group_score(s_c[warp], G, per, A.cfg.group_best, shift), G, A.cfg.topk_group, shift);
         }
 #pragma unroll
         for (int j = 0; j < NPL; j++) {
             const int e = j * 32 + lane;
-            if (e < E && !((keep >> (e / per)) & 1u)) o[j] = NINF;
+            if (e < E && !((keep >> (e / per)) & 1u)) key[j] = 0;
         }
     }
-    double my_p = 0.0;
-    int my_id = -1;
-    for (int r = 0; r < K; r++) {
-        double v = NINF, pv = 0.0;
-        int i = OPS_MAX_E;
+    uint32_t best = 0;
+#pragma unroll
+    for (int j = 0; j < NPL; j++) best = max(best, key[j]);
+    uint32_t bound = 1;
+    for (int r = 0; r <= K; r++) { /* (equal ones of several lanes go together: the bound is only lower for it) */
+        const uint32_t w = __reduce_max_sync(FULL, best);
+        if (w == 0) {
+            bound = 1;
+            break;
+        }
+        bound = w;
+        best = best == w ? 0u : best;
+    }
+    if (A.bias && bound > 1) { /* and those that may be as good for all fp32 can say */
+        const float v = rt_val(bound), low = v - RT_NEAR(v, v);
+        bound = low > -INFINITY ? rt_key(low) : 1u; /* (infinite choices: all that is open) */
+    }
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < NPL; j++) {
+        const bool in = key[j] >= bound;
+        const uint32_t m = __ballot_sync(FULL, in);
+        const int at = n + __popc(m & ((1u << lane) - 1u));
+        if (in && at < 32) s_best[warp][at] = make_uint2(key[j], (uint32_t)(j * 32 + lane));
+        n += __popc(m);
+    }
+    __syncwarp();
+    int slot = lane, id = -1; /* this lane writes slot `slot`, if there is one */
+    bool exact = false;
+    if (n <= 32) {
+        const uint2 own = lane < n ? s_best[warp][lane] : make_uint2(0u, 0u);
+        int rank = 0;
+        for (int i = 0; i < n; i++) {
+            const uint2 o = s_best[warp][i];
+            rank += o.x > own.x || (o.x == own.x && o.y < own.y);
+        }
+        __syncwarp();
+        if (lane < n) { /* (lanes behind the candidates keep their own slot: empty) */
+            slot = rank;
+            id = (int)own.y;
+            s_best[warp][rank] = own;
+        }
+        __syncwarp();
+        if (A.bias) { /* neighbours among the best K + 1 that are too close? */
+            bool near = false;
+            if (lane < K && lane + 1 < n) {
+                const float a = rt_val(s_best[warp][lane].x), b = rt_val(s_best[warp][lane + 1].x);
+                near = !(a - b > RT_NEAR(a, b));
+            }
+            if (__any_sync(FULL, near)) { /* rank the candidates again, by their exact choices */
+                id = lane < n ? (int)own.y : -1;
+                const double c = rt_exact_choice(A, t, shut, mx, id);
+                rank = 0;
+                for (int i = 0; i < n; i++) {
+                    const double oc = __shfl_sync(FULL, c, i);
+                    const int oi = __shfl_sync(FULL, id, i);
+                    rank += oc > c || (oc == c && oi < id);
+                }
+                slot = lane < n ? rank : lane;
+            }
+        }
+    } else if (!A.bias) { /* more equal keys than lanes */
+        uint32_t *c = reinterpret_cast<uint32_t *>(s_c[warp]);
 #pragma unroll
         for (int j = 0; j < NPL; j++)
-            if (o[j] > v) {
-                v = o[j];
-                i = j * 32 + lane;
-                pv = p[j];
-            }
-        const int mine = i;
-        rt_warp_best(v, i);
-        if (i == OPS_MAX_E) break; /* no open expert left */
-        const double wp = __shfl_sync(FULL, pv, i & 31);
-        if (mine == i) {
-#pragma unroll
-            for (int j = 0; j < NPL; j++)
-                if (j == (i >> 5)) o[j] = NINF;
-        }
-        if (lane == r) {
-            my_id = i;
-            my_p = wp;
-        }
+            if (j * 32 + lane < E) c[j * 32 + lane] = key[j];
+        __syncwarp();
+        id = rt_top<uint32_t>(c, 0u, E, K, keep, per);
+    } else {
+        exact = true;
+    }
+    if (exact) {
+        rt_exact_choices(A, t, shut, mx, s_c[warp]);
+        slot = lane;
+        id = rt_top<double>(s_c[warp], (double)-INFINITY, E, K, keep, per);
+    }
+    float p = 0.0f;
+    if (slot < K && id >= 0) {
+        const float v = fminf(rt_logit(A, t, id), FLT_MAX);
+        p = softmax ? __expf(v - mx) * inv : rt_sigmoid(v);
     }
     if (A.cfg.renorm) {
-        double s = my_p;
+        float s = p;
+#pragma unroll
         for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(FULL, s, d);
-        my_p = my_p / (s + 1e-20);
+        p = __fdiv_rn(p, s + 1e-20f);
     }
-    if (lane < K) {
-        A.ids[(int64_t)t * K + lane] = my_id;
-        A.weights[(int64_t)t * K + lane] = (float)(my_p * (double)A.cfg.scale);
+    if (slot < K) {
+        A.ids[(int64_t)t * K + slot] = id;
+        A.weights[(int64_t)t * K + slot] = p * A.cfg.scale;
     }
 }
 
+#define RT_SIZES(X) X(1) X(2) X(4) X(6) X(8) X(12) X(16) /* experts of a lane */
+
 extern "C" int ops_launch_route(const ops_route_t *a, void *stream) {
     const int grid = (a->n_tokens + RT_WARPS - 1) / RT_WARPS, E = a->cfg.n_experts;
-    cudaStream_t st = (cudaStream_t)stream;
-    if (E <= 32) k_ops_route<1><<<grid, 32 * RT_WARPS, 0, st>>>(*a);
-    else if (E <= 64) k_ops_route<2><<<grid, 32 * RT_WARPS, 0, st>>>(*a);
-    else if (E <= 128) k_ops_route<4><<<grid, 32 * RT_WARPS, 0, st>>>(*a);
-    else if (E <= 256) k_ops_route<8><<<grid, 32 * RT_WARPS, 0, st>>>(*a);
-    else k_ops_route<16><<<grid, 32 * RT_WARPS, 0, st>>>(*a);
-    return (int)cudaGetLastError();
+#define RT_GO(N)                                                                \
+    if (E <= 32 * N) {                                                          \
+        k_ops_route<N><<<grid, 32 * RT_WARPS, 0, (cudaStream_t)stream>>>(*a); \
+        return (int)cudaGetLastError();                                         \
+    }
+    RT_SIZES(RT_GO)
+#undef RT_GO
+    return (int)cudaErrorInvalidValue;
 }
 
 /* ------------------------------------------------------------------ norms around a block
@@ -421,7 +598,9 @@ extern "C" int ops_rows_init(void) {
     cudaFuncAttributes f;
     int rc = 0;
 #define RK(k) rc |= (int)cudaFuncGetAttributes(&f, (k))
-    RK(k_ops_route<1>); RK(k_ops_route<2>); RK(k_ops_route<4>); RK(k_ops_route<8>); RK(k_ops_route<16>);
+#define RT_RK(N) RK(k_ops_route<N>);
+    RT_SIZES(RT_RK)
+#undef RT_RK
     RK((k_ops_norm<true, 32, 1>)); RK((k_ops_norm<true, 32, 2>)); RK((k_ops_norm<true, 256, 1>));
     RK((k_ops_norm<true, 256, 2>)); RK((k_ops_norm<true, 256, 4>)); RK((k_ops_norm<true, 256, 8>));
     RK((k_ops_norm<false, 32, 1>)); RK((k_ops_norm<false, 32, 2>)); RK((k_ops_norm<false, 256, 1>));
