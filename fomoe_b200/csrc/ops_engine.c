@@ -14,7 +14,8 @@
 #include "ops_launch.h"
 
 struct fomoe_b200_ops {
-    int device, n_sm;
+    int device;
+    ops_device_t dev;
     volatile int *status; /* mapped host memory: kernels store into it, the host reads it without a copy */
     int *status_dev;
     uint64_t launches;
@@ -46,10 +47,10 @@ fomoe_b200_ops_t *fomoe_b200_ops_create(int device) {
     o->device = device;
     int ok = cudaSetDevice(device) == cudaSuccess &&
              cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) == cudaSuccess && major == 10 &&
-             cudaDeviceGetAttribute(&o->n_sm, cudaDevAttrMultiProcessorCount, device) == cudaSuccess &&
+             cudaDeviceGetAttribute(&o->dev.n_sm, cudaDevAttrMultiProcessorCount, device) == cudaSuccess &&
              cudaHostAlloc((void **)&o->status, 64, cudaHostAllocMapped) == cudaSuccess &&
              cudaHostGetDevicePointer((void **)&o->status_dev, (void *)o->status, 0) == cudaSuccess &&
-             ops_rows_init() == 0 && ops_f8_init() == 0;
+             ops_rows_init() == 0 && ops_f8_init(&o->dev) == 0;
     if (ok) {
         *o->status = FB_ST_OK;
     } else {
@@ -189,7 +190,7 @@ int fomoe_b200_ops_f8_matmul(fomoe_b200_ops_t *o, const fomoe_b200_f8_matmul_arg
     NEED(o, is_float(a->out_type) && fits(a->out, a->out_type) && fits(a->a_scales, FOMOE_B200_F32) && fits(a->b_scales, FOMOE_B200_F32), "f8_matmul: out is F32 or BF16, pointers aligned to their types");
     NEED(o, a->out_stride >= a->n || a->m == 1, "f8_matmul: out_stride is below n");
     int n = 0;
-    ON_DEVICE(o, "f8_matmul", n, ops_launch_f8_matmul(a, o->status_dev, o->n_sm, &n, stream));
+    ON_DEVICE(o, "f8_matmul", n, ops_launch_f8_matmul(a, o->status_dev, &o->dev, &n, stream));
     return 0;
 }
 
@@ -221,6 +222,6 @@ int fomoe_b200_ops_f8_experts(fomoe_b200_ops_t *o, const fomoe_b200_f8_experts_a
     NEED(o, workspace && ((uintptr_t)workspace & 255) == 0, "f8_experts: the workspace is NULL or not 256-byte aligned");
     NEED(o, workspace_bytes >= fomoe_b200_ops_f8_experts_workspace(a), "f8_experts: the workspace has %llu bytes, %llu are needed", (unsigned long long)workspace_bytes, (unsigned long long)fomoe_b200_ops_f8_experts_workspace(a));
     int n = 0;
-    ON_DEVICE(o, "f8_experts", n, ops_launch_f8_experts(a, (uint8_t *)workspace, o->status_dev, o->n_sm, &n, stream));
+    ON_DEVICE(o, "f8_experts", n, ops_launch_f8_experts(a, (uint8_t *)workspace, o->status_dev, &o->dev, &n, stream));
     return 0;
 }

@@ -267,6 +267,23 @@ __device__ __forceinline__ void f8_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+__device__ __forceinline__ uint32_t f8_cluster_size() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t f8_cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+/* (not a bounded wait: every thread of every block of the cluster comes here, whatever ran out before) */
+__device__ __forceinline__ void f8_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 /* a box of the map to shared memory */
 __device__ __forceinline__ void f8_tma2(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
     asm volatile(
@@ -303,7 +320,7 @@ template <int MODE, int NT>
 struct f8_cfg {
     static constexpr int B_BYTES = NT * 128;
     static constexpr int STAGE = (int)F8_A_BYTES + B_BYTES;
-    static constexpr int STAGES = NT == 256 ? (MODE == F8_GATE_UP ? 4 : 3) : NT == 128 ? 5 : 7;
+    static constexpr int STAGES = NT == 256 ? (MODE == F8_GATE_UP ? 4 : 3) : 5;
     static constexpr int NB = NT == 256 ? 2 : 4;
     static constexpr int BUFS = MODE == F8_GATE_UP ? 0 : NT == 256 ? 2 : 1; /* a warp's staging buffers of 32 rows x 128 bytes */
     static constexpr int OUT = F8_EPI_WARPS * BUFS * 4096;
@@ -388,7 +405,7 @@ __device__ __forceinline__ void f8_box_wait() {
     __syncwarp();
 }
 
-template <int MODE, int NT>
+template <int MODE, int NT, bool SPLIT>
 __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant__ f8_args_t P) {
     typedef f8_cfg<MODE, NT> cfg;
     constexpr int STAGES = cfg::STAGES, NB = cfg::NB;
@@ -398,7 +415,11 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
     f8_ctl_t *C = reinterpret_cast<f8_ctl_t *>(dyn_raw + (dyn_u - fb_smem_u32(dyn_raw)) + STAGES * cfg::STAGE + cfg::OUT);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int per_n = MODE == F8_GATE_UP ? NT / 2 : NT;
-    const int n_tiles = (P.n + per_n - 1) / per_n, kbs = (P.k + 127) / 128;
+    const int n_tiles = (P.n + per_n - 1) / per_n;
+    /* this block's blocks of k: all, or (SPLIT) its rank's share; the cluster's blocks have one tile */
+    const uint32_t ranks = SPLIT ? f8_cluster_size() : 1, rank = SPLIT ? f8_cluster_rank() : 0;
+    const int kb_all = (P.k + 127) / 128, kb_lo = (int)(rank * kb_all / ranks), kbs = (int)((rank + 1) * kb_all / ranks) - kb_lo;
+    const int first = (int)(blockIdx.x / ranks), stride = (int)(gridDim.x / ranks);
     const int tiles = (MODE == F8_DENSE ? (P.m + 127) / 128 : P.counts[0]) * n_tiles;
 
     if (tid == 0) {
@@ -435,7 +456,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             /* ---------------- operand tiles */
             uint32_t st = 0, ph = 0; /* stage, and the parity of its phase */
             bool ok = true;
-            for (int it = blockIdx.x; it < tiles && ok; it += gridDim.x) {
+            for (int it = first; it < tiles && ok; it += stride) {
                 const f8_tile_t t = f8_tile<MODE, NT>(P, it, n_tiles);
                 /* boxes of 32 rows, as many as the rows need; what is behind the tile's rows is never stored */
                 const int groups = (t.rows + 31) / 32, y = t.e * P.b_rec_rows + t.n0;
@@ -448,10 +469,11 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     }
                     if (f8_elect()) {
                         const uint32_t bar = fb_smem_u32(&C->full[st]);
+                        const int x = (kb_lo + kb) * 128;
                         fb_mbar_expect_tx(bar, bytes);
-                        f8_tma2(b_u, &P.tb, kb * 128, y, bar);
-                        if (MODE == F8_GATE_UP) f8_tma2(b_u + 16384u, &P.tb, kb * 128, y + P.n, bar);
-                        for (int g = 0; g < groups; g++) f8_tma2(a_u + g * 4096u, &P.ta, kb * 128, t.r0 + 32 * g, bar);
+                        f8_tma2(b_u, &P.tb, x, y, bar);
+                        if (MODE == F8_GATE_UP) f8_tma2(b_u + 16384u, &P.tb, x, y + P.n, bar);
+                        for (int g = 0; g < groups; g++) f8_tma2(a_u + g * 4096u, &P.ta, x, t.r0 + 32 * g, bar);
                     }
                     __syncwarp();
                     if (++st == STAGES) {
@@ -473,7 +495,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             const uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             uint32_t st = 0, ph = 0, b = 0, bph = 0, have_ab = 0, have_acc = 0;
             bool ok = true;
-            for (int it = blockIdx.x; it < tiles && ok; it += gridDim.x)
+            for (int it = first; it < tiles && ok; it += stride)
                 for (int kb = 0; kb < kbs; kb++) {
                     if ((!__all_sync(FULL, have_ab) && !f8_wait_all(fb_smem_u32(&C->full[st]), ph, C)) ||
                         (!__all_sync(FULL, have_acc) && !f8_wait_all(fb_smem_u32(&C->acc_empty[b]), bph ^ 1, C))) {
@@ -507,7 +529,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             const int i = tid - 320;
             uint32_t g = 0;
             bool ok = true;
-            for (int it = blockIdx.x; it < tiles && ok; it += gridDim.x) {
+            for (int it = first; it < tiles && ok; it += stride) {
                 const f8_tile_t t = f8_tile<MODE, NT>(P, it, n_tiles);
                 const float *a0 = P.a_scales + (int64_t)(t.r0 + min(i, t.rows - 1)) * P.as_stride;
                 const float *a1 = P.a_scales + (int64_t)(t.r0 + min(i + 64, t.rows - 1)) * P.as_stride;
@@ -518,7 +540,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     float va[2][F8_SC], vb[2][F8_SC];
 #pragma unroll
                     for (int q = 0; q < F8_SC; q++) {
-                        const int k = min(kb + q, kbs - 1);
+                        const int k = kb_lo + min(kb + q, kbs - 1);
                         va[0][q] = __ldg(a0 + k);
                         va[1][q] = __ldg(a1 + k);
                         vb[0][q] = __ldg(b0 + k);
@@ -547,7 +569,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
         const uint32_t t_row = tmem + ((uint32_t)(warp & 3) << 21);
         uint32_t step = 0, cnt = 0, grp = 0, have = 0;
         bool ok = true;
-        for (int it = blockIdx.x; it < tiles; it += gridDim.x, cnt++) {
+        for (int it = first; it < tiles; it += stride, cnt++) {
             const f8_tile_t t = f8_tile<MODE, NT>(P, it, n_tiles);
             const int c0 = t.n0 + (MODE == F8_GATE_UP ? 0 : wg * W); /* first row of b of this thread's columns */
             float2 acc[W / 2];
@@ -566,7 +588,17 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             grp++;                                                                                   \
         }                                                                                            \
     } while (0)
+            /* 32-row groups behind the tile's last row only pass the barriers on */
+            const bool live = (warp & 3) * 32 < t.rows;
             float n0, n1 = 0.0f;
+            if (!live) {
+                for (int kb = 0; kb < kbs; kb++, step++) {
+                    F8_FACTORS(kb);
+                    if (ok) ok = f8_wait_all(fb_smem_u32(&C->acc_full[step % NB]), (step / NB) & 1, C);
+                    if (ok && lane == 0) fb_mbar_arrive(fb_smem_u32(&C->acc_empty[step % NB]));
+                }
+                have = 0;
+            } else {
             F8_FACTORS(0);
             /* Chunks of 32 columns through two register buffers: while one is joined the next is on its way, also across
              * blocks.  (gate/up: the first half of a thread's columns are the gate's, the second the up's) */
@@ -585,7 +617,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                 if (!ok) continue;
 #pragma unroll
                 for (int c = 0; c < CH; c++) {
-                    const int w = CH == 1 ? 0 : c & 1; /* (a single chunk has no second buffer to go to) */
+                    const int w = c & 1;
                     f8_tmem_wait(r[w]);
                     if (c + 1 < CH) {
                         f8_tmem_ld32(F8_COL(b, c + 1), r[w ^ 1]);
@@ -594,8 +626,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                         __syncwarp();
                         if (lane == 0) fb_mbar_arrive(fb_smem_u32(&C->acc_empty[b]));
                         if (kb + 1 < kbs) {
-                            if (CH == 1 || !__all_sync(FULL, have)) ok = f8_wait_all(fb_smem_u32(&C->acc_full[(step + 1) % NB]), ((step + 1) / NB) & 1, C);
-                            if (ok && CH > 1) {
+                            if (!__all_sync(FULL, have)) ok = f8_wait_all(fb_smem_u32(&C->acc_full[(step + 1) % NB]), ((step + 1) / NB) & 1, C);
+                            if (ok) {
                                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                                 f8_tmem_ld32(F8_COL((step + 1) % NB, 0), r[w ^ 1]);
                             }
@@ -608,12 +640,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < 16; i++) f8_fma2(acc[16 * c + i], r[w][2 * i], r[w][2 * i + 1], f);
                     /* the next block's barrier is asked for a chunk ahead of its use */
-                    if (CH > 1 && c == CH - 2) have = f8_look(fb_smem_u32(&C->acc_full[(step + 1) % NB]), ((step + 1) / NB) & 1);
-                    if (CH == 1 && kb + 1 < kbs && ok) {
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        f8_tmem_ld32(F8_COL((step + 1) % NB, 0), r[0]);
-                    }
+                    if (c == CH - 2) have = f8_look(fb_smem_u32(&C->acc_full[(step + 1) % NB]), ((step + 1) / NB) & 1);
                 }
+            }
             }
             const uint32_t buf = out_u + warp * (uint32_t)(cfg::BUFS * 4096);
             if (MODE == F8_GATE_UP) {
@@ -643,6 +672,15 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     }
                     if (wg == 0) P.act_scales[(int64_t)(t.r0 + row) * (P.n >> 7) + (t.n0 >> 7)] = sc;
                 }
+            } else if (SPLIT) {
+                /* this rank's part of the tile, over the operand stages (every MMA has read them): 512 bytes a row, its
+                 * 16-byte piece q at q ^ row % 32 */
+                if (live)
+#pragma unroll
+                    for (uint32_t q = 0; q < W / 4; q++)
+                        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dyn_u + row * 512u + (((wg * (W / 4) + q) ^ (row & 31u)) << 4)),
+                                     "f"(acc[2 * q].x), "f"(acc[2 * q].y), "f"(acc[2 * q + 1].x), "f"(acc[2 * q + 1].y)
+                                     : "memory");
             } else {
                 /* rows of this warp that are the tile's; a box may only leave whole if none of its rows is another expert's */
                 const int w0 = (warp & 3) * 32, rows = ok ? max(0, min(32, t.rows - w0)) : 0, c0 = t.n0 + wg * W;
@@ -674,30 +712,15 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                             w[i] = *reinterpret_cast<const uint32_t *>(&v);
                         }
                     }
-                    if constexpr (W >= 64) {
-                        f8_box_wait();
+                    f8_box_wait();
 #pragma unroll
-                        for (int c = 0; c < W / 64; c++) { /* boxes of 64 columns */
-                            const int x = c0 + 64 * c;
-                            f8_stage(buf + c * 4096u, w + 32 * c);
-                            if (x < P.n)
-                                f8_box_out(buf + c * 4096u, &P.to, 2 * x, t.r0 + w0, tma,
-                                           reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + w0) * P.out_stride + x),
-                                           2 * P.out_stride, rows, 2 * (P.n - x), 2);
-                        }
-                    } else if (lane < rows) { /* 64 bytes a row: straight from the registers */
-                        uint8_t *o = reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + row) * P.out_stride + c0);
-#pragma unroll
-                        for (int i = 0; i < W / 8; i++) {
-                            if (P.out_tma && c0 + 8 * i + 8 <= P.n) {
-                                *reinterpret_cast<uint4 *>(o + 16 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-                            } else {
-#pragma unroll
-                                for (int k = 0; k < 8; k++)
-                                    if (c0 + 8 * i + k < P.n)
-                                        *reinterpret_cast<uint16_t *>(o + 16 * i + 2 * k) = (uint16_t)(w[4 * i + k / 2] >> (16 * (k & 1)));
-                            }
-                        }
+                    for (int c = 0; c < W / 64; c++) { /* boxes of 64 columns */
+                        const int x = c0 + 64 * c;
+                        f8_stage(buf + c * 4096u, w + 32 * c);
+                        if (x < P.n)
+                            f8_box_out(buf + c * 4096u, &P.to, 2 * x, t.r0 + w0, tma,
+                                       reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + w0) * P.out_stride + x),
+                                       2 * P.out_stride, rows, 2 * (P.n - x), 2);
                     }
                 } else {
 #pragma unroll
@@ -713,7 +736,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                 }
             }
         }
-        if (MODE != F8_GATE_UP) f8_box_wait(); /* the staging buffers go away with the block */
+        if (MODE != F8_GATE_UP && !SPLIT) f8_box_wait(); /* the staging buffers go away with the block */
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -721,6 +744,49 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
     if (C->abort_flag) {
         if (tid == 0) *P.status = FB_ST_WAIT_TIMEOUT;
         for (int i = 0; i < 100; i++) __nanosleep(1000); /* copies and MMAs under way land before their memory is released */
+    }
+    if (SPLIT) {
+        /* the parts meet: rank r sums rows r, r + ranks, ... in rank order, a warp a row */
+        f8_cluster_sync();
+        const f8_tile_t t = f8_tile<MODE, NT>(P, first, n_tiles);
+        for (int row = (int)rank + (int)ranks * warp; row < t.rows; row += (int)ranks * (F8_THREADS / 32)) {
+            const uint32_t at = dyn_u + row * 512u + (((uint32_t)lane ^ (row & 31u)) << 4);
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t s = 0; s < ranks; s++) {
+                float x[4];
+                uint32_t ra;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(at), "r"(s));
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+                             : "r"(ra)
+                             : "memory");
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] += x[i];
+            }
+            const int c = t.n0 + 4 * lane;
+            const int64_t o = (int64_t)(t.r0 + row) * P.out_stride + c;
+            if (P.out_bf16) {
+                __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(P.out) + o;
+                if (P.out_tma && c + 4 <= P.n) {
+                    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+                    *reinterpret_cast<uint2 *>(out) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (c + i < P.n) out[i] = __float2bfloat16_rn(v[i]);
+                }
+            } else {
+                float *out = reinterpret_cast<float *>(P.out) + o;
+                if (P.out_tma && c + 4 <= P.n) {
+                    *reinterpret_cast<float4 *>(out) = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (c + i < P.n) out[i] = v[i];
+                }
+            }
+        }
+        f8_cluster_sync(); /* nobody leaves while its part is being read */
     }
     __syncthreads();
     if (warp == 9)
@@ -1027,16 +1093,31 @@ static int f8_map(CUtensorMap *m, const void *p, uint64_t k, uint64_t rows, uint
                : (int)cudaErrorInvalidValue;
 }
 
-template <int MODE, int NT>
-static int f8_launch(f8_args_t &p, int64_t most_tiles, int n_sm, int *launches, cudaStream_t st) {
-    const int grid = (int)(most_tiles < n_sm ? most_tiles : n_sm);
-    k_f8_mma<MODE, NT><<<grid, F8_THREADS, f8_cfg<MODE, NT>::SMEM, st>>>(p);
+template <int MODE, int NT, bool SPLIT>
+static int f8_launch(f8_args_t &p, int64_t most_tiles, int ranks, int n_sm, int *launches, cudaStream_t st) {
+    cudaLaunchConfig_t c = {};
+    cudaLaunchAttribute at[1];
+    c.gridDim = dim3((unsigned)(SPLIT ? most_tiles * ranks : most_tiles < n_sm ? most_tiles : n_sm));
+    c.blockDim = dim3(F8_THREADS);
+    c.dynamicSmemBytes = f8_cfg<MODE, NT>::SMEM;
+    c.stream = st;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = ranks;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    c.attrs = at;
+    c.numAttrs = SPLIT ? 1 : 0;
     *launches += 1;
-    return (int)cudaGetLastError();
+    const cudaError_t rc = cudaLaunchKernelEx(&c, k_f8_mma<MODE, NT, SPLIT>, p);
+    return (int)(rc != cudaSuccess ? rc : cudaGetLastError());
 }
 
-extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *status, int n_sm, int *launches,
+#define F8_KB256 0.53 /* 64 x 4096 x 4096 in tiles of 256: 22.3 us, 64 x 8192 x 1024: 9.8 us */
+#define F8_KB128 0.33 /* in tiles of 128: 15.7 and 7.9 us */
+#define F8_MEET 2.2   /* 64 x 4096 x 4096 split over 2: 12.7 us, over 4: 10.7 us */
+
+extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *status, const ops_device_t *d, int *launches,
                                     void *stream) {
+    const int n_sm = d->n_sm;
     if (a->m <= 16) {
         const fr_args_t f = {a->m, a->n, a->k, a->a, a->a_stride, a->a_scales, a->a_scales_stride, a->b, a->b_stride, a->b_scales,
                              a->b_scales_stride, a->out, a->out_type == FOMOE_B200_BF16, a->out_stride};
@@ -1057,15 +1138,23 @@ extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *s
     p.status = status;
     cudaStream_t st = (cudaStream_t)stream;
     const int64_t m = a->m, n = a->n, mt = (m + 127) / 128;
-    /* the widest tile that still gives every SM one: wide tiles read the least (4096 x 8192 x 4096: 148 us with 256 columns) */
-    const int nt = mt * ((n + 255) / 256) >= n_sm ? 256 : mt * ((n + 127) / 128) >= n_sm ? 128 : 64;
+    /* Tiles of 256 columns read the least and take F8_KB256 a block of k, tiles of 128 columns F8_KB128 (microseconds, the
+     * serial time of the hand-overs); the blocks of k of few tiles are split over the ranks of a cluster, which costs the
+     * meeting.  The choice is the least of waves x blocks x time. */
+    const int64_t kb = (a->k + 127) / 128, t256 = mt * ((n + 255) / 256), t128 = mt * ((n + 127) / 128);
+    double best = (double)((t256 + n_sm - 1) / n_sm * kb) * F8_KB256;
+    int nt = 256, ranks = 1;
+    for (int i = 0, r = 1; i < 4 && r <= kb; i++, r *= 2) {
+        if (d->clusters[i] < 1) continue;
+        const double c = (double)((t128 + d->clusters[i] - 1) / d->clusters[i] * ((kb + r - 1) / r)) * F8_KB128 + (r > 1 ? F8_MEET : 0.0);
+        if (c < best) best = c, nt = 128, ranks = r;
+    }
     int rc = f8_map(&p.ta, a->a, a->k, a->m, a->a_stride, 32) | f8_map(&p.tb, a->b, a->k, a->n, a->b_stride, nt);
     if (p.out_tma) rc |= f8_map(&p.to, a->out, (uint64_t)a->n * eb, a->m, (os + 15) & ~15ull, 32);
     if (rc) return rc;
-    const int64_t tiles = mt * ((n + nt - 1) / nt);
-    return nt == 256   ? f8_launch<F8_DENSE, 256>(p, tiles, n_sm, launches, st)
-           : nt == 128 ? f8_launch<F8_DENSE, 128>(p, tiles, n_sm, launches, st)
-                       : f8_launch<F8_DENSE, 64>(p, tiles, n_sm, launches, st);
+    return nt == 256    ? f8_launch<F8_DENSE, 256, false>(p, t256, 1, n_sm, launches, st)
+           : ranks == 1 ? f8_launch<F8_DENSE, 128, false>(p, t128, 1, n_sm, launches, st)
+                        : f8_launch<F8_DENSE, 128, true>(p, t128, ranks, n_sm, launches, st);
 }
 
 /* ------------------------------------------------------------------ the pairs' rows of x side by side: one warp a row
@@ -1146,8 +1235,9 @@ extern "C" void ops_experts_layout(const fomoe_b200_f8_experts_args_t *a, ops_ex
     w->bytes = at;
 }
 
-extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint8_t *ws, int *status, int n_sm,
+extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint8_t *ws, int *status, const ops_device_t *d,
                                      int *launches, void *stream) {
+    const int n_sm = d->n_sm;
     cudaStream_t st = (cudaStream_t)stream;
     ops_experts_ws_t w;
     ops_experts_layout(a, &w);
@@ -1190,7 +1280,7 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     p.b_scales = a->gate_up_scales, p.bs_stride = H / 128, p.bs_rec = (int64_t)(2 * I / 128) * (H / 128), p.b_rec_rows = 2 * I;
     p.act_q = ws + w.act_q, p.act_scales = (float *)(ws + w.act_scales);
     rc = f8_map(&p.ta, ws + w.xp, H, w.n_pairs, H, 32) | f8_map(&p.tb, a->gate_up, H, recs * 2 * I, H, 128);
-    if (!rc) rc = f8_launch<F8_GATE_UP, 256>(p, tiles * (I / 128), n_sm, launches, st);
+    if (!rc) rc = f8_launch<F8_GATE_UP, 256, false>(p, tiles * (I / 128), 1, n_sm, launches, st);
     if (rc) return rc;
     p.n = H, p.k = I;
     p.a_scales = p.act_scales, p.as_stride = I / 128;
@@ -1198,7 +1288,7 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     p.out = ws + w.dots, p.out_stride = H, p.out_tma = 1, p.out_scales = (float *)(ws + w.dot_scales);
     rc = f8_map(&p.ta, ws + w.act_q, I, w.n_pairs, I, 32) | f8_map(&p.tb, a->down, I, recs * H, I, 256) |
          f8_map(&p.to, ws + w.dots, 2ull * H, w.n_pairs, 2ull * H, 32);
-    if (!rc) rc = f8_launch<F8_DOWN, 256>(p, tiles * ((H + 255) / 256), n_sm, launches, st);
+    if (!rc) rc = f8_launch<F8_DOWN, 256, false>(p, tiles * ((H + 255) / 256), 1, n_sm, launches, st);
     if (rc) return rc;
     const int vec = ((uintptr_t)a->out & 15) == 0 && (a->n_tokens == 1 || a->out_stride % 8 == 0);
     /* (the grid's y goes to 65535) */
@@ -1212,7 +1302,7 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     return (int)cudaGetLastError();
 }
 
-extern "C" int ops_f8_init(void) {
+extern "C" int ops_f8_init(ops_device_t *d) {
     cudaFuncAttributes f;
     int rc = 0;
     if (!f8_encode) {
@@ -1224,15 +1314,30 @@ extern "C" int ops_f8_init(void) {
         f8_encode = (f8_encode_t)fn;
     }
 #define RK(k) rc |= (int)cudaFuncGetAttributes(&f, (k))
-#define RM(MODE, NT)                                                                                             \
-    rc |= (int)cudaFuncSetAttribute(k_f8_mma<MODE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, f8_cfg<MODE, NT>::SMEM)
+#define RM(MODE, NT, SPLIT)                                                                                             \
+    rc |= (int)cudaFuncSetAttribute((k_f8_mma<MODE, NT, SPLIT>), cudaFuncAttributeMaxDynamicSharedMemorySize, f8_cfg<MODE, NT>::SMEM)
     RK(k_ops_combine); RK(k_ops_permute);
 #define RF(k) rc |= (int)cudaFuncSetAttribute((k), cudaFuncAttributeMaxDynamicSharedMemorySize, FR_SMEM)
     RF(k_f8_few<1>); RF(k_f8_few<2>); RF(k_f8_few_gate_up); RF(k_f8_few_down);
 #undef RF
-    RM(F8_DENSE, 256); RM(F8_DENSE, 128); RM(F8_DENSE, 64); RM(F8_GATE_UP, 256); RM(F8_DOWN, 256);
+    RM(F8_DENSE, 256, false); RM(F8_DENSE, 128, false); RM(F8_DENSE, 128, true); RM(F8_GATE_UP, 256, false);
+    RM(F8_DOWN, 256, false);
 #undef RM
 #undef RK
+    d->clusters[0] = d->n_sm;
+    for (int i = 1; i < 4; i++) {
+        cudaLaunchConfig_t c = {};
+        cudaLaunchAttribute at[1];
+        c.gridDim = dim3(1u << i);
+        c.blockDim = dim3(F8_THREADS);
+        c.dynamicSmemBytes = f8_cfg<F8_DENSE, 128>::SMEM;
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = 1u << i;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        c.attrs = at;
+        c.numAttrs = 1;
+        rc |= (int)cudaOccupancyMaxActiveClusters(&d->clusters[i], k_f8_mma<F8_DENSE, 128, true>, &c);
+    }
     rc |= (int)cudaFuncSetAttribute(k_ops_bucket<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, OPS_MAX_E * (BK_WARPS + 1) * 4);
     rc |= (int)cudaFuncSetAttribute(k_ops_bucket<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, OPS_MAX_E * (BK_WARPS + 1) * 4);
     return rc;

@@ -41,11 +41,17 @@ typedef struct {
     int n_pairs; /* routed and shared pairs */
 } ops_experts_ws_t;
 
-int ops_f8_init(void);
-int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *status, int n_sm, int *launches, void *stream);
+/* What the product launchers go by on a device. */
+typedef struct {
+    int n_sm;
+    int clusters[4]; /* clusters of 1, 2, 4, 8 blocks of the split product that the device runs at the same time */
+} ops_device_t;
+
+int ops_f8_init(ops_device_t *d); /* loads the kernels on the current device; n_sm is given */
+int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *status, const ops_device_t *d, int *launches, void *stream);
 void ops_experts_layout(const fomoe_b200_f8_experts_args_t *a, ops_experts_ws_t *w);
-int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint8_t *ws, int *status, int n_sm, int *launches,
-                          void *stream);
+int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint8_t *ws, int *status, const ops_device_t *d,
+                          int *launches, void *stream);
 
 #ifdef __cplusplus
 }

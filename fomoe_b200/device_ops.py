@@ -72,7 +72,9 @@ class DeviceOps:
         self._float = {torch.float32: F32, torch.bfloat16: BF16}
         self._out = {"f32": (torch.float32, F32), "bf16": (torch.bfloat16, BF16)}
         self._f8 = (torch.float8_e4m3fn, torch.uint8)
-        self._dev = torch.device("cuda", device)
+        self._f32, self._i32, self._u8 = (torch.float32,), (torch.int32,), (torch.uint8, torch.bool)
+        # the current stream's handle without building a Stream object around it, where torch offers that
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
     def close(self):
         """Release the handle; none of its calls may still be in flight."""
@@ -100,39 +102,41 @@ class DeviceOps:
             raise RuntimeError(f"{what}: {self._l.fomoe_b200_ops_last_error(self._h).decode()}")
 
     def _stream(self):
-        return self._t.cuda.current_stream(self._dev).cuda_stream
+        if self._raw_stream is not None:
+            return self._raw_stream(self.device)
+        return self._t.cuda.current_stream(self.device).cuda_stream
+
+    def _bad(self, t, name, types, shape, what):
+        raise ValueError(f"{name}: {what} of {' or '.join(map(str, types))} on CUDA device {self.device}"
+                         f"{'' if shape is None else f' of shape {tuple(shape)}'} is wanted, got {tuple(t.shape)} {t.dtype} on "
+                         f"{t.device} with strides {t.stride()}")
 
     def _rows(self, t, name, types, shape=None):
         """Checks a 2-D tensor with contiguous rows; -> its row stride."""
-        if t.dim() != 2 or t.dtype not in types or t.device != self._dev:
-            raise ValueError(f"{name}: a 2-D tensor on {self._dev} of {' or '.join(map(str, types))} is wanted, got "
-                             f"{t.dim()}-D {t.dtype} on {t.device}")
-        if shape is not None and tuple(t.shape) != shape:
-            raise ValueError(f"{name}: shape {shape} is wanted, got {tuple(t.shape)}")
-        if t.shape[1] > 1 and t.stride(1) != 1:
-            raise ValueError(f"{name}: rows have to be contiguous")
+        if (t.dim() != 2 or t.dtype not in types or t.get_device() != self.device or (t.stride(1) != 1 and t.shape[1] > 1)
+                or (shape is not None and t.shape != shape)):
+            self._bad(t, name, types, shape, "a 2-D tensor with contiguous rows")
         return t.stride(0)
 
     def _flat(self, t, name, types, shape):
         """Checks a contiguous tensor; -> its address."""
-        if tuple(t.shape) != shape or t.dtype not in types or t.device != self._dev or not t.is_contiguous():
-            raise ValueError(f"{name}: a contiguous tensor {shape} of {' or '.join(map(str, types))} on {self._dev} is wanted, "
-                             f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+        if t.shape != shape or t.dtype not in types or t.get_device() != self.device or not t.is_contiguous():
+            self._bad(t, name, types, shape, "a contiguous tensor")
         return t.data_ptr()
 
     def route(self, logits, top_k, *, score="softmax", bias=None, n_group=1, topk_group=1, group_best=1, renorm=True,
               scale=1.0, valid=None):
         """logits [T, E] f32 or bf16 -> (ids int32 [T, top_k], weights f32 [T, top_k]); see fomoe_b200_ops_route."""
         t = self._t
-        stride = self._rows(logits, "logits", tuple(self._float))
+        stride = self._rows(logits, "logits", self._float)
         T, E = logits.shape
         if score not in SCORES:
             raise ValueError(f"score: 'softmax' or 'sigmoid' is wanted, got {score!r}")
-        b = None if bias is None else self._flat(bias, "bias", (t.float32,), (E,))
-        v = None if valid is None else self._flat(valid, "valid", (t.uint8, t.bool), (T,))
-        ids = t.empty((T, max(top_k, 0)), dtype=t.int32, device=self._dev)
-        w = t.empty((T, max(top_k, 0)), dtype=t.float32, device=self._dev)
-        cfg = RouteConfig(E, top_k, SCORES[score], n_group, topk_group, group_best, int(bool(renorm)), scale)
+        b = None if bias is None else self._flat(bias, "bias", self._f32, (E,))
+        v = None if valid is None else self._flat(valid, "valid", self._u8, (T,))
+        k = top_k if top_k > 0 else 0
+        ids, w = logits.new_empty((T, k), dtype=t.int32), logits.new_empty((T, k), dtype=t.float32)
+        cfg = RouteConfig(E, top_k, SCORES[score], n_group, topk_group, group_best, 1 if renorm else 0, scale)
         self._ck(self._l.fomoe_b200_ops_route(self._h, cfg, T, logits.data_ptr(), self._float[logits.dtype], stride, b, v,
                                               ids.data_ptr(), w.data_ptr(), self._stream()), "route")
         return ids, w
@@ -142,68 +146,69 @@ class DeviceOps:
         """The norms around a block (see fomoe_b200_ops_norm): x [T, n]; pre, post f32 [n]; block [T, n]; gate of block's
         type, [T, n], [1, n] or [T, 1].  out: 'f32', 'bf16' or 'f8'.  -> (x', h), or (x', h, scales) with 'f8'.  x' is x
         itself with inplace or without a block; without pre there is no h (None)."""
-        t = self._t
-        fl = tuple(self._float)
-        T, n = x.shape if x.dim() == 2 else (0, 0)
-        a = NormArgs(T, n, eps, offset, scale)
-        a.x_stride, a.x, a.x_type = self._rows(x, "x", fl), x.data_ptr(), self._float[x.dtype]
-        x_out = x
+        t, fl = self._t, self._float
+        xs = self._rows(x, "x", fl)
+        T, n = x.shape
+        x_out, blk, bt, bs, po, ga, gs, gp, xo, xos = x, None, 0, 0, None, None, 0, 0, None, 0
         if block is not None:
-            a.block_stride = self._rows(block, "block", fl, (T, n))
-            a.block, a.block_type = block.data_ptr(), self._float[block.dtype]
+            bs = self._rows(block, "block", fl, (T, n))
+            blk, bt = block.data_ptr(), fl[block.dtype]
             if post is not None:
-                a.post = self._flat(post, "post", (t.float32,), (n,))
+                po = self._flat(post, "post", self._f32, (n,))
             if gate is not None:
-                if gate.dim() != 2 or gate.shape[0] not in (1, T) or gate.shape[1] not in (1, n):
-                    raise ValueError(f"gate: [T, n], [1, n] or [T, 1] is wanted, got {tuple(gate.shape)}")
-                s = self._rows(gate, "gate", (block.dtype,))
-                a.gate, a.gate_stride, a.gate_step = gate.data_ptr(), s if gate.shape[0] == T and T > 1 else 0, int(gate.shape[1] == n and n > 1)
+                gs = self._rows(gate, "gate", (block.dtype,))
+                gT, gn = gate.shape
+                if gT not in (1, T) or gn not in (1, n):
+                    raise ValueError(f"gate: [T, n], [1, n] or [T, 1] is wanted, got {(gT, gn)}")
+                ga, gs, gp = gate.data_ptr(), gs if gT > 1 else 0, 1 if gn == n and n > 1 else 0
             if not inplace:
-                x_out = t.empty((T, n), dtype=x.dtype, device=self._dev)
-            a.x_out, a.x_out_stride = x_out.data_ptr(), x_out.stride(0)
+                x_out = x.new_empty((T, n))
+            xo, xos = x_out.data_ptr(), x_out.stride(0)
         elif post is not None or gate is not None:
             raise ValueError("post and gate need a block")
-        h = sc = None
+        h = sc = pr = hp = sp = None
+        ht = nb = 0
         if pre is not None:
-            a.pre = self._flat(pre, "pre", (t.float32,), (n,))
+            pr = self._flat(pre, "pre", self._f32, (n,))
             if out == "f8":
-                h = t.empty((T, n), dtype=t.float8_e4m3fn, device=self._dev)
-                sc = t.empty((T, (n + 127) // 128), dtype=t.float32, device=self._dev)
-                a.h_type, a.h_scales, a.h_scales_stride = F8, sc.data_ptr(), (n + 127) // 128
+                ht, nb = F8, (n + 127) // 128
+                h, sc = x.new_empty((T, n), dtype=t.float8_e4m3fn), x.new_empty((T, nb), dtype=t.float32)
+                sp = sc.data_ptr()
             elif out in self._out:
-                dt, a.h_type = self._out[out]
-                h = t.empty((T, n), dtype=dt, device=self._dev)
+                dt, ht = self._out[out]
+                h = x.new_empty((T, n), dtype=dt)
             else:
                 raise ValueError(f"out: 'f32', 'bf16' or 'f8' is wanted, got {out!r}")
-            a.h, a.h_stride = h.data_ptr(), n
+            hp = h.data_ptr()
+        a = NormArgs(T, n, eps, offset, scale, x.data_ptr(), fl[x.dtype], xs, blk, bt, bs, po, ga, gs, gp, xo, xos, pr, hp, ht,
+                     n, sp, nb)
         self._ck(self._l.fomoe_b200_ops_norm(self._h, a, self._stream()), "norm")
         return (x_out, h, sc) if out == "f8" else (x_out, h)
 
     def f8_quantize(self, x):
         """x [T, n] f32 or bf16 -> (e4m3 [T, n], scales f32 [T, ceil(n / 128)])."""
         t = self._t
-        stride = self._rows(x, "x", tuple(self._float))
+        stride = self._rows(x, "x", self._float)
         T, n = x.shape
-        q = t.empty((T, n), dtype=t.float8_e4m3fn, device=self._dev)
-        sc = t.empty((T, (n + 127) // 128), dtype=t.float32, device=self._dev)
+        nb = (n + 127) // 128
+        q, sc = x.new_empty((T, n), dtype=t.float8_e4m3fn), x.new_empty((T, nb), dtype=t.float32)
         self._ck(self._l.fomoe_b200_ops_f8_quantize(self._h, T, n, x.data_ptr(), self._float[x.dtype], stride, q.data_ptr(), n,
-                                                    sc.data_ptr(), sc.shape[1], self._stream()), "f8_quantize")
+                                                    sc.data_ptr(), nb, self._stream()), "f8_quantize")
         return q, sc
 
     def f8_matmul(self, a, a_scales, b, b_scales, *, out="bf16"):
         """a [M, K] e4m3 with scales [M, ceil(K / 128)], b [N, K] with scales [ceil(N / 128), ceil(K / 128)] -> a b^T [M, N]."""
-        t = self._t
         if out not in self._out:
             raise ValueError(f"out: 'f32' or 'bf16' is wanted, got {out!r}")
         sa, sb = self._rows(a, "a", self._f8), self._rows(b, "b", self._f8)
-        (M, K), N = a.shape, b.shape[0]
-        if b.shape[1] != K:
-            raise ValueError(f"a has {K} columns, b has {b.shape[1]}")
+        (M, K), (N, bk) = a.shape, b.shape
+        if bk != K:
+            raise ValueError(f"a has {K} columns, b has {bk}")
         nb = (K + 127) // 128
-        ss = self._rows(a_scales, "a_scales", (t.float32,), (M, nb))
-        sw = self._rows(b_scales, "b_scales", (t.float32,), ((N + 127) // 128, nb))
+        ss = self._rows(a_scales, "a_scales", self._f32, (M, nb))
+        sw = self._rows(b_scales, "b_scales", self._f32, ((N + 127) // 128, nb))
         dt, ty = self._out[out]
-        c = t.empty((M, N), dtype=dt, device=self._dev)
+        c = a.new_empty((M, N), dtype=dt)
         args = MatmulArgs(M, N, K, a.data_ptr(), sa, a_scales.data_ptr(), ss, b.data_ptr(), sb, b_scales.data_ptr(), sw,
                           c.data_ptr(), ty, N)
         self._ck(self._l.fomoe_b200_ops_f8_matmul(self._h, args, self._stream()), "f8_matmul")
@@ -215,31 +220,31 @@ class DeviceOps:
         weights f32 [T, k], gate_up [R, 2 I, H], down [R, H, I] with their block scales; R records, the last one shared by
         all tokens if `shared`.  -> bf16 [T, H].  workspace: a uint8 tensor to use instead of one from torch's allocator
         (at least f8_experts_workspace bytes); calls that may overlap need their own."""
-        t = self._t
+        t, s = self._t, 1 if shared else 0
         xs = self._rows(x, "x", self._f8)
         T, H = x.shape
         R, I2 = gate_up.shape[:2]
         I = I2 // 2
         k = ids.shape[1] if ids.dim() == 2 else 0
-        if H % 128 or I % 128 or I2 % 256:
+        if H % 128 or I2 % 256:
             raise ValueError(f"hidden size {H} and intermediate size {I2} / 2: multiples of 128 are wanted")
-        ss = self._rows(x_scales, "x_scales", (t.float32,), (T, H // 128))
-        out = t.empty((T, H), dtype=t.bfloat16, device=self._dev)
-        args = ExpertsArgs(T, H, I, R - int(bool(shared)), k, int(bool(shared)), x.data_ptr(), xs, x_scales.data_ptr(), ss,
-                           self._flat(ids, "ids", (t.int32,), (T, k)), self._flat(weights, "weights", (t.float32,), (T, k)),
-                           self._flat(gate_up, "gate_up", self._f8, (R, 2 * I, H)),
-                           self._flat(gate_up_scales, "gate_up_scales", (t.float32,), (R, 2 * I // 128, H // 128)),
+        hb, ib = H // 128, I // 128
+        ss = self._rows(x_scales, "x_scales", self._f32, (T, hb))
+        out = x.new_empty((T, H), dtype=t.bfloat16)
+        args = ExpertsArgs(T, H, I, R - s, k, s, x.data_ptr(), xs, x_scales.data_ptr(), ss,
+                           self._flat(ids, "ids", self._i32, (T, k)), self._flat(weights, "weights", self._f32, (T, k)),
+                           self._flat(gate_up, "gate_up", self._f8, (R, I2, H)),
+                           self._flat(gate_up_scales, "gate_up_scales", self._f32, (R, 2 * ib, hb)),
                            self._flat(down, "down", self._f8, (R, H, I)),
-                           self._flat(down_scales, "down_scales", (t.float32,), (R, H // 128, I // 128)),
-                           out.data_ptr(), H)
-        need = self._l.fomoe_b200_ops_f8_experts_workspace(args)
+                           self._flat(down_scales, "down_scales", self._f32, (R, hb, ib)), out.data_ptr(), H)
         if workspace is None:
-            workspace = t.empty(need, dtype=t.uint8, device=self._dev)
-        elif workspace.device != self._dev or not workspace.is_contiguous():
-            raise ValueError("workspace: a contiguous tensor on the handle's device is wanted")
-        self._ck(self._l.fomoe_b200_ops_f8_experts(self._h, args, workspace.data_ptr(),
-                                                   workspace.numel() * workspace.element_size(), self._stream()),
-                 "f8_experts")
+            size = self._l.fomoe_b200_ops_f8_experts_workspace(args)
+            workspace = x.new_empty((size,), dtype=t.uint8)
+        else:
+            if workspace.get_device() != self.device or not workspace.is_contiguous():
+                raise ValueError("workspace: a contiguous tensor on the handle's device is wanted")
+            size = workspace.numel() * workspace.element_size()
+        self._ck(self._l.fomoe_b200_ops_f8_experts(self._h, args, workspace.data_ptr(), size, self._stream()), "f8_experts")
         return out
 
     def f8_experts_workspace(self, n_tokens, n_embd, n_inter, n_experts, top_k, shared=False):

@@ -27,7 +27,7 @@ def ops(fb, fake, monkeypatch):
         f.restype, f.argtypes = res, args
     monkeypatch.setattr(fb, "_lib", fake)
     o = fb.DeviceOps(0)
-    o._dev = torch.device("cpu")
+    o.device = -1   # where CPU tensors are
     o._stream = lambda: 0
     o.fake = fake
     yield o
