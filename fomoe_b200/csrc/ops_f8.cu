@@ -588,17 +588,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             grp++;                                                                                   \
         }                                                                                            \
     } while (0)
-            /* 32-row groups behind the tile's last row only pass the barriers on */
-            const bool live = (warp & 3) * 32 < t.rows;
             float n0, n1 = 0.0f;
-            if (!live) {
-                for (int kb = 0; kb < kbs; kb++, step++) {
-                    F8_FACTORS(kb);
-                    if (ok) ok = f8_wait_all(fb_smem_u32(&C->acc_full[step % NB]), (step / NB) & 1, C);
-                    if (ok && lane == 0) fb_mbar_arrive(fb_smem_u32(&C->acc_empty[step % NB]));
-                }
-                have = 0;
-            } else {
             F8_FACTORS(0);
             /* Chunks of 32 columns through two register buffers: while one is joined the next is on its way, also across
              * blocks.  (gate/up: the first half of a thread's columns are the gate's, the second the up's) */
@@ -643,7 +633,6 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     if (c == CH - 2) have = f8_look(fb_smem_u32(&C->acc_full[(step + 1) % NB]), ((step + 1) / NB) & 1);
                 }
             }
-            }
             const uint32_t buf = out_u + warp * (uint32_t)(cfg::BUFS * 4096);
             if (MODE == F8_GATE_UP) {
                 /* silu(g) u of this thread's 64 columns, and the amax over the row's 128 with the other warpgroup's */
@@ -675,7 +664,6 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             } else if (SPLIT) {
                 /* this rank's part of the tile, over the operand stages (every MMA has read them): 512 bytes a row, its
                  * 16-byte piece q at q ^ row % 32 */
-                if (live)
 #pragma unroll
                     for (uint32_t q = 0; q < W / 4; q++)
                         asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dyn_u + row * 512u + (((wg * (W / 4) + q) ^ (row & 31u)) << 4)),

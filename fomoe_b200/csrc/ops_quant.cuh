@@ -1,7 +1,6 @@
 /*
  * ops_quant.cuh -- one block of 128 values to e4m3 with an fp32 scale: scale = max(amax, 2^-100) / 448, q = e4m3(x / scale).
- * Division and conversion are IEEE operations (round to nearest even), so any implementation of the formula gets the
- * same bits.
+ * Division and conversion are rounded to nearest even, so any implementation of the formula gets the same bits.
  */
 #pragma once
 #include <cuda_fp8.h>
@@ -15,6 +14,15 @@ __device__ __forceinline__ float ops_amax(float a, float b) {
 }
 
 __device__ __forceinline__ float ops_f8_scale(float amax) { return __fdiv_rn(ops_amax(amax, 0x1p-100f), 448.0f); }
+
+/* x / scale rounded to nearest, from inv = 1 / scale rounded to nearest: a quotient that is off by a step at most, its exact
+ * remainder, and one correction (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
+ * processor", 1990).  Three operations where the division routine takes a dozen and a branch; scales are at least
+ * 2^-109, so nothing here leaves the range before the quotient has left e4m3's. */
+__device__ __forceinline__ float ops_f8_quot(float x, float scale, float inv) {
+    const float q = __fmul_rn(x, inv);
+    return __fmaf_rn(__fmaf_rn(-q, scale, x), inv, q);
+}
 
 /* four numbers as e4m3, the first in the low byte */
 __device__ __forceinline__ uint32_t ops_f8_pack4(float a, float b, float c, float d) {

@@ -12,6 +12,7 @@
 #include "launch.h"
 #include "ops_launch.h"
 #include "ops_quant.cuh"
+#include "stream.cuh"
 
 #ifndef FULL
 #define FULL 0xffffffffu
@@ -348,7 +349,9 @@ extern "C" int ops_launch_route(const ops_route_t *a, void *stream) {
  * written once whatever the number of norms.  16 neighbouring threads hold one block of 128, whose amax is a shuffle
  * reduction.  VEC: all pointers and strides allow 16-byte accesses and n is a multiple of 8; otherwise the same code
  * goes element by element. */
-#define NM_THREADS 256
+#define NM_THREADS(G) ((G) == 32 ? 256 : (G))
+#define NM_AHEAD 148 /* rows: what a later block reads is asked into L2 (8192 x 4096: 83 us, without 89, 592 rows ahead 85) */
+#define NM_FEW 1184  /* rows: eight an SM */
 
 template <bool VEC>
 __device__ __forceinline__ void nm_load8(const void *p, int bf16, int64_t at, int left, float (&v)[8]) {
@@ -408,14 +411,14 @@ __device__ __forceinline__ void nm_quant8(uint8_t *q, float *scales, int c, int 
     for (int i = 0; i < 8; i++) amax = ops_amax(amax, v[i]);
 #pragma unroll
     for (int s = 8; s > 0; s >>= 1) amax = ops_amax(amax, __shfl_xor_sync(FULL, amax, s));
-    const float sc = ops_f8_scale(amax);
+    const float sc = ops_f8_scale(amax), inv = __frcp_rn(sc);
     if (c < n) {
         if ((c & 127) == 0) scales[c >> 7] = sc;
         uint32_t w[2];
 #pragma unroll
         for (int h = 0; h < 2; h++)
-            w[h] = ops_f8_pack4(__fdiv_rn(v[4 * h], sc), __fdiv_rn(v[4 * h + 1], sc), __fdiv_rn(v[4 * h + 2], sc),
-                                __fdiv_rn(v[4 * h + 3], sc));
+            w[h] = ops_f8_pack4(ops_f8_quot(v[4 * h], sc, inv), ops_f8_quot(v[4 * h + 1], sc, inv),
+                                ops_f8_quot(v[4 * h + 2], sc, inv), ops_f8_quot(v[4 * h + 3], sc, inv));
         if (VEC) {
             *reinterpret_cast<uint2 *>(q + c) = make_uint2(w[0], w[1]);
         } else {
@@ -438,17 +441,23 @@ __device__ __forceinline__ float nm_row_sum(float v, float *s_red) {
     __syncthreads();
     float t = 0.0f;
 #pragma unroll
-    for (int w = 0; w < NM_THREADS / 32; w++) t += s_red[w];
+    for (int w = 0; w < G / 32; w++) t += s_red[w];
     return t;
 }
 
 template <bool VEC, int G, int IT>
-__global__ void __launch_bounds__(NM_THREADS) k_ops_norm(fomoe_b200_norm_args_t A) {
-    __shared__ float s_red[NM_THREADS / 32];
+__global__ void __launch_bounds__(NM_THREADS(G)) k_ops_norm(fomoe_b200_norm_args_t A) {
+    __shared__ float s_red[NM_THREADS(G) / 32];
     const int gt = threadIdx.x % G;
-    const int row = blockIdx.x * (NM_THREADS / G) + threadIdx.x / G;
+    const int row = blockIdx.x * (NM_THREADS(G) / G) + threadIdx.x / G;
     if (row >= A.n_tokens) return; /* whole warps (G = 32), or nobody (G = the block) */
     const int n = A.n;
+    if (VEC && G > 32 && threadIdx.x == 0 && row + NM_AHEAD < A.n_tokens) { /* a row that a later block will read, into L2 */
+        const int64_t r = row + NM_AHEAD;
+        const int xb = A.x_type ? 2 : 4, bb = A.block_type ? 2 : 4;
+        fb_prefetch_l2(reinterpret_cast<const uint8_t *>(A.x) + r * A.x_stride * xb, (uint32_t)(n * xb));
+        if (A.block) fb_prefetch_l2(reinterpret_cast<const uint8_t *>(A.block) + r * A.block_stride * bb, (uint32_t)(n * bb));
+    }
     float x[IT][8], b[IT][8];
 #pragma unroll
     for (int it = 0; it < IT; it++) {
@@ -543,13 +552,18 @@ static bool nm_al(const void *p, int64_t stride, int bytes) {
 template <bool VEC>
 static void nm_launch(const fomoe_b200_norm_args_t &a, cudaStream_t st) {
     const int rw = (a.n_tokens + 7) / 8, T = a.n_tokens, n = a.n;
-    /* a warp to a row as long as the row fits its registers with enough rows to fill the card; else a block to a row */
-    if (n <= 256) k_ops_norm<VEC, 32, 1><<<rw, NM_THREADS, 0, st>>>(a);
-    else if (n <= 512) k_ops_norm<VEC, 32, 2><<<rw, NM_THREADS, 0, st>>>(a);
-    else if (n <= 2048) k_ops_norm<VEC, 256, 1><<<T, NM_THREADS, 0, st>>>(a);
-    else if (n <= 4096) k_ops_norm<VEC, 256, 2><<<T, NM_THREADS, 0, st>>>(a);
-    else if (n <= 8192) k_ops_norm<VEC, 256, 4><<<T, NM_THREADS, 0, st>>>(a);
-    else k_ops_norm<VEC, 256, 8><<<T, NM_THREADS, 0, st>>>(a);
+    /* one run of columns a thread while the rows do not fill the card (1 x 4096: 3.2 us, with two runs 3.9), two and more
+     * blocks to an SM when they do (8192 x 4096: 76 us, with one run 80) */
+    const bool few = T <= NM_FEW;
+    if (n <= 256) k_ops_norm<VEC, 32, 1><<<rw, 256, 0, st>>>(a);
+    else if (n <= 512) k_ops_norm<VEC, 32, 2><<<rw, 256, 0, st>>>(a);
+    else if (n <= 1024) k_ops_norm<VEC, 128, 1><<<T, 128, 0, st>>>(a);
+    else if (n <= 2048) k_ops_norm<VEC, 256, 1><<<T, 256, 0, st>>>(a);
+    else if (n <= 4096 && few) k_ops_norm<VEC, 512, 1><<<T, 512, 0, st>>>(a);
+    else if (n <= 4096) k_ops_norm<VEC, 256, 2><<<T, 256, 0, st>>>(a);
+    else if (n <= 8192 && few) k_ops_norm<VEC, 1024, 1><<<T, 1024, 0, st>>>(a);
+    else if (n <= 8192) k_ops_norm<VEC, 512, 2><<<T, 512, 0, st>>>(a);
+    else k_ops_norm<VEC, 1024, 2><<<T, 1024, 0, st>>>(a);
 }
 
 extern "C" int ops_launch_norm(const fomoe_b200_norm_args_t *a, void *stream) {
@@ -601,10 +615,9 @@ extern "C" int ops_rows_init(void) {
 #define RT_RK(N) RK(k_ops_route<N>);
     RT_SIZES(RT_RK)
 #undef RT_RK
-    RK((k_ops_norm<true, 32, 1>)); RK((k_ops_norm<true, 32, 2>)); RK((k_ops_norm<true, 256, 1>));
-    RK((k_ops_norm<true, 256, 2>)); RK((k_ops_norm<true, 256, 4>)); RK((k_ops_norm<true, 256, 8>));
-    RK((k_ops_norm<false, 32, 1>)); RK((k_ops_norm<false, 32, 2>)); RK((k_ops_norm<false, 256, 1>));
-    RK((k_ops_norm<false, 256, 2>)); RK((k_ops_norm<false, 256, 4>)); RK((k_ops_norm<false, 256, 8>));
+#define NM_RK(G, IT) RK((k_ops_norm<true, G, IT>)); RK((k_ops_norm<false, G, IT>));
+    NM_RK(32, 1) NM_RK(32, 2) NM_RK(128, 1) NM_RK(256, 1) NM_RK(512, 1) NM_RK(256, 2) NM_RK(1024, 1) NM_RK(512, 2) NM_RK(1024, 2)
+#undef NM_RK
     RK(k_ops_quantize<true>); RK(k_ops_quantize<false>);
 #undef RK
     return rc;

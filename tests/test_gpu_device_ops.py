@@ -188,7 +188,7 @@ def check_f8(q, s, want, tol):
 
 
 SIZES = [(1, 1), (1, 128), (3, 7), (5, 64), (2, 130), (9, 256), (4, 264), (300, 512), (3, 1000), (2, 1024), (7, 2048),
-         (2, 2050), (3, 2880), (1, 4096), (3, 5000), (2, 7177), (2, 8192), (2, 16383), (1, 16384)]
+         (2, 2050), (3, 2880), (1, 4096), (3, 5000), (2, 7177), (2, 8192), (2, 16383), (1, 16384), (1200, 2888), (1190, 4100), (1185, 3001)]
 
 
 @pytest.mark.parametrize("T,n", SIZES)
@@ -287,6 +287,27 @@ def test_quantize(ops, T, n, dt):
     wide = torch.cat([x, x], 1)[:, n:]   # strided, perhaps unaligned rows
     q2, s2 = ops.f8_quantize(wide)
     assert (q2.view(torch.uint8) == q.view(torch.uint8)).all() and (s2 == s).all()
+
+
+def test_quotients_are_rounded_once(ops):
+    """x / scale for many pairs, as IEEE division rounds it: the e4m3 numbers are the division's."""
+    g = gen(77)
+    x = (torch.exp2(40 * torch.rand(2000, 1, generator=g, device="cuda") - 20) * randn(g, 2000, 8192)).float()
+    # values beside the borders between two e4m3 numbers: (m + 1/2) / 8 of a power of two times the scale
+    q, s = ops.f8_quantize(x)
+    b = x.view(2000, 64, 128)
+    m = torch.randint(0, 240, b.shape, generator=g, device="cuda")
+    edge = torch.exp2(torch.div(m, 16, rounding_mode="floor").float() - 7) * (1 + (2 * (m % 8) + 1).float() / 16) * s[:, :, None]
+    step = torch.randint(-2, 3, b.shape, generator=g, device="cuda", dtype=torch.int32)
+    edge = (edge.view(torch.int32) + step).view(torch.float32)
+    edge[:, :, 0] = 448 * s                         # keeps the scale
+    y = edge.view(2000, 8192)
+    for v in (x, y):
+        q, s = ops.f8_quantize(v)
+        amax = v.view(2000, 64, 128).abs().amax(2).clamp(min=TINY)
+        assert (s == torch.div(amax, torch.full_like(amax, 448.0))).all()
+        want = torch.div(v.view(2000, 64, 128), s[:, :, None]).to(torch.float8_e4m3fn).view(2000, 8192)
+        assert (q.view(torch.uint8) == want.view(torch.uint8)).all()
 
 
 def test_quantize_extremes(ops):
