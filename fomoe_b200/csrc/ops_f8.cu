@@ -781,6 +781,30 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(NB * NT)) : "memory");
 }
 
+/* ------------------------------------------------------------------ kernels of one call, one after the other
+ * Launched with the programmatic-serialization attribute a kernel may start while the one before it in the stream ends:
+ * what it does before f8_after() overlaps that end and must not touch anything the kernel before it writes; f8_after()
+ * returns when that kernel has completed and its writes are visible.  f8_next() in the kernel before lets the next one start
+ * that early (else it starts as the blocks exit). */
+__device__ __forceinline__ void f8_after() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void f8_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... P, typename... A>
+static int f8_launch_after(void (*k)(P...), dim3 grid, int threads, int smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t c = {};
+    cudaLaunchAttribute at[1];
+    c.gridDim = grid;
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = at;
+    c.numAttrs = 1;
+    const cudaError_t rc = cudaLaunchKernelEx(&c, k, args...);
+    return (int)(rc != cudaSuccess ? rc : cudaGetLastError());
+}
+
 /* ------------------------------------------------------------------ few rows: the weights' bytes are all that counts
  * Up to 16 rows of a, or single pairs of an expert.  A block of 8 warps takes 16 weight rows; warp w takes the units
  * (blocks of k; of all slots of a token for the down product) w, w + 8, ..., and the eight partial sums meet in shared
@@ -814,9 +838,10 @@ __device__ __forceinline__ void fr_ask(uint32_t slot, const uint8_t *r0, const u
 
 __device__ __forceinline__ void fr_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
-/* the oldest unit in flight has landed: the lane's pieces */
+/* the oldest of RING units in flight has landed: the lane's pieces */
+template <int RING>
 __device__ __forceinline__ void fr_take(uint4 (&w)[4], uint32_t slot) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(FR_RING - 1) : "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
 #pragma unroll
     for (int i = 0; i < 4; i++) w[i] = fb_lds128(slot + (threadIdx.x & 31) * 16u + 512u * i);
 }
@@ -861,24 +886,34 @@ __global__ void __launch_bounds__(32 * FR_WARPS) k_f8_few(const fr_args_t P) {
         if (kb < kbs) fr_ask(ring_u + i * 2048u, r0, r1, kb * 128 + 16 * t, P.k);
         fr_commit();
     }
-    float acc[C8][4] = {};
-    int slot = 0;
-    for (int kb = warp; kb < kbs; kb += FR_WARPS) {
+    uint4 nx[C8][2];
+    float n0s[C8], n1s[C8], nb = 0.0f;
+    auto ahead = [&](int kb) { /* the rows' values and the scales of a block, a block ahead of their use */
         const int at = kb * 128 + 16 * t;
         const uint4 z = make_uint4(0, 0, 0, 0);
-        uint4 x[C8][2];
-        float s0[C8], s1[C8];
-        const float sb = __ldg(bs + kb);
+        if (kb >= kbs) return;
+        nb = __ldg(bs + kb);
 #pragma unroll
         for (int h = 0; h < C8; h++) {
             const uint8_t *xp = P.a + (int64_t)min(8 * h + g, P.m - 1) * P.a_stride + at;
-            x[h][0] = at < P.k ? __ldg(reinterpret_cast<const uint4 *>(xp)) : z;
-            x[h][1] = at + 64 < P.k ? __ldg(reinterpret_cast<const uint4 *>(xp + 64)) : z;
-            s0[h] = __ldg(P.a_scales + (int64_t)min(8 * h + 2 * t, P.m - 1) * P.as_stride + kb);
-            s1[h] = __ldg(P.a_scales + (int64_t)min(8 * h + 2 * t + 1, P.m - 1) * P.as_stride + kb);
+            nx[h][0] = at < P.k ? __ldg(reinterpret_cast<const uint4 *>(xp)) : z;
+            nx[h][1] = at + 64 < P.k ? __ldg(reinterpret_cast<const uint4 *>(xp + 64)) : z;
+            n0s[h] = __ldg(P.a_scales + (int64_t)min(8 * h + 2 * t, P.m - 1) * P.as_stride + kb);
+            n1s[h] = __ldg(P.a_scales + (int64_t)min(8 * h + 2 * t + 1, P.m - 1) * P.as_stride + kb);
         }
+    };
+    ahead(warp);
+    float acc[C8][4] = {};
+    int slot = 0;
+    for (int kb = warp; kb < kbs; kb += FR_WARPS) {
+        uint4 x[C8][2];
+        float s0[C8], s1[C8];
+        const float sb = nb;
+#pragma unroll
+        for (int h = 0; h < C8; h++) x[h][0] = nx[h][0], x[h][1] = nx[h][1], s0[h] = n0s[h], s1[h] = n1s[h];
+        ahead(kb + FR_WARPS);
         uint4 w[4];
-        fr_take(w, ring_u + slot * 2048u);
+        fr_take<FR_RING>(w, ring_u + slot * 2048u);
 #pragma unroll
         for (int h = 0; h < C8; h++) {
             float c[4];
@@ -922,7 +957,8 @@ typedef struct {
     const float *weights;
     const uint8_t *gate_up, *down;
     const float *gu_scales, *dn_scales;
-    float *act; /* [pairs][n_inter] */
+    uint8_t *act_q; /* [pairs][n_inter] */
+    float *act_scales;
     __nv_bfloat16 *out;
     int64_t out_stride;
     int *status;
@@ -935,121 +971,158 @@ __device__ __forceinline__ int fr_expert(const fr_experts_t &P, int t, int j) {
     return (unsigned)e < (unsigned)P.n_experts ? e : -1;
 }
 
-/* act[pair][16 rows] = silu(gate x) (up x); block (rows, slot, token) */
-__global__ void __launch_bounds__(32 * FR_WARPS) k_f8_few_gate_up(const fr_experts_t P) {
-    __shared__ float s_part[FR_WARPS][2][16];
+/* act[pair][128 rows] = silu(gate x) (up x) in FP8; block (128 rows, slot, token) of 16 warps: warp w has rows
+ * 16 (w % 8) .. of the 128 and every other block of k, both matrices.  One block holds a whole block of activations, so its
+ * amax meets in shared memory; 192 KB an SM are in flight from the start to the end of a block. */
+#define FG_WARPS 16
+#define FG_RING 6
+#define FG_SMEM (FG_WARPS * FG_RING * 2048)
+
+__global__ void __launch_bounds__(32 * FG_WARPS) k_f8_few_gate_up(const __grid_constant__ fr_experts_t P) {
+    __shared__ __align__(16) float s_part[2][128];
     extern __shared__ __align__(16) uint8_t ring[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-    const uint32_t ring_u = fb_smem_u32(ring) + warp * (FR_RING * 2048u);
-    const int t = blockIdx.z, j = blockIdx.y, n0 = blockIdx.x * 16, H = P.n_embd, I = P.n_inter, kbs = H / 128;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3, khalf = warp >> 3;
+    const uint32_t ring_u = fb_smem_u32(ring) + warp * (FG_RING * 2048u);
+    const int t = blockIdx.z, j = blockIdx.y, n0 = blockIdx.x * 128, r0 = 16 * (warp & 7), H = P.n_embd, I = P.n_inter, kbs = H / 128;
     const int e = fr_expert(P, t, j);
+    f8_next(); /* (the down product's weights may be asked for while this one runs) */
     if (e < 0) {
         if (threadIdx.x == 0 && P.ids[t * P.top_k + j] != -1) *P.status = FB_ST_BAD_ID;
         return;
     }
-    const uint8_t *r0 = P.gate_up + ((int64_t)e * 2 * I + n0 + g) * H;
+    const uint8_t *w0 = P.gate_up + ((int64_t)e * 2 * I + n0 + r0 + g) * H;
     const int64_t up = (int64_t)I * H, low = (int64_t)8 * H;
     const float *gs = P.gu_scales + ((int64_t)e * 2 * (I / 128) + (n0 >> 7)) * kbs, *us = gs + (int64_t)(I / 128) * kbs;
     const uint8_t *x = P.x + t * P.x_stride + 16 * t4;
     const float *xs = P.x_scales + t * P.xs_stride;
+    const int its = (kbs - khalf + 1) / 2; /* this warp's blocks of k: khalf, khalf + 2, ... */
     /* units in turn: gate and up of a block of k */
 #pragma unroll
-    for (int i = 0; i < FR_RING; i++) {
-        const int kb = warp + FR_WARPS * (i / 2);
-        const uint8_t *r = r0 + (i & 1 ? up : 0);
-        if (kb < kbs) fr_ask(ring_u + i * 2048u, r, r + low, kb * 128 + 16 * t4, H);
+    for (int i = 0; i < FG_RING; i++) {
+        const uint8_t *r = w0 + (i & 1 ? up : 0);
+        if (i / 2 < its) fr_ask(ring_u + i * 2048u, r, r + low, (khalf + 2 * (i / 2)) * 128 + 16 * t4, H);
         fr_commit();
+    }
+    /* all factors at once, an iteration's in the lane of its number: one latency for them, not one a block */
+    float fg[2] = {}, fu[2] = {};
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int kb = khalf + 2 * (lane + 32 * h);
+        if (kb < kbs) {
+            const float sx = __ldg(xs + kb);
+            fg[h] = sx * __ldg(gs + kb);
+            fu[h] = sx * __ldg(us + kb);
+        }
     }
     float acc[2][2] = {}; /* {gate, up} x {row g, row g + 8} (every column holds the same token) */
     int slot = 0;
-    for (int kb = warp; kb < kbs; kb += FR_WARPS) {
-        const uint4 x0 = __ldg(reinterpret_cast<const uint4 *>(x + kb * 128)), x1 = __ldg(reinterpret_cast<const uint4 *>(x + kb * 128 + 64));
-        const float sx = __ldg(xs + kb), f[2] = {sx * __ldg(gs + kb), sx * __ldg(us + kb)};
-        const int next = kb + FR_WARPS * (FR_RING / 2);
+    uint4 nx0 = __ldg(reinterpret_cast<const uint4 *>(x + min(khalf, kbs - 1) * 128));
+    uint4 nx1 = __ldg(reinterpret_cast<const uint4 *>(x + min(khalf, kbs - 1) * 128 + 64));
+    for (int it = 0; it < its; it++) {
+        const uint4 x0 = nx0, x1 = nx1;
+        const int nk = min(khalf + 2 * (it + 1), kbs - 1);
+        nx0 = __ldg(reinterpret_cast<const uint4 *>(x + nk * 128));
+        nx1 = __ldg(reinterpret_cast<const uint4 *>(x + nk * 128 + 64));
 #pragma unroll
         for (int m = 0; m < 2; m++) {
             uint4 w[4];
             float c[4];
-            fr_take(w, ring_u + slot * 2048u);
+            fr_take<FG_RING>(w, ring_u + slot * 2048u);
             fr_block(c, w, x0, x1);
-            acc[m][0] = fmaf(c[0], f[m], acc[m][0]);
-            acc[m][1] = fmaf(c[2], f[m], acc[m][1]);
-            const uint8_t *r = r0 + (m ? up : 0);
-            if (next < kbs) fr_ask(ring_u + slot * 2048u, r, r + low, next * 128 + 16 * t4, H);
+            const float f = __shfl_sync(FULL, m ? (it < 32 ? fu[0] : fu[1]) : (it < 32 ? fg[0] : fg[1]), it & 31);
+            acc[m][0] = fmaf(c[0], f, acc[m][0]);
+            acc[m][1] = fmaf(c[2], f, acc[m][1]);
+            const int next = it + FG_RING / 2;
+            const uint8_t *r = w0 + (m ? up : 0);
+            if (next < its) fr_ask(ring_u + slot * 2048u, r, r + low, (khalf + 2 * next) * 128 + 16 * t4, H);
             fr_commit();
-            slot = (slot + 1) % FR_RING;
+            slot = slot + 1 == FG_RING ? 0 : slot + 1;
         }
     }
-    if (t4 == 0) {
-        s_part[warp][0][g] = acc[0][0];
-        s_part[warp][0][g + 8] = acc[0][1];
-        s_part[warp][1][g] = acc[1][0];
-        s_part[warp][1][g + 8] = acc[1][1];
+    /* the two halves of k, then the rows of the block */
+    if (khalf && t4 == 0) {
+        s_part[0][r0 + g] = acc[0][0];
+        s_part[0][r0 + g + 8] = acc[0][1];
+        s_part[1][r0 + g] = acc[1][0];
+        s_part[1][r0 + g + 8] = acc[1][1];
     }
     __syncthreads();
-    if (threadIdx.x < 16) {
-        float vg = 0.0f, vu = 0.0f;
+    if (!khalf && t4 == 0) {
+        s_part[0][r0 + g] = f8_silu_mul(acc[0][0] + s_part[0][r0 + g], acc[1][0] + s_part[1][r0 + g]);
+        s_part[0][r0 + g + 8] = f8_silu_mul(acc[0][1] + s_part[0][r0 + g + 8], acc[1][1] + s_part[1][r0 + g + 8]);
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const float4 v = *reinterpret_cast<const float4 *>(&s_part[0][4 * lane]);
+        float amax = ops_amax(ops_amax(ops_amax(ops_amax(0.0f, v.x), v.y), v.z), v.w);
 #pragma unroll
-        for (int w = 0; w < FR_WARPS; w++) {
-            vg += s_part[w][0][threadIdx.x];
-            vu += s_part[w][1][threadIdx.x];
-        }
-        P.act[(int64_t)(t * (P.top_k + P.has_shared) + j) * I + n0 + threadIdx.x] = f8_silu_mul(vg, vu);
+        for (int s = 16; s > 0; s >>= 1) amax = ops_amax(amax, __shfl_xor_sync(FULL, amax, s));
+        const float sc = ops_f8_scale(amax), inv = __frcp_rn(sc);
+        const int64_t row = (int64_t)t * (P.top_k + P.has_shared) + j;
+        *reinterpret_cast<uint32_t *>(P.act_q + row * I + n0 + 4 * lane) = ops_f8_pack4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        if (lane == 0) P.act_scales[row * (I / 128) + (n0 >> 7)] = sc;
     }
 }
 
-/* out[t][16 rows] = sum over the slots of weight (down act), the activations brought to FP8 on the way; block (rows, token).
+/* out[t][16 rows] = sum over the slots of weight (down act); block (rows, token).
  * The warps share the (slot, block of k) units of the token. */
-__global__ void __launch_bounds__(32 * FR_WARPS) k_f8_few_down(const fr_experts_t P) {
+#define FD_RING 6
+#define FD_SMEM (FR_WARPS * FD_RING * 2048)
+#define FD_SMEM_MOST (FD_SMEM + 96 * 1024) /* with the activations of a token */
+
+__global__ void __launch_bounds__(32 * FR_WARPS) k_f8_few_down(const __grid_constant__ fr_experts_t P) {
     __shared__ float s_part[FR_WARPS][16];
-    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ int s_e[OPS_MAX_K + 1];
+    extern __shared__ __align__(16) uint8_t ring[]; /* the rings, then the token's activations in FP8, then their scales */
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-    const uint32_t ring_u = fb_smem_u32(ring) + warp * (FR_RING * 2048u);
+    const uint32_t ring_u = fb_smem_u32(ring) + warp * (FD_RING * 2048u);
     const int t = blockIdx.y, n0 = blockIdx.x * 16, H = P.n_embd, I = P.n_inter, kbs = I / 128;
     const int slots = P.top_k + P.has_shared, units = slots * kbs;
+    uint8_t *s_q = ring + FD_SMEM;
+    float *s_f = reinterpret_cast<float *>(s_q + slots * I); /* [units]: activation scale x weight scale x slot weight */
+    if (threadIdx.x < slots) s_e[threadIdx.x] = fr_expert(P, t, threadIdx.x);
+    __syncthreads();
     auto ask = [&](int un, int slot) {
         if (un < units) {
-            const int j = un / kbs, kb = un - j * kbs, e = fr_expert(P, t, j);
+            const int j = un / kbs, kb = un - j * kbs, e = s_e[j];
             const uint8_t *r0 = P.down + ((int64_t)max(e, 0) * H + n0 + g) * I;
             if (e >= 0) fr_ask(ring_u + slot * 2048u, r0, r0 + (int64_t)8 * I, kb * 128 + 16 * t4, I);
         }
         fr_commit();
     };
 #pragma unroll
-    for (int i = 0; i < FR_RING; i++) ask(warp + FR_WARPS * i, i);
+    for (int i = 0; i < FD_RING; i++) ask(warp + FR_WARPS * i, i);
+    f8_after(); /* the activations are there */
+    /* the token's activations (16 bytes a thread) and each unit's factor */
+    const int64_t row0 = (int64_t)t * slots;
+    for (int i = threadIdx.x; i < units * 8; i += 32 * FR_WARPS)
+        if (s_e[i / (kbs * 8)] >= 0)
+            reinterpret_cast<uint4 *>(s_q)[i] = *reinterpret_cast<const uint4 *>(P.act_q + row0 * I + 16 * i);
+    for (int un = threadIdx.x; un < units; un += 32 * FR_WARPS) {
+        const int j = un / kbs, kb = un - j * kbs, e = s_e[j];
+        if (e >= 0)
+            s_f[un] = (j < P.top_k ? P.weights[t * P.top_k + j] : 1.0f) * P.act_scales[row0 * kbs + un] *
+                      __ldg(P.dn_scales + ((int64_t)e * (H / 128) + (n0 >> 7)) * kbs + kb);
+    }
+    __syncthreads();
     float acc[2] = {};
     int slot = 0;
     for (int un = warp; un < units; un += FR_WARPS) {
-        const int j = un / kbs, kb = un - j * kbs, e = fr_expert(P, t, j);
-        if (e >= 0) { /* the same for the whole warp */
-            const float4 a = *reinterpret_cast<const float4 *>(P.act + (int64_t)(t * slots + j) * I + kb * 128 + 4 * lane);
-            const float f = (j < P.top_k ? P.weights[t * P.top_k + j] : 1.0f) *
-                            __ldg(P.dn_scales + ((int64_t)e * (H / 128) + (n0 >> 7)) * kbs + kb);
-            float amax = ops_amax(ops_amax(ops_amax(ops_amax(0.0f, a.x), a.y), a.z), a.w);
-#pragma unroll
-            for (int s = 16; s > 0; s >>= 1) amax = ops_amax(amax, __shfl_xor_sync(FULL, amax, s));
-            const float sc = ops_f8_scale(amax), inv = __frcp_rn(sc);
-            const uint32_t q = ops_f8_pack4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-            uint4 x0, x1;
-            x0.x = __shfl_sync(FULL, q, 4 * t4);
-            x0.y = __shfl_sync(FULL, q, 4 * t4 + 1);
-            x0.z = __shfl_sync(FULL, q, 4 * t4 + 2);
-            x0.w = __shfl_sync(FULL, q, 4 * t4 + 3);
-            x1.x = __shfl_sync(FULL, q, 16 + 4 * t4);
-            x1.y = __shfl_sync(FULL, q, 16 + 4 * t4 + 1);
-            x1.z = __shfl_sync(FULL, q, 16 + 4 * t4 + 2);
-            x1.w = __shfl_sync(FULL, q, 16 + 4 * t4 + 3);
+        if (s_e[un / kbs] >= 0) {
+            const uint4 x0 = *reinterpret_cast<const uint4 *>(s_q + un * 128 + 16 * t4);
+            const uint4 x1 = *reinterpret_cast<const uint4 *>(s_q + un * 128 + 64 + 16 * t4);
+            const float f = s_f[un];
             uint4 w[4];
             float c[4];
-            fr_take(w, ring_u + slot * 2048u);
+            fr_take<FD_RING>(w, ring_u + slot * 2048u);
             fr_block(c, w, x0, x1);
-            acc[0] = fmaf(c[0], f * sc, acc[0]);
-            acc[1] = fmaf(c[2], f * sc, acc[1]);
+            acc[0] = fmaf(c[0], f, acc[0]);
+            acc[1] = fmaf(c[2], f, acc[1]);
         } else {
-            asm volatile("cp.async.wait_group %0;" ::"n"(FR_RING - 1) : "memory");
+            asm volatile("cp.async.wait_group %0;" ::"n"(FD_RING - 1) : "memory");
         }
-        ask(un + FR_WARPS * FR_RING, slot);
-        slot = (slot + 1) % FR_RING;
+        ask(un + FR_WARPS * FD_RING, slot);
+        slot = slot + 1 == FD_RING ? 0 : slot + 1;
     }
     if (t4 == 0) {
         s_part[warp][g] = acc[0];
@@ -1216,8 +1289,7 @@ extern "C" void ops_experts_layout(const fomoe_b200_f8_experts_args_t *a, ops_ex
     PART(xp_scales, np * (a->n_embd / 128) * 4);
     PART(act_q, np * a->n_inter);
     PART(act_scales, np * (a->n_inter / 128) * 4);
-    /* (the activations in fp32 where there are few pairs) */
-    PART(dots, np * (a->n_embd > 2 * a->n_inter ? a->n_embd * 2ull : a->n_inter * 4ull));
+    PART(dots, np * a->n_embd * 2);
     PART(dot_scales, np * (a->n_embd / 128) * 4);
 #undef PART
     w->bytes = at;
@@ -1230,14 +1302,15 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     ops_experts_ws_t w;
     ops_experts_layout(a, &w);
     const int few_slots = a->top_k + (a->has_shared ? 1 : 0);
-    if (w.n_pairs <= EXPERTS_FEW) {
+    const int few_smem = FD_SMEM + few_slots * a->n_inter + few_slots * (a->n_inter / 128) * 4; /* of the down product */
+    if (w.n_pairs <= EXPERTS_FEW && few_smem <= FD_SMEM_MOST) {
         const fr_experts_t f = {a->n_embd, a->n_inter, a->n_experts, a->top_k, a->has_shared ? 1 : 0, a->n_tokens * a->top_k, a->x,
                                 a->x_stride, a->x_scales, a->x_scales_stride, a->ids, a->weights, a->gate_up, a->down,
-                                a->gate_up_scales, a->down_scales, (float *)(ws + w.dots), (__nv_bfloat16 *)a->out, a->out_stride, status};
-        k_f8_few_gate_up<<<dim3(a->n_inter / 16, few_slots, a->n_tokens), 32 * FR_WARPS, FR_SMEM, st>>>(f);
-        k_f8_few_down<<<dim3(a->n_embd / 16, a->n_tokens), 32 * FR_WARPS, FR_SMEM, st>>>(f);
+                                a->gate_up_scales, a->down_scales, ws + w.act_q, (float *)(ws + w.act_scales), (__nv_bfloat16 *)a->out, a->out_stride, status};
+        k_f8_few_gate_up<<<dim3(a->n_inter / 128, few_slots, a->n_tokens), 32 * FG_WARPS, FG_SMEM, st>>>(f);
         *launches += 2;
-        return (int)cudaGetLastError();
+        const int rc = (int)cudaGetLastError();
+        return rc ? rc : f8_launch_after(k_f8_few_down, dim3(a->n_embd / 16, a->n_tokens), 32 * FR_WARPS, few_smem, st, f);
     }
     const int n_routed = a->n_tokens * a->top_k, n_shared = a->has_shared ? a->n_tokens : 0, H = a->n_embd, I = a->n_inter;
     int *counts = (int *)(ws + w.counts), *pairs = (int *)(ws + w.pairs), *pos = (int *)(ws + w.pos);
@@ -1305,8 +1378,8 @@ extern "C" int ops_f8_init(ops_device_t *d) {
 #define RM(MODE, NT, SPLIT)                                                                                             \
     rc |= (int)cudaFuncSetAttribute((k_f8_mma<MODE, NT, SPLIT>), cudaFuncAttributeMaxDynamicSharedMemorySize, f8_cfg<MODE, NT>::SMEM)
     RK(k_ops_combine); RK(k_ops_permute);
-#define RF(k) rc |= (int)cudaFuncSetAttribute((k), cudaFuncAttributeMaxDynamicSharedMemorySize, FR_SMEM)
-    RF(k_f8_few<1>); RF(k_f8_few<2>); RF(k_f8_few_gate_up); RF(k_f8_few_down);
+#define RF(k, smem) rc |= (int)cudaFuncSetAttribute((k), cudaFuncAttributeMaxDynamicSharedMemorySize, (smem))
+    RF(k_f8_few<1>, FR_SMEM); RF(k_f8_few<2>, FR_SMEM); RF(k_f8_few_gate_up, FG_SMEM); RF(k_f8_few_down, FD_SMEM_MOST);
 #undef RF
     RM(F8_DENSE, 256, false); RM(F8_DENSE, 128, false); RM(F8_DENSE, 128, true); RM(F8_GATE_UP, 256, false);
     RM(F8_DOWN, 256, false);
