@@ -1270,10 +1270,16 @@ __global__ void __launch_bounds__(256) k_ops_combine(const __half *dots, const f
     }
 }
 
-/* up to this many pairs each pair reads its own expert's weights */
-#ifndef EXPERTS_FEW
-#define EXPERTS_FEW 32
-#endif
+/* Each pair by itself, or bucketed by expert: microseconds of either.  Few pairs stream their experts' weights once a pair
+ * (5 TB/s and 8 us around it: one token with 11 experts of 4096 x 1024 34.5 us, bucketed 59; 64 pairs of 2048 x 768 67 and
+ * 74 us), bucketed they are read once an expert but five kernels and their tiles come first (4096 x 1024, 45 pairs: 114 us
+ * by themselves, bucketed 102).  How many different experts there will be is known on the device only: the expectation of
+ * equally likely ones stands for it. */
+static int experts_few(const fomoe_b200_f8_experts_args_t *a, int n_pairs) {
+    const double bytes = 3.0 * a->n_embd * a->n_inter, routed = (double)a->n_tokens * a->top_k;
+    const double hit = a->n_experts * (1.0 - exp(-routed / a->n_experts)) + (a->has_shared ? 1.0 : 0.0);
+    return n_pairs <= 256 && 8.0 + n_pairs * bytes / 5.0e6 <= 30.0 + hit * bytes / 5.5e6;
+}
 
 extern "C" void ops_experts_layout(const fomoe_b200_f8_experts_args_t *a, ops_experts_ws_t *w) {
     const uint64_t np = (uint64_t)a->n_tokens * (a->top_k + (a->has_shared ? 1 : 0));
@@ -1303,7 +1309,7 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     ops_experts_layout(a, &w);
     const int few_slots = a->top_k + (a->has_shared ? 1 : 0);
     const int few_smem = FD_SMEM + few_slots * a->n_inter + few_slots * (a->n_inter / 128) * 4; /* of the down product */
-    if (w.n_pairs <= EXPERTS_FEW && few_smem <= FD_SMEM_MOST) {
+    if (experts_few(a, w.n_pairs) && few_smem <= FD_SMEM_MOST) {
         const fr_experts_t f = {a->n_embd, a->n_inter, a->n_experts, a->top_k, a->has_shared ? 1 : 0, a->n_tokens * a->top_k, a->x,
                                 a->x_stride, a->x_scales, a->x_scales_stride, a->ids, a->weights, a->gate_up, a->down,
                                 a->gate_up_scales, a->down_scales, ws + w.act_q, (float *)(ws + w.act_scales), (__nv_bfloat16 *)a->out, a->out_stride, status};
