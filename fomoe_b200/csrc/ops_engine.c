@@ -93,6 +93,8 @@ uint64_t fomoe_b200_ops_kernel_launches(fomoe_b200_ops_t *o) { return o ? o->lau
         (o)->launches += (uint64_t)(n_launch);                                                         \
     } while (0)
 
+#define OPS_MOST (1 << 30) /* rows, columns: index arithmetic in 32 bits goes a little past them */
+
 static int is_float(int type) { return type == FOMOE_B200_F32 || type == FOMOE_B200_BF16; }
 static int fits(const void *p, int type) { /* aligned to its own type */
     return ((uintptr_t)p & (type == FOMOE_B200_F32 ? 3u : 1u)) == 0;
@@ -109,7 +111,7 @@ int fomoe_b200_ops_route(fomoe_b200_ops_t *o, const fomoe_b200_route_config_t *c
     NEED(o, c->topk_group > 0 && c->topk_group <= c->n_group, "route: topk_group is 1 to n_group");
     NEED(o, c->group_best == 1 || c->group_best == 2, "route: group_best is 1 or 2");
     NEED(o, is_float(logits_type), "route: logits are F32 or BF16");
-    NEED(o, n_tokens >= 0, "route: %d tokens", n_tokens);
+    NEED(o, n_tokens >= 0 && n_tokens <= OPS_MOST, "route: %d tokens", n_tokens);
     if (n_tokens == 0) return 0;
     NEED(o, logits && ids && weights, "route: a pointer is NULL");
     NEED(o, fits(logits, logits_type) && fits(bias, FOMOE_B200_F32) && fits(ids, FOMOE_B200_F32) && fits(weights, FOMOE_B200_F32), "route: a pointer is not aligned to its type");
@@ -131,7 +133,7 @@ int fomoe_b200_ops_route(fomoe_b200_ops_t *o, const fomoe_b200_route_config_t *c
 int fomoe_b200_ops_norm(fomoe_b200_ops_t *o, const fomoe_b200_norm_args_t *a, void *stream) {
     if (!o) return -1;
     NEED(o, a && a->n > 0 && a->n <= OPS_MAX_N, "norm: 1 to %d columns", OPS_MAX_N);
-    NEED(o, a->n_tokens >= 0, "norm: %d tokens", a->n_tokens);
+    NEED(o, a->n_tokens >= 0 && a->n_tokens <= OPS_MOST, "norm: %d tokens", a->n_tokens);
     if (a->n_tokens == 0) return 0;
     NEED(o, a->x && is_float(a->x_type) && fits(a->x, a->x_type), "norm: x is F32 or BF16, aligned to its type");
     NEED(o, a->x_stride >= a->n || a->n_tokens == 1, "norm: x_stride is below n");
@@ -165,19 +167,19 @@ int fomoe_b200_ops_norm(fomoe_b200_ops_t *o, const fomoe_b200_norm_args_t *a, vo
 int fomoe_b200_ops_f8_quantize(fomoe_b200_ops_t *o, int rows, int cols, const void *x, int x_type, int64_t x_stride,
                                uint8_t *q, int64_t q_stride, float *scales, int64_t scales_stride, void *stream) {
     if (!o) return -1;
-    NEED(o, rows >= 0 && cols > 0, "f8_quantize: %d x %d", rows, cols);
+    NEED(o, rows >= 0 && rows <= OPS_MOST && cols > 0 && cols <= OPS_MOST, "f8_quantize: %d x %d", rows, cols);
     if (rows == 0) return 0;
     NEED(o, x && q && scales, "f8_quantize: a pointer is NULL");
     NEED(o, is_float(x_type) && fits(x, x_type) && fits(scales, FOMOE_B200_F32), "f8_quantize: x is F32 or BF16, pointers aligned to their types");
     NEED(o, rows == 1 || (x_stride >= 0 && q_stride >= cols && scales_stride >= ((int64_t)cols + 127) / 128), "f8_quantize: a stride is too small");
-    NEED(o, (int64_t)rows * (((int64_t)cols + 127) / 128) <= (int64_t)16 * 0x7fffffff, "f8_quantize: too many blocks for one call");
     ON_DEVICE(o, "f8_quantize", 1, ops_launch_f8_quantize(rows, cols, x, x_type == FOMOE_B200_BF16, x_stride, q, q_stride, scales, scales_stride, stream));
     return 0;
 }
 
 int fomoe_b200_ops_f8_matmul(fomoe_b200_ops_t *o, const fomoe_b200_f8_matmul_args_t *args, void *stream) {
     if (!o) return -1;
-    NEED(o, args && args->m >= 0 && args->n >= 0 && args->k > 0 && args->k % 16 == 0, "f8_matmul: k is a positive multiple of 16");
+    NEED(o, args && args->m >= 0 && args->m <= OPS_MOST && args->n >= 0 && args->n <= OPS_MOST, "f8_matmul: m and n are 0 to 2^30");
+    NEED(o, args->k > 0 && args->k <= OPS_MOST && args->k % 16 == 0, "f8_matmul: k is a positive multiple of 16");
     if (args->m == 0 || args->n == 0) return 0;
     fomoe_b200_f8_matmul_args_t own = *args, *a = &own;
     if (a->m == 1) a->a_stride = a->k; /* a single row's stride means nothing */

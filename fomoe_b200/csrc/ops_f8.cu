@@ -1319,13 +1319,28 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
         return rc ? rc : f8_launch_after(k_f8_few_down, dim3(a->n_embd / 16, a->n_tokens), 32 * FR_WARPS, few_smem, st, f);
     }
     const int n_routed = a->n_tokens * a->top_k, n_shared = a->has_shared ? a->n_tokens : 0, H = a->n_embd, I = a->n_inter;
-    int *counts = (int *)(ws + w.counts), *pairs = (int *)(ws + w.pairs), *pos = (int *)(ws + w.pos);
-    int4 *items = (int4 *)(ws + w.counts + 256);
     const int64_t recs = a->n_experts + (a->has_shared ? 1 : 0);
+    int *counts = (int *)(ws + w.counts), *pairs = (int *)(ws + w.pairs), *pos = (int *)(ws + w.pos);
+    int *block_counts = (int *)(ws + w.block_counts);
+    int4 *items = (int4 *)(ws + w.counts + 256);
+    f8_args_t gu = {}, dn;
+    gu.counts = counts, gu.pairs = pairs, gu.items = items, gu.status = status;
+    dn = gu;
+    gu.n = I, gu.k = H;
+    gu.a_scales = (const float *)(ws + w.xp_scales), gu.as_stride = H / 128;
+    gu.b_scales = a->gate_up_scales, gu.bs_stride = H / 128, gu.bs_rec = (int64_t)(2 * I / 128) * (H / 128), gu.b_rec_rows = 2 * I;
+    gu.act_q = ws + w.act_q, gu.act_scales = (float *)(ws + w.act_scales);
+    dn.n = H, dn.k = I;
+    dn.a_scales = gu.act_scales, dn.as_stride = I / 128;
+    dn.b_scales = a->down_scales, dn.bs_stride = I / 128, dn.bs_rec = (int64_t)(H / 128) * (I / 128), dn.b_rec_rows = H;
+    dn.out = ws + w.dots, dn.out_stride = H, dn.out_tma = 1, dn.out_scales = (float *)(ws + w.dot_scales);
+    int rc = f8_map(&gu.ta, ws + w.xp, H, w.n_pairs, H, 32) | f8_map(&gu.tb, a->gate_up, H, recs * 2 * I, H, 128) |
+             f8_map(&dn.ta, ws + w.act_q, I, w.n_pairs, I, 32) | f8_map(&dn.tb, a->down, I, recs * H, I, 256) |
+             f8_map(&dn.to, ws + w.dots, 2ull * H, w.n_pairs, 2ull * H, 32);
+    if (rc) return rc;
     int run = (n_routed + BK_BLOCKS - 1) / BK_BLOCKS;
     run = run < BK_RUN ? BK_RUN : run;
     const int nb = (n_routed + run - 1) / run, bk_smem = a->n_experts * (BK_WARPS + 1) * 4;
-    int *block_counts = (int *)(ws + w.block_counts);
     if (nb > 1) {
         k_ops_bucket<true><<<nb, BK_THREADS, bk_smem, st>>>(a->ids, n_routed, run, a->n_tokens, a->n_experts, a->has_shared,
                                                           block_counts, counts, pairs, pos, items, status);
@@ -1336,26 +1351,11 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     k_ops_permute<<<(w.n_pairs + 7) / 8, 256, 0, st>>>(a->x, a->x_stride, a->x_scales, a->x_scales_stride, H, counts, pairs,
                                                       n_routed, a->top_k, n_shared, ws + w.xp, (float *)(ws + w.xp_scales));
     *launches += 2;
-    int rc = (int)cudaGetLastError();
-    if (rc) return rc;
+    rc = (int)cudaGetLastError();
     /* no more tiles than this (the device knows how many there are) */
     const int64_t tiles = w.n_pairs / 128 + recs;
-    f8_args_t p = {};
-    p.counts = counts, p.pairs = pairs, p.items = items, p.status = status;
-    p.n = I, p.k = H;
-    p.a_scales = (const float *)(ws + w.xp_scales), p.as_stride = H / 128;
-    p.b_scales = a->gate_up_scales, p.bs_stride = H / 128, p.bs_rec = (int64_t)(2 * I / 128) * (H / 128), p.b_rec_rows = 2 * I;
-    p.act_q = ws + w.act_q, p.act_scales = (float *)(ws + w.act_scales);
-    rc = f8_map(&p.ta, ws + w.xp, H, w.n_pairs, H, 32) | f8_map(&p.tb, a->gate_up, H, recs * 2 * I, H, 128);
-    if (!rc) rc = f8_launch<F8_GATE_UP, 256, false>(p, tiles * (I / 128), 1, n_sm, launches, st);
-    if (rc) return rc;
-    p.n = H, p.k = I;
-    p.a_scales = p.act_scales, p.as_stride = I / 128;
-    p.b_scales = a->down_scales, p.bs_stride = I / 128, p.bs_rec = (int64_t)(H / 128) * (I / 128), p.b_rec_rows = H;
-    p.out = ws + w.dots, p.out_stride = H, p.out_tma = 1, p.out_scales = (float *)(ws + w.dot_scales);
-    rc = f8_map(&p.ta, ws + w.act_q, I, w.n_pairs, I, 32) | f8_map(&p.tb, a->down, I, recs * H, I, 256) |
-         f8_map(&p.to, ws + w.dots, 2ull * H, w.n_pairs, 2ull * H, 32);
-    if (!rc) rc = f8_launch<F8_DOWN, 256, false>(p, tiles * ((H + 255) / 256), 1, n_sm, launches, st);
+    if (!rc) rc = f8_launch<F8_GATE_UP, 256, false>(gu, tiles * (I / 128), 1, n_sm, launches, st);
+    if (!rc) rc = f8_launch<F8_DOWN, 256, false>(dn, tiles * ((H + 255) / 256), 1, n_sm, launches, st);
     if (rc) return rc;
     const int vec = ((uintptr_t)a->out & 15) == 0 && (a->n_tokens == 1 || a->out_stride % 8 == 0);
     /* (the grid's y goes to 65535) */

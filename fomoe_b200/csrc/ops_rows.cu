@@ -579,31 +579,35 @@ extern "C" int ops_launch_norm(const fomoe_b200_norm_args_t *a, void *stream) {
     return (int)cudaGetLastError();
 }
 
-/* ------------------------------------------------------------------ rows to FP8: 16 threads per block of 128 */
+/* ------------------------------------------------------------------ rows to FP8: 16 threads per block of 128
+ * (4096 x 4096 bf16: 13.6 us, 3.7 TB/s; two or four pieces of 8 columns a thread are no faster and cost small calls 0.3 us) */
 template <bool VEC>
 __global__ void __launch_bounds__(256) k_ops_quantize(int rows, int cols, int nb, const void *x, int bf16, int64_t x_stride,
                                                      uint8_t *q, int64_t q_stride, float *scales, int64_t s_stride) {
-    const int64_t blk = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
-    const int64_t row = blk / nb;
-    const int b = (int)(blk - row * nb), c = b * 128 + (threadIdx.x & 15) * 8;
-    const bool in = row < rows && c < cols;
+    const uint32_t blk = blockIdx.x * 16 + (threadIdx.x >> 4), r = blk / (uint32_t)nb; /* (the host keeps rows * nb below 2^30) */
+    const int64_t row = r < (uint32_t)rows ? r : 0;
+    const int c = r < (uint32_t)rows ? (int)(blk - r * nb) * 128 + (threadIdx.x & 15) * 8 : cols;
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (in) nm_load8<VEC>(x, bf16, row * x_stride + c, cols - c, v);
-    nm_quant8<VEC>(q + row * q_stride, scales + row * s_stride, in ? c : cols, cols, v);
+    if (c < cols) nm_load8<VEC>(x, bf16, row * x_stride + c, cols - c, v);
+    nm_quant8<VEC>(q + row * q_stride, scales + row * s_stride, min(c, cols), cols, v);
 }
 
 extern "C" int ops_launch_f8_quantize(int rows, int cols, const void *x, int x_bf16, int64_t x_stride, uint8_t *q,
                                       int64_t q_stride, float *scales, int64_t scales_stride, void *stream) {
     const int nb = (cols + 127) / 128;
-    const int64_t grid = ((int64_t)rows * nb + 15) / 16;
     const bool vec = cols % 8 == 0 && nm_al(x, rows > 1 ? x_stride : 0, x_bf16 ? 2 : 4) && ((uintptr_t)q & 7) == 0 &&
                      (rows == 1 || q_stride % 8 == 0);
-    if (vec)
-        k_ops_quantize<true><<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>(rows, cols, nb, x, x_bf16, x_stride, q, q_stride,
-                                                                             scales, scales_stride);
-    else
-        k_ops_quantize<false><<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>(rows, cols, nb, x, x_bf16, x_stride, q,
-                                                                              q_stride, scales, scales_stride);
+    const int at_once = (1 << 30) / nb; /* rows of a launch */
+    for (int64_t r0 = 0; r0 < rows; r0 += at_once) {
+        const int n = rows - r0 < at_once ? (int)(rows - r0) : at_once, grid = (int)(((int64_t)n * nb + 15) / 16);
+        const uint8_t *xr = reinterpret_cast<const uint8_t *>(x) + r0 * x_stride * (x_bf16 ? 2 : 4);
+        if (vec)
+            k_ops_quantize<true><<<grid, 256, 0, (cudaStream_t)stream>>>(n, cols, nb, xr, x_bf16, x_stride, q + r0 * q_stride,
+                                                                       q_stride, scales + r0 * scales_stride, scales_stride);
+        else
+            k_ops_quantize<false><<<grid, 256, 0, (cudaStream_t)stream>>>(n, cols, nb, xr, x_bf16, x_stride, q + r0 * q_stride,
+                                                                        q_stride, scales + r0 * scales_stride, scales_stride);
+    }
     return (int)cudaGetLastError();
 }
 

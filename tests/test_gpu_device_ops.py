@@ -154,6 +154,20 @@ def test_route_near_ties(ops, score, n_group):
     check_route(ops, x.bfloat16(), 8, score=score, bias=torch.zeros(128, device="cuda"), n_group=n_group, topk_group=(n_group + 1) // 2)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("n_group", [1, 4])
+def test_route_infinite_and_huge_bias(ops, score, n_group):
+    g = gen(9)
+    x = randn(g, 40, 64)
+    x[torch.rand(40, 64, generator=g, device="cuda") < 0.2] = float("-inf")
+    kw = dict(score=score, n_group=n_group, topk_group=min(2, n_group), group_best=2)
+    for where, what in (([3, 9, 40], float("inf")), ([3, 9, 40], 1e30), (list(range(0, 64, 2)), 1e6), (list(range(64)), -1e6),
+                        (list(range(1, 64)), float("-inf"))):
+        b = 0.1 * randn(g, 64)
+        b[where] = what
+        check_route(ops, x, 6, bias=b, **kw)
+
+
 def test_route_strided_rows_and_many_tokens(ops):
     g = gen(8)
     wide = randn(g, 300, 203)
@@ -486,6 +500,8 @@ def test_experts_odd_ids(ops, T):
         within(out, want, tol)
         if not shared:
             assert (out[0] == 0).all()
+    none = ops.f8_experts(xq, xs, torch.full_like(ids, -1), w, *[t[:6].contiguous() for t in (gu, gus, dn, dns)])
+    assert (none == 0).all()
     ids.fill_(4)
     within(ops.f8_experts(xq, xs, ids, w, gu, gus, dn, dns, shared=True), *experts64(xq, xs, ids, w, gu, gus, dn, dns, True))
     ids.fill_(-1)
