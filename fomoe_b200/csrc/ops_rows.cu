@@ -161,7 +161,8 @@ __device__ __forceinline__ float rt_sigmoid(float x) { /* (x = -inf: 0) */
     return x >= 0.0f ? q : e * q;
 }
 
-template <int NPL>
+/* NPL: experts of a lane; LOW: as many as every lane has for certain (the size before in RT_SIZES) */
+template <int NPL, int LOW>
 __global__ void __launch_bounds__(32 * RT_WARPS) k_ops_route(const __grid_constant__ ops_route_t A) {
     __shared__ double s_c[RT_WARPS][OPS_MAX_E];
     __shared__ uint2 s_best[RT_WARPS][32];
@@ -171,47 +172,52 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_ops_route(const __grid_consta
     const int E = A.cfg.n_experts, K = A.cfg.top_k, G = A.cfg.n_group;
     const bool shut = A.valid && A.valid[t] == 0, softmax = A.cfg.score == FOMOE_B200_SOFTMAX;
     float x[NPL];
+#define RT_AT(j) ((j) < LOW ? (j) * 32 + lane : min((j) * 32 + lane, E - 1)) /* an expert that is there */
     if (A.logits_bf16) { /* (all loads first) */
         const uint16_t *p = reinterpret_cast<const uint16_t *>(A.logits) + (int64_t)t * A.row_stride;
 #pragma unroll
-        for (int j = 0; j < NPL; j++) x[j] = __uint_as_float((uint32_t)__ldg(p + min(j * 32 + lane, E - 1)) << 16);
+        for (int j = 0; j < NPL; j++) x[j] = __uint_as_float((uint32_t)__ldg(p + RT_AT(j)) << 16);
     } else {
         const float *p = reinterpret_cast<const float *>(A.logits) + (int64_t)t * A.row_stride;
 #pragma unroll
-        for (int j = 0; j < NPL; j++) x[j] = __ldg(p + min(j * 32 + lane, E - 1));
+        for (int j = 0; j < NPL; j++) x[j] = __ldg(p + RT_AT(j));
     }
+    /* closed experts: -inf.  (fmaxf takes a NaN to -inf, fminf +inf to FLT_MAX) */
     float mx = -INFINITY, inv = 1.0f;
 #pragma unroll
     for (int j = 0; j < NPL; j++) {
-        x[j] = j * 32 + lane < E && !shut && x[j] > -INFINITY ? fminf(x[j], FLT_MAX) : -INFINITY;
+        x[j] = fminf(fmaxf(x[j], -INFINITY), FLT_MAX);
+        if (j >= LOW && j * 32 + lane >= E) x[j] = -INFINITY;
+        if (shut) x[j] = -INFINITY;
         mx = fmaxf(mx, x[j]);
     }
-    uint32_t key[NPL]; /* the choice, or without a bias the logit itself */
-    const bool need_p = A.bias || G > 1;
     if (softmax) {
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, s));
         float sum = 0.0f;
+        const float m0 = mx > -INFINITY ? mx : 0.0f;
 #pragma unroll
-        for (int j = 0; j < NPL; j++) sum += x[j] > -INFINITY ? __expf(x[j] - mx) : 0.0f;
+        for (int j = 0; j < NPL; j++) sum += __expf(x[j] - m0);
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(FULL, sum, s);
         inv = sum > 0.0f ? __fdiv_rn(1.0f, sum) : 0.0f;
     }
-    if (need_p) {
+    /* what decides the order: the choice, or without a bias the logit itself; -inf where closed */
+    float v[NPL];
+    if (A.bias || G > 1) {
+        const float m0 = mx > -INFINITY ? mx : 0.0f;
 #pragma unroll
         for (int j = 0; j < NPL; j++) {
             const int e = j * 32 + lane;
-            const bool open = x[j] > -INFINITY;
-            float c = softmax ? __expf(x[j] - mx) * inv : rt_sigmoid(x[j]);
-            if (A.bias) c += __ldg(A.bias + min(e, E - 1));
-            c = open && c > -INFINITY ? c : -INFINITY;
-            key[j] = A.bias ? (c > -INFINITY ? rt_key(c) : 0u) : (open ? rt_key(x[j]) : 0u);
+            float c = softmax ? __expf(x[j] - m0) * inv : rt_sigmoid(x[j]);
+            if (A.bias) c += __ldg(A.bias + RT_AT(j));
+            c = x[j] > -INFINITY && c > -INFINITY ? c : -INFINITY;
+            v[j] = A.bias ? c : x[j];
             if (G > 1 && e < E) reinterpret_cast<float *>(s_c[warp])[e] = c;
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < NPL; j++) key[j] = x[j] > -INFINITY ? rt_key(x[j]) : 0u;
+        for (int j = 0; j < NPL; j++) v[j] = x[j];
     }
     const int per = E / G;
     uint32_t keep = 0xffffffffu;
@@ -234,34 +240,34 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_ops_route(const __grid_consta
 #pragma unroll
         for (int j = 0; j < NPL; j++) {
             const int e = j * 32 + lane;
-            if (e < E && !((keep >> (e / per)) & 1u)) key[j] = 0;
+            if (e < E && !((keep >> (e / per)) & 1u)) v[j] = -INFINITY;
         }
     }
-    uint32_t best = 0;
+    float most = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < NPL; j++) best = max(best, key[j]);
-    uint32_t bound = 1;
+    for (int j = 0; j < NPL; j++) most = fmaxf(most, v[j]);
+    uint32_t best = most > -INFINITY ? rt_key(most) : 0u;
+    float bound = -FLT_MAX; /* (all that is open; a value below it would be an infinite bias) */
     for (int r = 0; r <= K; r++) { /* (equal ones of several lanes go together: the bound is only lower for it) */
         const uint32_t w = __reduce_max_sync(FULL, best);
-        if (w == 0) {
-            bound = 1;
-            break;
-        }
-        bound = w;
+        bound = w == 0 ? -FLT_MAX : rt_val(w);
+        if (w == 0) break;
         best = best == w ? 0u : best;
     }
-    if (A.bias && bound > 1) { /* and those that may be as good for all fp32 can say */
-        const float v = rt_val(bound), low = v - RT_NEAR(v, v);
-        bound = low > -INFINITY ? rt_key(low) : 1u; /* (infinite choices: all that is open) */
+    if (A.bias) { /* and those that may be as good for all fp32 can say */
+        const float low = bound - RT_NEAR(bound, bound);
+        bound = low >= -FLT_MAX ? low : -FLT_MAX; /* (infinite choices: all that is open) */
     }
     int n = 0;
 #pragma unroll
     for (int j = 0; j < NPL; j++) {
-        const bool in = key[j] >= bound;
+        const bool in = v[j] >= bound;
         const uint32_t m = __ballot_sync(FULL, in);
-        const int at = n + __popc(m & ((1u << lane) - 1u));
-        if (in && at < 32) s_best[warp][at] = make_uint2(key[j], (uint32_t)(j * 32 + lane));
-        n += __popc(m);
+        if (m) { /* (most have none) */
+            const int at = n + __popc(m & ((1u << lane) - 1u));
+            if (in && at < 32) s_best[warp][at] = make_uint2(rt_key(v[j]), (uint32_t)(j * 32 + lane));
+            n += __popc(m);
+        }
     }
     __syncwarp();
     int slot = lane, id = -1; /* this lane writes slot `slot`, if there is one */
@@ -302,7 +308,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_ops_route(const __grid_consta
         uint32_t *c = reinterpret_cast<uint32_t *>(s_c[warp]);
 #pragma unroll
         for (int j = 0; j < NPL; j++)
-            if (j * 32 + lane < E) c[j * 32 + lane] = key[j];
+            if (j * 32 + lane < E) c[j * 32 + lane] = v[j] > -INFINITY ? rt_key(v[j]) : 0u;
         __syncwarp();
         id = rt_top<uint32_t>(c, 0u, E, K, keep, per);
     } else {
@@ -330,13 +336,13 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_ops_route(const __grid_consta
     }
 }
 
-#define RT_SIZES(X) X(1) X(2) X(4) X(6) X(8) X(12) X(16) /* experts of a lane */
+#define RT_SIZES(X) X(1, 0) X(2, 1) X(4, 2) X(6, 4) X(8, 6) X(12, 8) X(16, 12) /* experts of a lane, at most and at least */
 
 extern "C" int ops_launch_route(const ops_route_t *a, void *stream) {
     const int grid = (a->n_tokens + RT_WARPS - 1) / RT_WARPS, E = a->cfg.n_experts;
-#define RT_GO(N)                                                                \
+#define RT_GO(N, LOW)                                                           \
     if (E <= 32 * N) {                                                          \
-        k_ops_route<N><<<grid, 32 * RT_WARPS, 0, (cudaStream_t)stream>>>(*a); \
+        k_ops_route<N, LOW><<<grid, 32 * RT_WARPS, 0, (cudaStream_t)stream>>>(*a); \
         return (int)cudaGetLastError();                                         \
     }
     RT_SIZES(RT_GO)
@@ -616,7 +622,7 @@ extern "C" int ops_rows_init(void) {
     cudaFuncAttributes f;
     int rc = 0;
 #define RK(k) rc |= (int)cudaFuncGetAttributes(&f, (k))
-#define RT_RK(N) RK(k_ops_route<N>);
+#define RT_RK(N, LOW) RK((k_ops_route<N, LOW>));
     RT_SIZES(RT_RK)
 #undef RT_RK
 #define NM_RK(G, IT) RK((k_ops_norm<true, G, IT>)); RK((k_ops_norm<false, G, IT>));

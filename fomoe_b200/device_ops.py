@@ -162,26 +162,26 @@ class DeviceOps:
                     raise ValueError(f"gate: [T, n], [1, n] or [T, 1] is wanted, got {(gT, gn)}")
                 ga, gs, gp = gate.data_ptr(), gs if gT > 1 else 0, 1 if gn == n and n > 1 else 0
             if not inplace:
-                x_out = x.new_empty((T, n))
+                x_out = t.empty_like(x)
             xo, xos = x_out.data_ptr(), x_out.stride(0)
         elif post is not None or gate is not None:
             raise ValueError("post and gate need a block")
         h = sc = pr = hp = sp = None
-        ht = nb = 0
+        ht = nb = hs = 0
         if pre is not None:
             pr = self._flat(pre, "pre", self._f32, (n,))
             if out == "f8":
                 ht, nb = F8, (n + 127) // 128
-                h, sc = x.new_empty((T, n), dtype=t.float8_e4m3fn), x.new_empty((T, nb), dtype=t.float32)
+                h, sc = t.empty_like(x, dtype=t.float8_e4m3fn), x.new_empty((T, nb), dtype=t.float32)
                 sp = sc.data_ptr()
             elif out in self._out:
                 dt, ht = self._out[out]
-                h = x.new_empty((T, n), dtype=dt)
+                h = t.empty_like(x, dtype=dt)
             else:
                 raise ValueError(f"out: 'f32', 'bf16' or 'f8' is wanted, got {out!r}")
-            hp = h.data_ptr()
+            hp, hs = h.data_ptr(), h.stride(0)
         a = NormArgs(T, n, eps, offset, scale, x.data_ptr(), fl[x.dtype], xs, blk, bt, bs, po, ga, gs, gp, xo, xos, pr, hp, ht,
-                     n, sp, nb)
+                     hs, sp, nb)
         self._ck(self._l.fomoe_b200_ops_norm(self._h, a, self._stream()), "norm")
         return (x_out, h, sc) if out == "f8" else (x_out, h)
 
@@ -191,8 +191,8 @@ class DeviceOps:
         stride = self._rows(x, "x", self._float)
         T, n = x.shape
         nb = (n + 127) // 128
-        q, sc = x.new_empty((T, n), dtype=t.float8_e4m3fn), x.new_empty((T, nb), dtype=t.float32)
-        self._ck(self._l.fomoe_b200_ops_f8_quantize(self._h, T, n, x.data_ptr(), self._float[x.dtype], stride, q.data_ptr(), n,
+        q, sc = t.empty_like(x, dtype=t.float8_e4m3fn), x.new_empty((T, nb), dtype=t.float32)
+        self._ck(self._l.fomoe_b200_ops_f8_quantize(self._h, T, n, x.data_ptr(), self._float[x.dtype], stride, q.data_ptr(), q.stride(0),
                                                     sc.data_ptr(), nb, self._stream()), "f8_quantize")
         return q, sc
 
