@@ -19,6 +19,30 @@
 #define FULL 0xffffffffu
 #endif
 
+/* ------------------------------------------------------------------ kernels of one call, one after the other
+ * Launched with the programmatic-serialization attribute a kernel may start while the one before it in the stream ends:
+ * what it does before f8_after() overlaps that end and must not touch anything the kernel before it writes; f8_after()
+ * returns when that kernel has completed and its writes are visible.  f8_next() in the kernel before lets the next one start
+ * that early (else it starts as the blocks exit). */
+__device__ __forceinline__ void f8_after() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void f8_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... P, typename... A>
+static int f8_launch_after(void (*k)(P...), dim3 grid, int threads, int smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t c = {};
+    cudaLaunchAttribute at[1];
+    c.gridDim = grid;
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = at;
+    c.numAttrs = 1;
+    const cudaError_t rc = cudaLaunchKernelEx(&c, k, args...);
+    return (int)(rc != cudaSuccess ? rc : cudaGetLastError());
+}
+
 /* ------------------------------------------------------------------ bucket: the pairs of every expert, in pair order
  * Block b owns a run of pairs, warp w a run of the block's.  A first walk counts each warp's pairs of every expert, prefixes
  * over (expert, block, warp) give every warp its first place, a second walk places the pairs.  The order inside an expert is
@@ -38,7 +62,9 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
     extern __shared__ int s_cnt[]; /* [n_experts][BK_WARPS], then [n_experts]: the block's first place */
     __shared__ int s_tot[BK_WARPS], s_til[BK_WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    f8_next();
     for (int i = tid; i < n_experts * BK_WARPS; i += BK_THREADS) s_cnt[i] = 0;
+    if (!COUNT) f8_after();
     __syncthreads();
     const int run = ((block_run + BK_THREADS - 1) / BK_THREADS) * 32; /* pairs of a warp */
     const int q1 = min(n_routed, ((int)blockIdx.x + 1) * block_run);
@@ -416,11 +442,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int per_n = MODE == F8_GATE_UP ? NT / 2 : NT;
     const int n_tiles = (P.n + per_n - 1) / per_n;
+    if (MODE != F8_DENSE) f8_next();
     /* this block's blocks of k: all, or (SPLIT) its rank's share; the cluster's blocks have one tile */
     const uint32_t ranks = SPLIT ? f8_cluster_size() : 1, rank = SPLIT ? f8_cluster_rank() : 0;
     const int kb_all = (P.k + 127) / 128, kb_lo = (int)(rank * kb_all / ranks), kbs = (int)((rank + 1) * kb_all / ranks) - kb_lo;
     const int first = (int)(blockIdx.x / ranks), stride = (int)(gridDim.x / ranks);
-    const int tiles = (MODE == F8_DENSE ? (P.m + 127) / 128 : P.counts[0]) * n_tiles;
+    int tiles = MODE == F8_DENSE ? (P.m + 127) / 128 * n_tiles : 0;
 
     if (tid == 0) {
         for (int s = 0; s < STAGES; s++) {
@@ -448,6 +475,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = C->tmem_base;
+    if (MODE != F8_DENSE) f8_after();
+    if (MODE != F8_DENSE) tiles = P.counts[0] * n_tiles;
 
     if (warp >= F8_EPI_WARPS) {
         /* 384 x 168 registers at launch = 128 x 72 + 256 x 216 */
@@ -779,30 +808,6 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
     __syncthreads();
     if (warp == 9)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(NB * NT)) : "memory");
-}
-
-/* ------------------------------------------------------------------ kernels of one call, one after the other
- * Launched with the programmatic-serialization attribute a kernel may start while the one before it in the stream ends:
- * what it does before f8_after() overlaps that end and must not touch anything the kernel before it writes; f8_after()
- * returns when that kernel has completed and its writes are visible.  f8_next() in the kernel before lets the next one start
- * that early (else it starts as the blocks exit). */
-__device__ __forceinline__ void f8_after() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void f8_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
-template <typename... P, typename... A>
-static int f8_launch_after(void (*k)(P...), dim3 grid, int threads, int smem, cudaStream_t st, A... args) {
-    cudaLaunchConfig_t c = {};
-    cudaLaunchAttribute at[1];
-    c.gridDim = grid;
-    c.blockDim = dim3(threads);
-    c.dynamicSmemBytes = smem;
-    c.stream = st;
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    c.attrs = at;
-    c.numAttrs = 1;
-    const cudaError_t rc = cudaLaunchKernelEx(&c, k, args...);
-    return (int)(rc != cudaSuccess ? rc : cudaGetLastError());
 }
 
 /* ------------------------------------------------------------------ few rows: the weights' bytes are all that counts
@@ -1157,16 +1162,21 @@ static int f8_map(CUtensorMap *m, const void *p, uint64_t k, uint64_t rows, uint
 template <int MODE, int NT, bool SPLIT>
 static int f8_launch(f8_args_t &p, int64_t most_tiles, int ranks, int n_sm, int *launches, cudaStream_t st) {
     cudaLaunchConfig_t c = {};
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[1] = {};
     c.gridDim = dim3((unsigned)(SPLIT ? most_tiles * ranks : most_tiles < n_sm ? most_tiles : n_sm));
     c.blockDim = dim3(F8_THREADS);
     c.dynamicSmemBytes = f8_cfg<MODE, NT>::SMEM;
     c.stream = st;
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ranks;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    if (SPLIT) {
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = ranks;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    } else if (MODE != F8_DENSE) {
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+    }
     c.attrs = at;
-    c.numAttrs = SPLIT ? 1 : 0;
+    c.numAttrs = SPLIT || MODE != F8_DENSE ? 1 : 0;
     *launches += 1;
     const cudaError_t rc = cudaLaunchKernelEx(&c, k_f8_mma<MODE, NT, SPLIT>, p);
     return (int)(rc != cudaSuccess ? rc : cudaGetLastError());
@@ -1225,6 +1235,8 @@ __global__ void __launch_bounds__(256) k_ops_permute(const uint8_t *x, int64_t x
                                                      const int *counts, const int *pairs, int n_routed, int top_k, int n_shared,
                                                      uint8_t *xp, float *xps) {
     const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    f8_next();
+    f8_after();
     if (r >= counts[1] + n_shared) return;
     const int p = pairs[r], t = p < n_routed ? p / top_k : p - n_routed;
     const uint4 *src = reinterpret_cast<const uint4 *>(x + t * x_stride);
@@ -1239,6 +1251,7 @@ __global__ void __launch_bounds__(256) k_ops_combine(const __half *dots, const f
                                                     const float *weights, int n_embd, int n_experts, int top_k, int n_routed,
                                                     int has_shared, __nv_bfloat16 *out, int64_t out_stride, int vec) {
     const int t = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 8;
+    f8_after();
     if (c >= n_embd) return;
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     for (int j = 0; j < top_k + has_shared; j++) {
@@ -1341,18 +1354,26 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     int run = (n_routed + BK_BLOCKS - 1) / BK_BLOCKS;
     run = run < BK_RUN ? BK_RUN : run;
     const int nb = (n_routed + run - 1) / run, bk_smem = a->n_experts * (BK_WARPS + 1) * 4;
+    const int *ids = a->ids;
     if (nb > 1) {
-        k_ops_bucket<true><<<nb, BK_THREADS, bk_smem, st>>>(a->ids, n_routed, run, a->n_tokens, a->n_experts, a->has_shared,
-                                                          block_counts, counts, pairs, pos, items, status);
+        k_ops_bucket<true><<<nb, BK_THREADS, bk_smem, st>>>(ids, n_routed, run, a->n_tokens, a->n_experts, a->has_shared, block_counts,
+                                                          counts, pairs, pos, items, status);
+        rc = (int)cudaGetLastError();
+        if (!rc)
+            rc = f8_launch_after(k_ops_bucket<false>, dim3(nb), BK_THREADS, bk_smem, st, ids, n_routed, run, a->n_tokens, a->n_experts,
+                                 a->has_shared, block_counts, counts, pairs, pos, items, status);
         *launches += 1;
+    } else {
+        k_ops_bucket<false><<<nb, BK_THREADS, bk_smem, st>>>(ids, n_routed, run, a->n_tokens, a->n_experts, a->has_shared, block_counts,
+                                                           counts, pairs, pos, items, status);
+        rc = (int)cudaGetLastError();
     }
-    k_ops_bucket<false><<<nb, BK_THREADS, bk_smem, st>>>(a->ids, n_routed, run, a->n_tokens, a->n_experts, a->has_shared,
-                                                       block_counts, counts, pairs, pos, items, status);
-    k_ops_permute<<<(w.n_pairs + 7) / 8, 256, 0, st>>>(a->x, a->x_stride, a->x_scales, a->x_scales_stride, H, counts, pairs,
-                                                      n_routed, a->top_k, n_shared, ws + w.xp, (float *)(ws + w.xp_scales));
+    if (!rc)
+        rc = f8_launch_after(k_ops_permute, dim3((w.n_pairs + 7) / 8), 256, 0, st, a->x, a->x_stride, a->x_scales, a->x_scales_stride, H,
+                             (const int *)counts, (const int *)pairs, n_routed, a->top_k, n_shared, ws + w.xp, (float *)(ws + w.xp_scales));
     *launches += 2;
-    rc = (int)cudaGetLastError();
-    /* no more tiles than this (the device knows how many there are) */
+    /* no more tiles than this (the device knows how many there are).  Tiles of 32 rows, with more weights in flight and a
+     * joining warp of each warpgroup, were tried for few pairs an expert: 61 tokens of 8 in 256 experts 155 us as with 128. */
     const int64_t tiles = w.n_pairs / 128 + recs;
     if (!rc) rc = f8_launch<F8_GATE_UP, 256, false>(gu, tiles * (I / 128), 1, n_sm, launches, st);
     if (!rc) rc = f8_launch<F8_DOWN, 256, false>(dn, tiles * ((H + 255) / 256), 1, n_sm, launches, st);
@@ -1361,12 +1382,13 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     /* (the grid's y goes to 65535) */
     for (int t0 = 0; t0 < a->n_tokens; t0 += 65535) {
         const int nt = a->n_tokens - t0 < 65535 ? a->n_tokens - t0 : 65535, p0 = t0 * a->top_k;
-        k_ops_combine<<<dim3((H / 8 + 255) / 256, nt), 256, 0, st>>>(
-            (const __half *)(ws + w.dots), (const float *)(ws + w.dot_scales), pos + p0, a->ids + p0, a->weights + p0, H, a->n_experts,
-            a->top_k, n_routed + t0 - p0, a->has_shared, (__nv_bfloat16 *)a->out + t0 * a->out_stride, a->out_stride, vec);
+        rc = f8_launch_after(k_ops_combine, dim3((H / 8 + 255) / 256, nt), 256, 0, st, (const __half *)(ws + w.dots),
+                             (const float *)(ws + w.dot_scales), (const int *)pos + p0, ids + p0, a->weights + p0, H, a->n_experts,
+                             a->top_k, n_routed + t0 - p0, a->has_shared, (__nv_bfloat16 *)a->out + t0 * a->out_stride, a->out_stride, vec);
+        if (rc) return rc;
         *launches += 1;
     }
-    return (int)cudaGetLastError();
+    return 0;
 }
 
 extern "C" int ops_f8_init(ops_device_t *d) {

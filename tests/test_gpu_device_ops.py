@@ -471,7 +471,8 @@ def make_experts(seed, T, H, I, E, k, shared, dropped=0.0, skew=0.7):
 EXPERTS = [(1, 128, 128, 1, 1, False, 0.0), (1, 256, 128, 4, 2, True, 0.0), (1, 1024, 512, 32, 10, True, 0.0), (2, 512, 256, 16, 8, False, 0.3),
            (3, 640, 384, 7, 7, True, 0.2), (5, 256, 128, 512, 16, False, 0.0), (13, 384, 640, 9, 3, True, 0.1), (33, 512, 256, 3, 2, False, 0.0),
            (64, 256, 256, 64, 8, True, 0.2), (129, 512, 128, 5, 1, False, 0.0), (257, 384, 384, 4, 3, True, 0.4), (700, 256, 256, 10, 6, False, 0.1),
-           (1500, 256, 128, 33, 4, True, 0.0), (2000, 128, 128, 70, 7, True, 0.1)]
+           (1500, 256, 128, 33, 4, True, 0.0), (2000, 128, 128, 70, 7, True, 0.1),
+           (300, 384, 256, 200, 4, True, 0.1), (600, 256, 384, 400, 3, False, 0.3), (90, 128, 1024, 64, 4, True, 0.0)]
 
 
 @pytest.mark.parametrize("T,H,I,E,k,shared,dropped", EXPERTS)
