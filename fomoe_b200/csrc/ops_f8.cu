@@ -389,25 +389,27 @@ __device__ __forceinline__ void f8_stage(uint32_t buf, const uint32_t *w) {
                      : "memory");
 }
 
-/* the staged box to global memory: all of it by TMA, or the first `rows` rows by the warp.  row0: where the first row's
- * 128 bytes go, stride: bytes from row to row, left: bytes of a row that are inside out, elem: bytes of a value */
-__device__ __forceinline__ void f8_box_out(uint32_t buf, const CUtensorMap *map, int x, int y, bool tma, uint8_t *row0,
-                                           int64_t stride, int rows, int left, int elem) {
-    const int lane = threadIdx.x & 31;
-    if (tma) {
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (f8_elect()) {
-            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x),
-                         "r"(y), "r"(buf)
-                         : "memory");
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        }
-        __syncwarp();
-        return;
+/* staged boxes are about to be read by the copy engine */
+__device__ __forceinline__ void f8_staged() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+}
+
+/* a staged box to global memory, whole */
+__device__ __forceinline__ void f8_box_out(uint32_t buf, const CUtensorMap *map, int x, int y) {
+    if (f8_elect()) {
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+                     "r"(buf)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
     __syncwarp();
-    const int per = 128 / elem;
+}
+
+/* the first `rows` rows of a staged box, by the warp.  row0: where the first row's 128 bytes go, stride: bytes from row to
+ * row, left: bytes of a row that are inside out, elem: bytes of a value */
+__device__ __forceinline__ void f8_rows_out(uint32_t buf, uint8_t *row0, int64_t stride, int rows, int left, int elem) {
+    const int lane = threadIdx.x & 31, per = 128 / elem;
     for (int i = lane; i < rows * per; i += 32) {
         const int r = i / per, c = i - r * per;
         if (c * elem >= left) continue;
@@ -707,11 +709,20 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     if constexpr (MODE == F8_DOWN) {
                         /* fp16 relative to a power of two above the row's 128 values: 2^-12 of the largest, a sixteenth of the
                          * rounding to bf16 that the sum over the experts ends with, at half of fp32's bytes both ways */
-                        float top = 0.0f;
+                        float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                         for (int i = 0; i < W / 2; i++) {
-                            const float x = fabsf(acc[i].x), y = fabsf(acc[i].y);
-                            top = fmaxf(top, fmaxf(x < INFINITY ? x : 0.0f, y < INFINITY ? y : 0.0f));
+                            m[(2 * i) & 3] = fmaxf(m[(2 * i) & 3], fabsf(acc[i].x));
+                            m[(2 * i + 1) & 3] = fmaxf(m[(2 * i + 1) & 3], fabsf(acc[i].y));
+                        }
+                        float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])); /* (NaN left out) */
+                        if (top == INFINITY) { /* the largest of the finite ones */
+                            top = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < W / 2; i++) {
+                                top = fabsf(acc[i].x) < INFINITY ? fmaxf(top, fabsf(acc[i].x)) : top;
+                                top = fabsf(acc[i].y) < INFINITY ? fmaxf(top, fabsf(acc[i].y)) : top;
+                            }
                         }
                         const uint32_t e = min((__float_as_uint(top) >> 23) + 1u, 253u);
                         const float down = __uint_as_float((254u - e) << 23);
@@ -731,13 +742,16 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     }
                     f8_box_wait();
 #pragma unroll
-                    for (int c = 0; c < W / 64; c++) { /* boxes of 64 columns */
+                    for (int c = 0; c < W / 64; c++) f8_stage(buf + c * 4096u, w + 32 * c); /* boxes of 64 columns */
+                    f8_staged();
+#pragma unroll
+                    for (int c = 0; c < W / 64; c++) {
                         const int x = c0 + 64 * c;
-                        f8_stage(buf + c * 4096u, w + 32 * c);
-                        if (x < P.n)
-                            f8_box_out(buf + c * 4096u, &P.to, 2 * x, t.r0 + w0, tma,
-                                       reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + w0) * P.out_stride + x),
-                                       2 * P.out_stride, rows, 2 * (P.n - x), 2);
+                        if (x >= P.n) continue;
+                        if (tma) f8_box_out(buf + c * 4096u, &P.to, 2 * x, t.r0 + w0);
+                        else
+                            f8_rows_out(buf + c * 4096u, reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + w0) * P.out_stride + x),
+                                        2 * P.out_stride, rows, 2 * (P.n - x), 2);
                     }
                 } else {
 #pragma unroll
@@ -745,10 +759,13 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                         const int x = c0 + 32 * c;
                         if (c % cfg::BUFS == 0) f8_box_wait();
                         f8_stage(buf + c % cfg::BUFS * 4096u, reinterpret_cast<const uint32_t *>(acc) + 32 * c);
-                        if (x < P.n)
-                            f8_box_out(buf + c % cfg::BUFS * 4096u, &P.to, 4 * x, t.r0 + w0, tma,
-                                       reinterpret_cast<uint8_t *>(P.out) + 4 * ((int64_t)(t.r0 + w0) * P.out_stride + x),
-                                       4 * P.out_stride, rows, 4 * (P.n - x), 4);
+                        f8_staged();
+                        if (x >= P.n) continue;
+                        if (tma) f8_box_out(buf + c % cfg::BUFS * 4096u, &P.to, 4 * x, t.r0 + w0);
+                        else
+                            f8_rows_out(buf + c % cfg::BUFS * 4096u,
+                                        reinterpret_cast<uint8_t *>(P.out) + 4 * ((int64_t)(t.r0 + w0) * P.out_stride + x),
+                                        4 * P.out_stride, rows, 4 * (P.n - x), 4);
                     }
                 }
             }
