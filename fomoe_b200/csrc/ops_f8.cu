@@ -427,6 +427,13 @@ __device__ __forceinline__ void f8_rows_out(uint32_t buf, uint8_t *row0, int64_t
     __syncwarp();
 }
 
+/* 32 bytes of a row (a whole sector) */
+__device__ __forceinline__ void f8_st32(void *p, const uint32_t *w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
 /* the warp's boxes have left its staging buffers */
 __device__ __forceinline__ void f8_box_wait() {
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -619,7 +626,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             grp++;                                                                                   \
         }                                                                                            \
     } while (0)
-            float n0, n1 = 0.0f;
+            float n0, n1 = 0.0f, fsum = 0.0f;
             F8_FACTORS(0);
             /* Chunks of 32 columns through two register buffers: while one is joined the next is on its way, also across
              * blocks.  (gate/up: the first half of a thread's columns are the gate's, the second the up's) */
@@ -635,6 +642,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             for (int kb = 0; kb < kbs; kb++, step++) {
                 const int b = step % NB;
                 const float f0 = n0, f1 = MODE == F8_GATE_UP ? n1 : n0;
+                if (MODE == F8_DOWN) fsum += fabsf(f0);
                 if (!ok) continue;
 #pragma unroll
                 for (int c = 0; c < CH; c++) {
@@ -707,24 +715,13 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                 uint32_t w[W / 2];
                 if (MODE == F8_DOWN || P.out_bf16) {
                     if constexpr (MODE == F8_DOWN) {
-                        /* fp16 relative to a power of two above the row's 128 values: 2^-12 of the largest, a sixteenth of the
-                         * rounding to bf16 that the sum over the experts ends with, at half of fp32's bytes both ways */
-                        float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int i = 0; i < W / 2; i++) {
-                            m[(2 * i) & 3] = fmaxf(m[(2 * i) & 3], fabsf(acc[i].x));
-                            m[(2 * i + 1) & 3] = fmaxf(m[(2 * i + 1) & 3], fabsf(acc[i].y));
-                        }
-                        float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])); /* (NaN left out) */
-                        if (top == INFINITY) { /* the largest of the finite ones */
-                            top = 0.0f;
-#pragma unroll
-                            for (int i = 0; i < W / 2; i++) {
-                                top = fabsf(acc[i].x) < INFINITY ? fmaxf(top, fabsf(acc[i].x)) : top;
-                                top = fabsf(acc[i].y) < INFINITY ? fmaxf(top, fabsf(acc[i].y)) : top;
-                            }
-                        }
-                        const uint32_t e = min((__float_as_uint(top) >> 23) + 1u, 253u);
+                        /* fp16 relative to a power of two: 2^-11 of a value, a sixteenth of the rounding to bf16 that the sum
+                         * over the experts ends with, at half of fp32's bytes both ways.  No sum of products passes
+                         * sum |sa sb| 128 448^2 = top: with that below 2^15 nothing overflows, and only values under 2^-28 of
+                         * top have fewer bits (steps of 2^-38 top).  (Looking for the row's largest value instead cost 600 of
+                         * 11,000 cycles a tile.) */
+                        const float top = fsum * (128.0f * 448.0f * 448.0f);
+                        const uint32_t e = min(max(__float_as_uint(top) >> 23, 15u) - 14u, 253u);
                         const float down = __uint_as_float((254u - e) << 23);
 #pragma unroll
                         for (int i = 0; i < W / 2; i++) {
@@ -739,6 +736,14 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                             const __nv_bfloat162 v = __floats2bfloat162_rn(acc[i].x, acc[i].y);
                             w[i] = *reinterpret_cast<const uint32_t *>(&v);
                         }
+                    }
+                    if (MODE == F8_DOWN && !tma) { /* (61 tokens of 8 in 256 experts: 150 us by staged rows, 133 so) */
+                        if (lane < rows && c0 < P.n) {
+                            uint8_t *o = reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + row) * P.out_stride + c0);
+#pragma unroll
+                            for (int i = 0; i < W / 16; i++) f8_st32(o + 32 * i, w + 8 * i);
+                        }
+                        continue;
                     }
                     f8_box_wait();
 #pragma unroll
