@@ -579,8 +579,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
 #pragma unroll
                     for (int q = 0; q < F8_SC; q++) {
                         const int k = kb_lo + min(kb + q, kbs - 1);
-                        va[0][q] = __ldg(a0 + k);
-                        va[1][q] = __ldg(a1 + k);
+                        va[0][q] = __ldcg(a0 + k); /* (the kernel before this one may have written them as this one started) */
+                        va[1][q] = __ldcg(a1 + k);
                         vb[0][q] = __ldg(b0 + k);
                         vb[1][q] = __ldg(b1 + k);
                     }
