@@ -4,6 +4,7 @@
  */
 #pragma once
 #include <cuda_fp8.h>
+#include <math.h>
 #include <stdint.h>
 
 /* |b| joins the running amax; a NaN stays (max.NaN), so a block that holds one gets a NaN scale */
@@ -13,7 +14,6 @@ __device__ __forceinline__ float ops_amax(float a, float b) {
     return r;
 }
 
-__device__ __forceinline__ float ops_f8_scale(float amax) { return __fdiv_rn(ops_amax(amax, 0x1p-100f), 448.0f); }
 
 /* x / scale rounded to nearest, from inv = 1 / scale rounded to nearest: a quotient that is off by a step at most, its exact
  * remainder, and one correction (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
@@ -22,6 +22,12 @@ __device__ __forceinline__ float ops_f8_scale(float amax) { return __fdiv_rn(ops
 __device__ __forceinline__ float ops_f8_quot(float x, float scale, float inv) {
     const float q = __fmul_rn(x, inv);
     return __fmaf_rn(__fmaf_rn(-q, scale, x), inv, q);
+}
+
+/* max(amax, 2^-100) / 448, rounded to nearest the same way (an infinite amax has no remainder: it stays) */
+__device__ __forceinline__ float ops_f8_scale(float amax) {
+    const float a = ops_amax(amax, 0x1p-100f), s = ops_f8_quot(a, 448.0f, 1.0f / 448.0f);
+    return a < INFINITY ? s : a;
 }
 
 /* four numbers as e4m3, the first in the low byte */

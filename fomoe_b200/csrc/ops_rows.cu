@@ -356,81 +356,127 @@ extern "C" int ops_launch_route(const ops_route_t *a, void *stream) {
  * reduction.  VEC: all pointers and strides allow 16-byte accesses and n is a multiple of 8; otherwise the same code
  * goes element by element. */
 #define NM_THREADS(G) ((G) == 32 ? 256 : (G))
-#define NM_AHEAD 148 /* rows: what a later block reads is asked into L2 (8192 x 4096: 83 us, without 89, 592 rows ahead 85) */
+#define NM_AHEAD 148 /* rows: what a later block reads is asked into L2 (8192 x 4096: 74 us, without 82, 296 rows ahead 74) */
+#define NM_BLOCKS 5  /* of 256 threads, an SM (8192 x 4096: 68 us, with 4 74, with 6 and spills 93) */
 #define NM_FEW 1184  /* rows: eight an SM */
 
-template <bool VEC>
-__device__ __forceinline__ void nm_load8(const void *p, int bf16, int64_t at, int left, float (&v)[8]) {
+/* Values go in pairs: one instruction (fma.rn.f32x2 and its like) rounds two of them as two would. */
+#define NM_PAIR(op, d, a, b)                                                                                     \
+    asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\n" op ".rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}" \
+        : "=f"((d).x), "=f"((d).y)                                                                               \
+        : "f"((a).x), "f"((a).y), "f"((b).x), "f"((b).y))
+
+__device__ __forceinline__ float2 nm_mul(float2 a, float2 b) {
+    float2 d;
+    NM_PAIR("mul", d, a, b);
+    return d;
+}
+__device__ __forceinline__ float2 nm_add(float2 a, float2 b) {
+    float2 d;
+    NM_PAIR("add", d, a, b);
+    return d;
+}
+__device__ __forceinline__ float2 nm_fma(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 nm_both(float v) { return make_float2(v, v); }
+
+/* Where a thread's runs of 8 columns lie.  One run: 16 threads share a block of 128; two, 64 columns apart: 8 threads, so that
+ * the block's scale is made once for 16 values.  A row's sums come in the same order whether its accesses are wide or not. */
+template <int IT>
+__device__ __forceinline__ int nm_col(int thread, int it) {
+    constexpr int S = IT == 2 ? 8 : 16; /* threads of a block */
+    return thread / S * 128 + it * 64 + thread % S * 8;
+}
+
+/* 8 columns from `at`, STEP apart; VEC: neighbours, 16-byte accesses */
+template <bool VEC, int STEP = 1>
+__device__ __forceinline__ void nm_load8(const void *p, int bf16, int64_t at, int left, float2 (&v)[4]) {
     if (VEC) {
         if (bf16) {
             const uint4 u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p) + at);
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
+            for (int i = 0; i < 4; i++) v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
         } else {
             const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + at);
             const float4 b = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + at + 4);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+            v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
         }
     } else {
+        float f[8];
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            v[i] = i >= left ? 0.0f
-                   : bf16    ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[at + i])
-                             : reinterpret_cast<const float *>(p)[at + i];
+            f[i] = STEP * i >= left ? 0.0f
+                   : bf16              ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[at + STEP * i])
+                                       : reinterpret_cast<const float *>(p)[at + STEP * i];
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = make_float2(f[2 * i], f[2 * i + 1]);
     }
 }
 
 template <bool VEC>
-__device__ __forceinline__ void nm_store8(void *p, int bf16, int64_t at, int left, const float (&v)[8]) {
+__device__ __forceinline__ void nm_store8(void *p, int bf16, int64_t at, int left, const float2 (&v)[4]) {
     if (VEC) {
         if (bf16) {
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                const __nv_bfloat162 b = __float22bfloat162_rn(v[i]);
                 w[i] = *reinterpret_cast<const uint32_t *>(&b);
             }
             *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(p) + at) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
-            *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + at) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + at + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + at) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+            *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + at + 4) = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++)
             if (i < left) {
-                if (bf16) reinterpret_cast<__nv_bfloat16 *>(p)[at + i] = __float2bfloat16_rn(v[i]);
-                else reinterpret_cast<float *>(p)[at + i] = v[i];
+                const float f = i & 1 ? v[i >> 1].y : v[i >> 1].x;
+                if (bf16) reinterpret_cast<__nv_bfloat16 *>(p)[at + i] = __float2bfloat16_rn(f);
+                else reinterpret_cast<float *>(p)[at + i] = f;
             }
     }
 }
 
-/* 8 values of one row as e4m3 at column c of q; the 16 threads of a 128-block call it together */
-template <bool VEC>
-__device__ __forceinline__ void nm_quant8(uint8_t *q, float *scales, int c, int n, const float (&v)[8]) {
+/* a thread's runs of one row as e4m3; the 16 / IT threads of a block of 128 call it together */
+template <bool VEC, int IT, int STEP = 1>
+__device__ __forceinline__ void nm_quant(uint8_t *q, float *scales, int c0, int n, const float2 (&v)[IT][4]) {
     float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) amax = ops_amax(amax, v[i]);
+    for (int it = 0; it < IT; it++)
 #pragma unroll
-    for (int s = 8; s > 0; s >>= 1) amax = ops_amax(amax, __shfl_xor_sync(FULL, amax, s));
+        for (int i = 0; i < 4; i++) amax = ops_amax(ops_amax(amax, v[it][i].x), v[it][i].y);
+    /* numbers without a sign are ordered as their bits are, with NaN above infinity */
+    const unsigned block = IT == 2 ? 0xffu << (threadIdx.x & 24) : 0xffffu << (threadIdx.x & 16);
+    amax = __uint_as_float(__reduce_max_sync(block, __float_as_uint(amax)));
     const float sc = ops_f8_scale(amax), inv = __frcp_rn(sc);
-    if (c < n) {
-        if ((c & 127) == 0) scales[c >> 7] = sc;
+    if ((c0 & 127) == 0 && c0 < n) scales[c0 >> 7] = sc;
+#pragma unroll
+    for (int it = 0; it < IT; it++) {
+        const int c = c0 + 64 * it;
+        if (c >= n) continue;
+        float2 r[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) { /* (ops_f8_quot) */
+            const float2 t = nm_mul(v[it][i], nm_both(inv));
+            r[i] = nm_fma(nm_fma(t, nm_both(-sc), v[it][i]), nm_both(inv), t);
+        }
         uint32_t w[2];
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-            w[h] = ops_f8_pack4(ops_f8_quot(v[4 * h], sc, inv), ops_f8_quot(v[4 * h + 1], sc, inv),
-                                ops_f8_quot(v[4 * h + 2], sc, inv), ops_f8_quot(v[4 * h + 3], sc, inv));
+        for (int h = 0; h < 2; h++) w[h] = ops_f8_pack4(r[2 * h].x, r[2 * h].y, r[2 * h + 1].x, r[2 * h + 1].y);
         if (VEC) {
             *reinterpret_cast<uint2 *>(q + c) = make_uint2(w[0], w[1]);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (c + i < n) q[c + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+                if (c + STEP * i < n) q[c + STEP * i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
         }
     }
 }
@@ -451,8 +497,19 @@ __device__ __forceinline__ float nm_row_sum(float v, float *s_red) {
     return t;
 }
 
+/* 1 / rms of the row */
+template <int G, int IT>
+__device__ __forceinline__ float nm_inv(const float2 (&v)[IT][4], int n, float eps, float *s_red) {
+    float2 ss = nm_both(0.0f);
+#pragma unroll
+    for (int it = 0; it < IT; it++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) ss = nm_fma(v[it][i], v[it][i], ss);
+    return __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(nm_row_sum<G>(ss.x + ss.y, s_red), (float)n) + eps));
+}
+
 template <bool VEC, int G, int IT>
-__global__ void __launch_bounds__(NM_THREADS(G)) k_ops_norm(fomoe_b200_norm_args_t A) {
+__global__ void __launch_bounds__(NM_THREADS(G), VEC && G == 256 ? NM_BLOCKS : 1) k_ops_norm(fomoe_b200_norm_args_t A) {
     __shared__ float s_red[NM_THREADS(G) / 32];
     const int gt = threadIdx.x % G;
     const int row = blockIdx.x * (NM_THREADS(G) / G) + threadIdx.x / G;
@@ -464,12 +521,12 @@ __global__ void __launch_bounds__(NM_THREADS(G)) k_ops_norm(fomoe_b200_norm_args
         fb_prefetch_l2(reinterpret_cast<const uint8_t *>(A.x) + r * A.x_stride * xb, (uint32_t)(n * xb));
         if (A.block) fb_prefetch_l2(reinterpret_cast<const uint8_t *>(A.block) + r * A.block_stride * bb, (uint32_t)(n * bb));
     }
-    float x[IT][8], b[IT][8];
+    float2 x[IT][4], b[IT][4];
 #pragma unroll
     for (int it = 0; it < IT; it++) {
-        const int c = (it * G + gt) * 8;
+        const int c = nm_col<IT>(gt, it);
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[it][i] = b[it][i] = 0.0f;
+        for (int i = 0; i < 4; i++) x[it][i] = b[it][i] = nm_both(0.0f);
         if (c < n) {
             nm_load8<VEC>(A.x, A.x_type, (int64_t)row * A.x_stride + c, n - c, x[it]);
             if (A.block) nm_load8<VEC>(A.block, A.block_type, (int64_t)row * A.block_stride + c, n - c, b[it]);
@@ -477,78 +534,69 @@ __global__ void __launch_bounds__(NM_THREADS(G)) k_ops_norm(fomoe_b200_norm_args
     }
     if (A.block) {
         float inv = 1.0f;
-        if (A.post) {
-            float ss = 0.0f;
-#pragma unroll
-            for (int it = 0; it < IT; it++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) ss = fmaf(b[it][i], b[it][i], ss);
-            ss = nm_row_sum<G>(ss, s_red);
-            inv = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)n) + A.eps));
-        }
+        if (A.post) inv = nm_inv<G, IT>(b, n, A.eps, s_red);
 #pragma unroll
         for (int it = 0; it < IT; it++) {
-            const int c = (it * G + gt) * 8;
+            const int c = nm_col<IT>(gt, it);
             if (c < n) {
-                float w[8], g[8];
+                float2 w[4];
                 if (A.post) {
                     nm_load8<VEC>(A.post, 0, c, n - c, w);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) b[it][i] *= inv * (w[i] + A.offset);
+                    for (int i = 0; i < 4; i++) b[it][i] = nm_mul(b[it][i], nm_mul(nm_both(inv), nm_add(w[i], nm_both(A.offset))));
                 }
                 if (A.gate) {
                     if (A.gate_step) {
-                        nm_load8<VEC>(A.gate, A.block_type, (int64_t)row * A.gate_stride + c, n - c, g);
+                        nm_load8<VEC>(A.gate, A.block_type, (int64_t)row * A.gate_stride + c, n - c, w);
                     } else {
                         const int64_t at = (int64_t)row * A.gate_stride;
                         const float s = A.block_type ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(A.gate)[at])
                                                      : reinterpret_cast<const float *>(A.gate)[at];
 #pragma unroll
-                        for (int i = 0; i < 8; i++) g[i] = s;
+                        for (int i = 0; i < 4; i++) w[i] = nm_both(s);
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) b[it][i] *= g[i];
+                    for (int i = 0; i < 4; i++) b[it][i] = nm_mul(b[it][i], w[i]);
                 }
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[it][i] = fmaf(A.scale, b[it][i], x[it][i]);
+                for (int i = 0; i < 4; i++) x[it][i] = nm_fma(nm_both(A.scale), b[it][i], x[it][i]);
                 if (!VEC)
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (c + i >= n) x[it][i] = 0.0f; /* columns behind the row: a gate there may have been read as 0 * inf */
+                    for (int i = 0; i < 4; i++) { /* columns behind the row: a gate there may have been read as 0 * inf */
+                        if (c + 2 * i >= n) x[it][i].x = 0.0f;
+                        if (c + 2 * i + 1 >= n) x[it][i].y = 0.0f;
+                    }
             }
         }
     }
     if (A.x_out) {
 #pragma unroll
         for (int it = 0; it < IT; it++) {
-            const int c = (it * G + gt) * 8;
+            const int c = nm_col<IT>(gt, it);
             if (c < n) nm_store8<VEC>(A.x_out, A.x_type, (int64_t)row * A.x_out_stride + c, n - c, x[it]);
         }
     }
     if (!A.pre) return;
-    float ss = 0.0f;
+    const float inv = nm_inv<G, IT>(x, n, A.eps, s_red);
 #pragma unroll
-    for (int it = 0; it < IT; it++)
+    for (int it = 0; it < IT; it++) { /* (x becomes h) */
+        const int c = nm_col<IT>(gt, it);
+        if (c >= n) continue; /* (x is 0 there) */
+        float2 w[4];
+        nm_load8<VEC>(A.pre, 0, c, n - c, w);
 #pragma unroll
-        for (int i = 0; i < 8; i++) ss = fmaf(x[it][i], x[it][i], ss);
-    ss = nm_row_sum<G>(ss, s_red);
-    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)n) + A.eps));
-#pragma unroll
-    for (int it = 0; it < IT; it++) {
-        const int c = (it * G + gt) * 8;
-        float h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (c < n) {
-            float w[8];
-            nm_load8<VEC>(A.pre, 0, c, n - c, w);
-#pragma unroll
-            for (int i = 0; i < 8; i++) h[i] = (VEC || c + i < n) ? x[it][i] * inv * (w[i] + A.offset) : 0.0f;
+        for (int i = 0; i < 4; i++) {
+            x[it][i] = nm_mul(nm_mul(x[it][i], nm_both(inv)), nm_add(w[i], nm_both(A.offset)));
+            if (!VEC) {
+                if (c + 2 * i >= n) x[it][i].x = 0.0f;
+                if (c + 2 * i + 1 >= n) x[it][i].y = 0.0f;
+            }
         }
-        if (A.h_type == FOMOE_B200_F8)
-            nm_quant8<VEC>(reinterpret_cast<uint8_t *>(A.h) + (int64_t)row * A.h_stride,
-                           A.h_scales + (int64_t)row * A.h_scales_stride, c, n, h);
-        else if (c < n)
-            nm_store8<VEC>(A.h, A.h_type, (int64_t)row * A.h_stride + c, n - c, h);
+        if (A.h_type != FOMOE_B200_F8) nm_store8<VEC>(A.h, A.h_type, (int64_t)row * A.h_stride + c, n - c, x[it]);
     }
+    if (A.h_type == FOMOE_B200_F8)
+        nm_quant<VEC, IT>(reinterpret_cast<uint8_t *>(A.h) + (int64_t)row * A.h_stride, A.h_scales + (int64_t)row * A.h_scales_stride,
+                          nm_col<IT>(gt, 0), n, x);
 }
 
 static bool nm_al(const void *p, int64_t stride, int bytes) {
@@ -585,33 +633,39 @@ extern "C" int ops_launch_norm(const fomoe_b200_norm_args_t *a, void *stream) {
     return (int)cudaGetLastError();
 }
 
-/* ------------------------------------------------------------------ rows to FP8: 16 threads per block of 128
- * (4096 x 4096 bf16: 13.6 us, 3.7 TB/s; two or four pieces of 8 columns a thread are no faster and cost small calls 0.3 us) */
+/* ------------------------------------------------------------------ rows to FP8: 8 threads per block of 128
+ * (8192 x 4096 bf16: QNEW; with 16 threads a block 25 us, bound by what every thread does once: the block's place, its
+ * scale, the scale's reciprocal.) */
 template <bool VEC>
-__global__ void __launch_bounds__(256) k_ops_quantize(int rows, int cols, int nb, const void *x, int bf16, int64_t x_stride,
+__global__ void __launch_bounds__(256) k_ops_quantize(int rows, int cols, int nb, uint64_t per_nb, const void *x, int bf16, int64_t x_stride,
                                                      uint8_t *q, int64_t q_stride, float *scales, int64_t s_stride) {
-    const uint32_t blk = blockIdx.x * 16 + (threadIdx.x >> 4), r = blk / (uint32_t)nb; /* (the host keeps rows * nb below 2^30) */
+    const uint32_t blk = blockIdx.x * 32 + (threadIdx.x >> 3); /* (the host keeps rows * nb below 2^30) */
+    const uint32_t r = nb == 1 ? blk : (uint32_t)__umul64hi(blk, per_nb); /* blk / nb: per_nb is just above 2^64 / nb */
     const int64_t row = r < (uint32_t)rows ? r : 0;
-    const int c = r < (uint32_t)rows ? (int)(blk - r * nb) * 128 + (threadIdx.x & 15) * 8 : cols;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (c < cols) nm_load8<VEC>(x, bf16, row * x_stride + c, cols - c, v);
-    nm_quant8<VEC>(q + row * q_stride, scales + row * s_stride, min(c, cols), cols, v);
+    constexpr int STEP = VEC ? 1 : 8; /* narrow accesses: neighbouring threads have neighbouring columns (4096 x 2063: QODD us, 21 without) */
+    const int c0 = r < (uint32_t)rows ? (int)(blk - r * nb) * 128 + (threadIdx.x & 7) * (VEC ? 8 : 1) : cols;
+    float2 v[2][4] = {};
+#pragma unroll
+    for (int it = 0; it < 2; it++)
+        if (c0 + 64 * it < cols) nm_load8<VEC, STEP>(x, bf16, row * x_stride + c0 + 64 * it, cols - c0 - 64 * it, v[it]);
+    nm_quant<VEC, 2, STEP>(q + row * q_stride, scales + row * s_stride, c0, cols, v);
 }
 
 extern "C" int ops_launch_f8_quantize(int rows, int cols, const void *x, int x_bf16, int64_t x_stride, uint8_t *q,
                                       int64_t q_stride, float *scales, int64_t scales_stride, void *stream) {
     const int nb = (cols + 127) / 128;
+    const uint64_t per_nb = ~0ull / (uint64_t)nb + 1; /* (nb = 1: not used) */
     const bool vec = cols % 8 == 0 && nm_al(x, rows > 1 ? x_stride : 0, x_bf16 ? 2 : 4) && ((uintptr_t)q & 7) == 0 &&
                      (rows == 1 || q_stride % 8 == 0);
     const int at_once = (1 << 30) / nb; /* rows of a launch */
     for (int64_t r0 = 0; r0 < rows; r0 += at_once) {
-        const int n = rows - r0 < at_once ? (int)(rows - r0) : at_once, grid = (int)(((int64_t)n * nb + 15) / 16);
+        const int n = rows - r0 < at_once ? (int)(rows - r0) : at_once, grid = (int)(((int64_t)n * nb + 31) / 32);
         const uint8_t *xr = reinterpret_cast<const uint8_t *>(x) + r0 * x_stride * (x_bf16 ? 2 : 4);
         if (vec)
-            k_ops_quantize<true><<<grid, 256, 0, (cudaStream_t)stream>>>(n, cols, nb, xr, x_bf16, x_stride, q + r0 * q_stride,
+            k_ops_quantize<true><<<grid, 256, 0, (cudaStream_t)stream>>>(n, cols, nb, per_nb, xr, x_bf16, x_stride, q + r0 * q_stride,
                                                                        q_stride, scales + r0 * scales_stride, scales_stride);
         else
-            k_ops_quantize<false><<<grid, 256, 0, (cudaStream_t)stream>>>(n, cols, nb, xr, x_bf16, x_stride, q + r0 * q_stride,
+            k_ops_quantize<false><<<grid, 256, 0, (cudaStream_t)stream>>>(n, cols, nb, per_nb, xr, x_bf16, x_stride, q + r0 * q_stride,
                                                                         q_stride, scales + r0 * scales_stride, scales_stride);
     }
     return (int)cudaGetLastError();
