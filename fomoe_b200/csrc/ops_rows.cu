@@ -419,35 +419,73 @@ __device__ __forceinline__ void nm_load8(const void *p, int bf16, int64_t at, in
     }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void nm_store8(void *p, int bf16, int64_t at, int left, const float2 (&v)[4]) {
-    if (VEC) {
-        if (bf16) {
-            uint32_t w[4];
+__device__ __forceinline__ void nm_store8(void *p, int bf16, int64_t at, const float2 (&v)[4]) {
+    if (bf16) {
+        uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const __nv_bfloat162 b = __float22bfloat162_rn(v[i]);
-                w[i] = *reinterpret_cast<const uint32_t *>(&b);
-            }
-            *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(p) + at) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-            *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + at) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-            *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + at + 4) = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 b = __float22bfloat162_rn(v[i]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&b);
         }
+        *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(p) + at) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
+        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + at) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + at + 4) = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+    }
+}
+
+/* A warp's run `it` by narrow accesses: neighbouring lanes take neighbouring columns, and the 256 values change hands in
+ * shared memory (s_w, the warp's).  nm_place: the column of value i of the warp's. */
+template <int IT>
+__device__ __forceinline__ int nm_place(int thread, int it, int i) {
+    return thread / 32 * (IT * 256) + (IT == 2 ? i / 64 * 128 + it * 64 + i % 64 : i);
+}
+
+/* a thread's run `it` of the row of n values from p[at] on; !VEC: the whole warp calls it, and columns behind the row are 0 */
+template <bool VEC, int IT>
+__device__ __forceinline__ void nm_get(const void *p, int bf16, int64_t at, int n, int thread, int it, float2 (&v)[4], float *s_w) {
+    if (VEC) {
+        nm_load8<true>(p, bf16, at + nm_col<IT>(thread, it), 8, v);
+    } else {
+        const int lane = thread & 31;
+        float f[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < left) {
-                const float f = i & 1 ? v[i >> 1].y : v[i >> 1].x;
-                if (bf16) reinterpret_cast<__nv_bfloat16 *>(p)[at + i] = __float2bfloat16_rn(f);
-                else reinterpret_cast<float *>(p)[at + i] = f;
-            }
+        for (int i = 0; i < 8; i++) {
+            const int c = nm_place<IT>(thread, it, 32 * i + lane);
+            f[i] = c >= n ? 0.0f : bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[at + c]) : reinterpret_cast<const float *>(p)[at + c];
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; i++) s_w[32 * i + lane] = f[i];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = *reinterpret_cast<const float2 *>(s_w + 8 * lane + 2 * i);
+    }
+}
+
+template <bool VEC, int IT>
+__device__ __forceinline__ void nm_put(void *p, int bf16, int64_t at, int n, int thread, int it, const float2 (&v)[4], float *s_w) {
+    if (VEC) {
+        nm_store8(p, bf16, at + nm_col<IT>(thread, it), v);
+    } else {
+        const int lane = thread & 31;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; i++) *reinterpret_cast<float2 *>(s_w + 8 * lane + 2 * i) = v[i];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int c = nm_place<IT>(thread, it, 32 * i + lane);
+            if (c >= n) continue;
+            if (bf16) reinterpret_cast<__nv_bfloat16 *>(p)[at + c] = __float2bfloat16_rn(s_w[32 * i + lane]);
+            else reinterpret_cast<float *>(p)[at + c] = s_w[32 * i + lane];
+        }
     }
 }
 
 /* a thread's runs of one row as e4m3; the 16 / IT threads of a block of 128 call it together */
 template <bool VEC, int IT, int STEP = 1>
-__device__ __forceinline__ void nm_quant(uint8_t *q, float *scales, int c0, int n, const float2 (&v)[IT][4]) {
+__device__ __forceinline__ void nm_quant(uint8_t *q, float *scales, int thread, int c0, int n, const float2 (&v)[IT][4], uint32_t *s_w = nullptr) {
     float amax = 0.0f;
 #pragma unroll
     for (int it = 0; it < IT; it++)
@@ -461,7 +499,7 @@ __device__ __forceinline__ void nm_quant(uint8_t *q, float *scales, int c0, int 
 #pragma unroll
     for (int it = 0; it < IT; it++) {
         const int c = c0 + 64 * it;
-        if (c >= n) continue;
+        if ((VEC || STEP > 1) && c >= n) continue;
         float2 r[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) { /* (ops_f8_quot) */
@@ -473,10 +511,20 @@ __device__ __forceinline__ void nm_quant(uint8_t *q, float *scales, int c0, int 
         for (int h = 0; h < 2; h++) w[h] = ops_f8_pack4(r[2 * h].x, r[2 * h].y, r[2 * h + 1].x, r[2 * h + 1].y);
         if (VEC) {
             *reinterpret_cast<uint2 *>(q + c) = make_uint2(w[0], w[1]);
-        } else {
+        } else if (STEP > 1) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 if (c + STEP * i < n) q[c + STEP * i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+        } else { /* (as nm_put) */
+            const int lane = threadIdx.x & 31;
+            __syncwarp();
+            s_w[2 * lane] = w[0], s_w[2 * lane + 1] = w[1];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int to = nm_place<IT>(thread, it, 32 * i + lane);
+                if (to < n) q[to] = reinterpret_cast<const uint8_t *>(s_w)[32 * i + lane];
+            }
         }
     }
 }
@@ -511,6 +559,8 @@ __device__ __forceinline__ float nm_inv(const float2 (&v)[IT][4], int n, float e
 template <bool VEC, int G, int IT>
 __global__ void __launch_bounds__(NM_THREADS(G), VEC && G == 256 ? NM_BLOCKS : 1) k_ops_norm(fomoe_b200_norm_args_t A) {
     __shared__ float s_red[NM_THREADS(G) / 32];
+    __shared__ __align__(16) float s_turn[VEC ? 1 : NM_THREADS(G) / 32][256];
+    float *s_w = s_turn[VEC ? 0 : threadIdx.x / 32];
     const int gt = threadIdx.x % G;
     const int row = blockIdx.x * (NM_THREADS(G) / G) + threadIdx.x / G;
     if (row >= A.n_tokens) return; /* whole warps (G = 32), or nobody (G = the block) */
@@ -527,9 +577,9 @@ __global__ void __launch_bounds__(NM_THREADS(G), VEC && G == 256 ? NM_BLOCKS : 1
         const int c = nm_col<IT>(gt, it);
 #pragma unroll
         for (int i = 0; i < 4; i++) x[it][i] = b[it][i] = nm_both(0.0f);
-        if (c < n) {
-            nm_load8<VEC>(A.x, A.x_type, (int64_t)row * A.x_stride + c, n - c, x[it]);
-            if (A.block) nm_load8<VEC>(A.block, A.block_type, (int64_t)row * A.block_stride + c, n - c, b[it]);
+        if (!VEC || c < n) {
+            nm_get<VEC, IT>(A.x, A.x_type, (int64_t)row * A.x_stride, n, gt, it, x[it], s_w);
+            if (A.block) nm_get<VEC, IT>(A.block, A.block_type, (int64_t)row * A.block_stride, n, gt, it, b[it], s_w);
         }
     }
     if (A.block) {
@@ -538,16 +588,16 @@ __global__ void __launch_bounds__(NM_THREADS(G), VEC && G == 256 ? NM_BLOCKS : 1
 #pragma unroll
         for (int it = 0; it < IT; it++) {
             const int c = nm_col<IT>(gt, it);
-            if (c < n) {
+            if (!VEC || c < n) {
                 float2 w[4];
                 if (A.post) {
-                    nm_load8<VEC>(A.post, 0, c, n - c, w);
+                    nm_get<VEC, IT>(A.post, 0, 0, n, gt, it, w, s_w);
 #pragma unroll
                     for (int i = 0; i < 4; i++) b[it][i] = nm_mul(b[it][i], nm_mul(nm_both(inv), nm_add(w[i], nm_both(A.offset))));
                 }
                 if (A.gate) {
                     if (A.gate_step) {
-                        nm_load8<VEC>(A.gate, A.block_type, (int64_t)row * A.gate_stride + c, n - c, w);
+                        nm_get<VEC, IT>(A.gate, A.block_type, (int64_t)row * A.gate_stride, n, gt, it, w, s_w);
                     } else {
                         const int64_t at = (int64_t)row * A.gate_stride;
                         const float s = A.block_type ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(A.gate)[at])
@@ -573,7 +623,7 @@ __global__ void __launch_bounds__(NM_THREADS(G), VEC && G == 256 ? NM_BLOCKS : 1
 #pragma unroll
         for (int it = 0; it < IT; it++) {
             const int c = nm_col<IT>(gt, it);
-            if (c < n) nm_store8<VEC>(A.x_out, A.x_type, (int64_t)row * A.x_out_stride + c, n - c, x[it]);
+            if (!VEC || c < n) nm_put<VEC, IT>(A.x_out, A.x_type, (int64_t)row * A.x_out_stride, n, gt, it, x[it], s_w);
         }
     }
     if (!A.pre) return;
@@ -581,9 +631,9 @@ __global__ void __launch_bounds__(NM_THREADS(G), VEC && G == 256 ? NM_BLOCKS : 1
 #pragma unroll
     for (int it = 0; it < IT; it++) { /* (x becomes h) */
         const int c = nm_col<IT>(gt, it);
-        if (c >= n) continue; /* (x is 0 there) */
+        if (VEC && c >= n) continue; /* (x is 0 there) */
         float2 w[4];
-        nm_load8<VEC>(A.pre, 0, c, n - c, w);
+        nm_get<VEC, IT>(A.pre, 0, 0, n, gt, it, w, s_w);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             x[it][i] = nm_mul(nm_mul(x[it][i], nm_both(inv)), nm_add(w[i], nm_both(A.offset)));
@@ -592,11 +642,11 @@ __global__ void __launch_bounds__(NM_THREADS(G), VEC && G == 256 ? NM_BLOCKS : 1
                 if (c + 2 * i + 1 >= n) x[it][i].y = 0.0f;
             }
         }
-        if (A.h_type != FOMOE_B200_F8) nm_store8<VEC>(A.h, A.h_type, (int64_t)row * A.h_stride + c, n - c, x[it]);
+        if (A.h_type != FOMOE_B200_F8) nm_put<VEC, IT>(A.h, A.h_type, (int64_t)row * A.h_stride, n, gt, it, x[it], s_w);
     }
     if (A.h_type == FOMOE_B200_F8)
         nm_quant<VEC, IT>(reinterpret_cast<uint8_t *>(A.h) + (int64_t)row * A.h_stride, A.h_scales + (int64_t)row * A.h_scales_stride,
-                          nm_col<IT>(gt, 0), n, x);
+                          gt, nm_col<IT>(gt, 0), n, x, reinterpret_cast<uint32_t *>(s_w));
 }
 
 static bool nm_al(const void *p, int64_t stride, int bytes) {
@@ -648,7 +698,7 @@ __global__ void __launch_bounds__(256) k_ops_quantize(int rows, int cols, int nb
 #pragma unroll
     for (int it = 0; it < 2; it++)
         if (c0 + 64 * it < cols) nm_load8<VEC, STEP>(x, bf16, row * x_stride + c0 + 64 * it, cols - c0 - 64 * it, v[it]);
-    nm_quant<VEC, 2, STEP>(q + row * q_stride, scales + row * s_stride, c0, cols, v);
+    nm_quant<VEC, 2, STEP>(q + row * q_stride, scales + row * s_stride, 0, c0, cols, v);
 }
 
 extern "C" int ops_launch_f8_quantize(int rows, int cols, const void *x, int x_bf16, int64_t x_stride, uint8_t *q,
