@@ -48,7 +48,8 @@ static int f8_launch_after(void (*k)(P...), dim3 grid, int threads, int smem, cu
  * over (expert, block, warp) give every warp its first place, a second walk places the pairs.  The order inside an expert is
  * the order of the pairs, so results do not depend on timing.  The shared expert's pairs (n_routed + t) come last.  With more
  * than one block a first launch (COUNT) leaves each block's counts in `block_counts`.  Eight ids a lane are in flight at
- * once.  (65,536 pairs: one block, one id a lane 150 us; eight ids 100 us, bound by one SM's scattered stores.) */
+ * once.  (65,536 pairs in 64 experts: one block 150 us, eight ids
+ * a lane 100 us, bound by one SM's scattered stores; by 16 blocks in two launches 19 us.) */
 #define BK_THREADS 1024
 #define BK_WARPS 32
 #define BK_AHEAD 8
@@ -181,9 +182,9 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
  * warps 0..7 are two warpgroups that each join half of the columns.  Tensor memory holds NB buffers of NT columns, so the
  * MMAs of the next block run while this one's sums are joined.
  *
- * What bounds it (4096 x 8192 x 4096, 148 us, 1.85 PFLOP/s): the MMAs with nothing but their barriers take 121 us -- the
+ * What bounds it (4096 x 8192 x 4096, 144.5 us, 1.90 PFLOP/s): the MMAs with nothing but their barriers take 121 us -- the
  * operands of 128 x 256 tiles pass shared memory twice, 192 bytes a cycle at the tensor cores' full rate --, the joining
- * FMAs 13 us more and the way out 14 us.  Two SMs a tile of 256 x 256 (cta_group::2: two thirds of the operand bytes) came
+ * FMAs 13 us more and the way out 10 us.  Two SMs a tile of 256 x 256 (cta_group::2: two thirds of the operand bytes) came
  * to 147 us, with more padding for the experts (1.81 against 1.76 ms): its hand-overs between the SMs cost what the bytes
  * saved.  Handing the columns over in two halves (180 us) and 16 joining warps (158 us) were slower: every barrier is
  * shared-memory traffic too.

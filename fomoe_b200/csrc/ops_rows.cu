@@ -30,7 +30,7 @@
  * The best K + 1 keys: each lane's best key first; the (K + 1)-th best of those is a bound that every one of the best K + 1
  * keys reaches, and few others do.  The keys that reach it are put side by side in shared memory, one to a lane, and each
  * counts how many are better.  (16,384 tokens x 384 experts, sigmoid + bias, top 8: 87 us in 64 bits with a round over all
- * keys for every slot) */
+ * keys for every slot, 25 us so; bound by its instructions, 1000 a token at 58 % of the issue slots) */
 #define RT_WARPS 4
 #define RT_NEAR(a, b) (8e-6f + 1e-6f * (fabsf(a) + fabsf(b)))
 
@@ -351,10 +351,17 @@ extern "C" int ops_launch_route(const ops_route_t *a, void *stream) {
 }
 
 /* ------------------------------------------------------------------ norms around a block
+ * r = block / rms(block) (w_post + offset) g;  x' = x + scale r;  h = x' / rms(x') (w_pre + offset)
  * G threads share a row; every thread holds IT runs of 8 neighbouring columns in registers, so the row is read once and
- * written once whatever the number of norms.  16 neighbouring threads hold one block of 128, whose amax is a shuffle
- * reduction.  VEC: all pointers and strides allow 16-byte accesses and n is a multiple of 8; otherwise the same code
- * goes element by element. */
+ * written once whatever the number of norms.  The threads of a block of 128 are neighbours: its amax is one reduction.
+ * VEC: all pointers and strides allow 16-byte accesses and n is a multiple of 8; otherwise neighbouring lanes take
+ * neighbouring columns and the values change hands in shared memory, so that each thread has the same ones.
+ *
+ * What bounds it (8192 x 4096, fp32 residual, bf16 block, FP8 out): 69 us, 5.3 TB/s of 6.5.  The chain of a row -- load, two
+ * sums over the block, two square roots, the scale of a block -- is long, so it takes many rows at once on an SM: blocks of 256
+ * threads whose registers let five share one, and the next rows asked into L2.  Rings of rows in shared memory under persistent
+ * blocks (108 us and more: they take the L1 that holds the weights) and 128 threads with four runs each (85 us) were slower;
+ * values in pairs (fma.rn.f32x2) saved 2 us, one scale for 16 values a thread the quantiser a quarter of its time. */
 #define NM_THREADS(G) ((G) == 32 ? 256 : (G))
 #define NM_AHEAD 148 /* rows: what a later block reads is asked into L2 (8192 x 4096: 74 us, without 82, 296 rows ahead 74) */
 #define NM_BLOCKS 5  /* of 256 threads, an SM (8192 x 4096: 68 us, with 4 74, with 6 and spills 93) */
@@ -684,15 +691,15 @@ extern "C" int ops_launch_norm(const fomoe_b200_norm_args_t *a, void *stream) {
 }
 
 /* ------------------------------------------------------------------ rows to FP8: 8 threads per block of 128
- * (8192 x 4096 bf16: QNEW; with 16 threads a block 25 us, bound by what every thread does once: the block's place, its
- * scale, the scale's reciprocal.) */
+ * (8192 x 4096 bf16: 18.2 us, 5.5 TB/s, 75 % of the issue slots; with 16 threads a block 25 us, bound by what every thread does
+ * once: the block's place, its scale, the scale's reciprocal.) */
 template <bool VEC>
 __global__ void __launch_bounds__(256) k_ops_quantize(int rows, int cols, int nb, uint64_t per_nb, const void *x, int bf16, int64_t x_stride,
                                                      uint8_t *q, int64_t q_stride, float *scales, int64_t s_stride) {
     const uint32_t blk = blockIdx.x * 32 + (threadIdx.x >> 3); /* (the host keeps rows * nb below 2^30) */
     const uint32_t r = nb == 1 ? blk : (uint32_t)__umul64hi(blk, per_nb); /* blk / nb: per_nb is just above 2^64 / nb */
     const int64_t row = r < (uint32_t)rows ? r : 0;
-    constexpr int STEP = VEC ? 1 : 8; /* narrow accesses: neighbouring threads have neighbouring columns (4096 x 2063: QODD us, 21 without) */
+    constexpr int STEP = VEC ? 1 : 8; /* narrow accesses: neighbouring threads have neighbouring columns (4096 x 2063: 15 us, 21 without) */
     const int c0 = r < (uint32_t)rows ? (int)(blk - r * nb) * 128 + (threadIdx.x & 7) * (VEC ? 8 : 1) : cols;
     float2 v[2][4] = {};
 #pragma unroll
