@@ -1306,15 +1306,15 @@ __global__ void __launch_bounds__(256) k_ops_combine(const __half *dots, const f
     }
 }
 
-/* Each pair by itself, or bucketed by expert: microseconds of either.  Few pairs stream their experts' weights once a pair
- * (5 TB/s and 8 us around it: one token with 11 experts of 4096 x 1024 34.5 us, bucketed 59; 64 pairs of 2048 x 768 67 and
- * 74 us), bucketed they are read once an expert but five kernels and their tiles come first (4096 x 1024, 45 pairs: 114 us
- * by themselves, bucketed 102).  How many different experts there will be is known on the device only: the expectation of
- * equally likely ones stands for it. */
+/* Each pair by itself, or bucketed by expert: microseconds of either.  Few pairs stream their experts' weights once a pair, at
+ * 5.3 TB/s and with 8 us around it and a block's start a pair; bucketed they are read once an expert, but five kernels and
+ * their tiles come first.  (By themselves | bucketed: one token with 11 experts of 4096 x 1024 34.8 | 56 us, 27 pairs of it
+ * 74 | 86, 45 pairs 114 | 94; 2048 x 768, 32 pairs 39 | 46, 64 pairs 67 | 64; 192 pairs in 17 experts of 512 x 256 30 | 23.)
+ * How many different experts there will be is known on the device only: the expectation of equally likely ones stands for it. */
 static int experts_few(const fomoe_b200_f8_experts_args_t *a, int n_pairs) {
     const double bytes = 3.0 * a->n_embd * a->n_inter, routed = (double)a->n_tokens * a->top_k;
     const double hit = a->n_experts * (1.0 - exp(-routed / a->n_experts)) + (a->has_shared ? 1.0 : 0.0);
-    return n_pairs <= 256 && 8.0 + n_pairs * bytes / 5.0e6 <= 30.0 + hit * bytes / 5.5e6;
+    return n_pairs <= 256 && 8.0 + n_pairs * (0.05 + bytes / 5.3e6) <= 22.0 + hit * bytes / 5.5e6;
 }
 
 extern "C" void ops_experts_layout(const fomoe_b200_f8_experts_args_t *a, ops_experts_ws_t *w) {
