@@ -85,6 +85,8 @@ class DeviceOps:
     def __del__(self):
         try:
             if getattr(self, "_h", None):
+                if self._t.cuda.is_current_stream_capturing():
+                    return  # a wait would end the capture: the handle's 64 bytes stay
                 self._t.cuda.synchronize(self.device)  # its status word may still be written to
         except Exception:
             return

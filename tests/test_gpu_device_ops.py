@@ -611,3 +611,19 @@ def test_tensors_elsewhere_are_refused(ops):
         ops.route(torch.zeros(2, 8), 2)
     with pytest.raises(ValueError):
         ops.f8_quantize(torch.zeros(2, 8))
+
+
+def test_handle_dropped_while_capturing(ops, fb):
+    """A handle that goes away while another's call is captured leaves the capture alone."""
+    x = torch.arange(300, device="cuda").float().view(3, 100)
+    ops.f8_quantize(x)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    other = fb.DeviceOps(0)
+    with torch.cuda.graph(gr):
+        q, s = ops.f8_quantize(x)
+        del other
+    gr.replay()
+    torch.cuda.synchronize()
+    want = ops.f8_quantize(x)
+    assert (q.view(torch.uint8) == want[0].view(torch.uint8)).all() and (s == want[1]).all()
