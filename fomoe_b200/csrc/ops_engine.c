@@ -178,7 +178,7 @@ int fomoe_b200_ops_f8_quantize(fomoe_b200_ops_t *o, int rows, int cols, const vo
 
 int fomoe_b200_ops_f8_matmul(fomoe_b200_ops_t *o, const fomoe_b200_f8_matmul_args_t *args, void *stream) {
     if (!o) return -1;
-    NEED(o, args && args->m >= 0 && args->m <= OPS_MOST && args->n >= 0 && args->n <= OPS_MOST, "f8_matmul: m and n are 0 to 2^30");
+    NEED(o, args && args->m >= 0 && args->m <= OPS_MOST && args->n >= 0 && args->n <= OPS_MOST / 2, "f8_matmul: m is 0 to 2^30, n 0 to 2^29"); /* (bytes of a row of out go into a signed coordinate) */
     NEED(o, args->k > 0 && args->k <= OPS_MOST && args->k % 16 == 0, "f8_matmul: k is a positive multiple of 16");
     if (args->m == 0 || args->n == 0) return 0;
     fomoe_b200_f8_matmul_args_t own = *args, *a = &own;

@@ -471,7 +471,7 @@ int fomoe_b200_ops_f8_quantize(fomoe_b200_ops_t *ops, int rows, int cols, const 
                                void *stream);
 
 /* out[m][n] = sum_k a[m][k] b[n][k], a FP8 rows, b an FP8 weight matrix.  k a multiple of 16; a and b 16-byte aligned,
- * their strides (bytes) multiples of 16; scale strides in elements. */
+ * their strides (bytes) multiples of 16; scale strides in elements.  m, k <= 2^30, n <= 2^29. */
 typedef struct {
     int m, n, k;
     const uint8_t *a;

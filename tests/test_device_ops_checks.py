@@ -172,3 +172,17 @@ def test_other_device_is_current_again_and_a_failed_launch_is_reported(ops):
     ops.fake.cudaGetDevice(C.byref(got))
     assert got.value == 1 and ops.kernel_launches() == before
     dev(0)
+
+
+def test_matmul_limits(ops):
+    """The largest sizes whose coordinates fit, and the next ones (the launcher is a stand-in: nothing is read)."""
+    from fomoe_b200.device_ops import F32, MatmulArgs
+
+    def call(m, n, k):
+        nb = (k + 127) // 128
+        return ops._l.fomoe_b200_ops_f8_matmul(ops._h, MatmulArgs(m, n, k, 1 << 20, k, 1 << 20, nb, 1 << 20, k, 1 << 20, nb, 1 << 20,
+                                                                 F32, n), None)
+    assert call(32, 1 << 29, 16) == 0 and call(1 << 30, 16, 16) == 0 and call(1, 1, 1 << 30) == 0
+    n = launches(ops)
+    assert call(32, (1 << 29) + 1, 16) == -1 and call((1 << 30) + 1, 16, 16) == -1 and call(1, 1, (1 << 30) + 16) == -1
+    assert launches(ops) == n
