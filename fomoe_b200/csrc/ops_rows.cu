@@ -30,8 +30,9 @@
  * The best K + 1 keys: each lane's best key first; the (K + 1)-th best of those is a bound that every one of the best K + 1
  * keys reaches, and few others do.  The keys that reach it are put side by side in shared memory, one to a lane, and each
  * counts how many are better.  (16,384 tokens x 384 experts, sigmoid + bias, top 8: 87 us in 64 bits with a round over all
- * keys for every slot, 25 us so; bound by its instructions, 1000 a token at 58 % of the issue slots) */
+ * keys for every slot, 18 us so; bound by its instructions, 810 a token at 69 % of the issue slots) */
 #define RT_WARPS 4
+#define RT_BLOCKS 8 /* an SM: registers for so many (16,384 x 512, bias, top 16: 35 us, unbounded 36, for ten 44) */
 #define RT_NEAR(a, b) (8e-6f + 1e-6f * (fabsf(a) + fabsf(b)))
 
 /* floats as unsigned numbers in the same order; 0 stands for "closed" (below -inf) */
@@ -62,7 +63,8 @@ __device__ __forceinline__ T rt_group_score(const T *c, int G, int per, int best
     return best == 2 && b > NINF ? a + b : a;
 }
 
-/* mask of the groups that stay: those with fewer than topk better ones (lower group first among equals) */
+/* The groups that stay: those with fewer than topk better ones (lower group first among equals), bit g << shift for group g.
+ * Group g's score is in the lane of that number. */
 template <typename T>
 __device__ __forceinline__ uint32_t rt_groups_stay(T gs, int G, int topk, int shift) {
     const int lane = threadIdx.x & 31, g = lane >> shift;
@@ -71,11 +73,10 @@ __device__ __forceinline__ uint32_t rt_groups_stay(T gs, int G, int topk, int sh
         const T o = __shfl_sync(FULL, gs, h << shift);
         rank += o > gs || (o == gs && h < g);
     }
-    const uint32_t m = __ballot_sync(FULL, (lane & ((1 << shift) - 1)) == 0 && g < G && rank < topk);
-    uint32_t keep = 0;
-    for (int h = 0; h < G; h++) keep |= ((m >> (h << shift)) & 1u) << h;
-    return keep;
+    return __ballot_sync(FULL, (lane & ((1 << shift) - 1)) == 0 && g < G && rank < topk);
 }
+/* expert e's bit of it; mul: 2^20 / per, rounded up (exact for e < 512) */
+#define RT_STAYS(stay, e, mul, shift) (((stay) >> ((((uint32_t)(e) * (mul)) >> 20) << (shift))) & 1u)
 
 __device__ __forceinline__ float rt_logit(const ops_route_t &A, int t, int e) {
     const int64_t at = (int64_t)t * A.row_stride + e;
@@ -84,12 +85,12 @@ __device__ __forceinline__ float rt_logit(const ops_route_t &A, int t, int e) {
 }
 
 /* The choices in 64 bits, to c[0 .. E) (-inf where closed).  Rare: written for size. */
-__device__ __noinline__ void rt_exact_choices(const ops_route_t &A, int t, bool shut, float mx, double *c) {
+__device__ __noinline__ void rt_exact_choices(const ops_route_t &A, int t, float mx, double *c) {
     const int lane = threadIdx.x & 31, E = A.cfg.n_experts;
     double sum = 0.0;
     for (int e = lane; e < E; e += 32) {
         const float v = rt_logit(A, t, e);
-        const bool open = !shut && v > -INFINITY;
+        const bool open = v > -INFINITY;
         const double x = fmin((double)v, (double)FLT_MAX);
         double p = 0.0;
         if (open) p = A.cfg.score == FOMOE_B200_SOFTMAX ? exp(x - (double)mx) : 1.0 / (1.0 + exp(-x));
@@ -109,14 +110,14 @@ __device__ __noinline__ void rt_exact_choices(const ops_route_t &A, int t, bool 
 }
 
 /* The choice of expert e in 64 bits (the whole warp calls it: softmax needs the sum over all experts). */
-__device__ __noinline__ double rt_exact_choice(const ops_route_t &A, int t, bool shut, float mx, int e) {
+__device__ __noinline__ double rt_exact_choice(const ops_route_t &A, int t, float mx, int e) {
     const int lane = threadIdx.x & 31, E = A.cfg.n_experts;
     const bool softmax = A.cfg.score == FOMOE_B200_SOFTMAX;
     double sum = 0.0;
     if (softmax) {
         for (int i = lane; i < E; i += 32) {
             const float v = rt_logit(A, t, i);
-            if (!shut && v > -INFINITY) sum += exp(fmin((double)v, (double)FLT_MAX) - (double)mx);
+            if (v > -INFINITY) sum += exp(fmin((double)v, (double)FLT_MAX) - (double)mx);
         }
         for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(FULL, sum, s);
     }
@@ -127,14 +128,14 @@ __device__ __noinline__ double rt_exact_choice(const ops_route_t &A, int t, bool
 
 /* the top_k of c by rounds over all of it; closed: what is never chosen; lane r gets the id of slot r */
 template <typename T>
-__device__ __noinline__ int rt_top(T *c, T closed, int E, int K, uint32_t keep, int per) {
+__device__ __noinline__ int rt_top(T *c, T closed, int E, int K, uint32_t keep, uint32_t mul, int shift) {
     const int lane = threadIdx.x & 31;
     int my_id = -1;
     for (int r = 0; r < K; r++) {
         T v = closed;
         int i = OPS_MAX_E;
         for (int e = lane; e < E; e += 32)
-            if (c[e] > v && ((keep >> (e / per)) & 1u)) {
+            if (c[e] > v && RT_STAYS(keep, e, mul, shift)) {
                 v = c[e];
                 i = e;
             }
@@ -161,16 +162,32 @@ __device__ __forceinline__ float rt_sigmoid(float x) { /* (x = -inf: 0) */
     return x >= 0.0f ? q : e * q;
 }
 
+/* the same for a choice, whose absolute error is what counts: 1 / (1 + 2^(-x log2 e)), and 0 where that power overflows */
+__device__ __forceinline__ float rt_sigmoid_choice(float x) {
+    float e, p;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(1.0f + e));
+    return p;
+}
+
 /* NPL: experts of a lane; LOW: as many as every lane has for certain (the size before in RT_SIZES) */
 template <int NPL, int LOW>
-__global__ void __launch_bounds__(32 * RT_WARPS) k_ops_route(const __grid_constant__ ops_route_t A) {
+__global__ void __launch_bounds__(32 * RT_WARPS, RT_BLOCKS) k_ops_route(const __grid_constant__ ops_route_t A) {
     __shared__ double s_c[RT_WARPS][OPS_MAX_E];
-    __shared__ uint2 s_best[RT_WARPS][32];
+    __shared__ uint2 s_best[RT_WARPS][32]; /* candidates: choice, expert */
+    __shared__ __align__(16) uint32_t s_key[RT_WARPS][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int t = blockIdx.x * RT_WARPS + warp;
     if (t >= A.n_tokens) return;
     const int E = A.cfg.n_experts, K = A.cfg.top_k, G = A.cfg.n_group;
-    const bool shut = A.valid && A.valid[t] == 0, softmax = A.cfg.score == FOMOE_B200_SOFTMAX;
+    const bool softmax = A.cfg.score == FOMOE_B200_SOFTMAX;
+    if (A.valid && A.valid[t] == 0) { /* padding: every expert is closed */
+        if (lane < K) {
+            A.ids[(int64_t)t * K + lane] = -1;
+            A.weights[(int64_t)t * K + lane] = 0.0f;
+        }
+        return;
+    }
     float x[NPL];
 #define RT_AT(j) ((j) < LOW ? (j) * 32 + lane : min((j) * 32 + lane, E - 1)) /* an expert that is there */
     if (A.logits_bf16) { /* (all loads first) */
@@ -188,10 +205,10 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_ops_route(const __grid_consta
     for (int j = 0; j < NPL; j++) {
         x[j] = fminf(fmaxf(x[j], -INFINITY), FLT_MAX);
         if (j >= LOW && j * 32 + lane >= E) x[j] = -INFINITY;
-        if (shut) x[j] = -INFINITY;
-        mx = fmaxf(mx, x[j]);
     }
     if (softmax) {
+#pragma unroll
+        for (int j = 0; j < NPL; j++) mx = fmaxf(mx, x[j]);
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, s));
         float sum = 0.0f;
@@ -205,55 +222,69 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_ops_route(const __grid_consta
     /* what decides the order: the choice, or without a bias the logit itself; -inf where closed */
     float v[NPL];
     if (A.bias || G > 1) {
-        const float m0 = mx > -INFINITY ? mx : 0.0f;
+        if (softmax) {
+            const float m0 = mx > -INFINITY ? mx : 0.0f;
 #pragma unroll
-        for (int j = 0; j < NPL; j++) {
-            const int e = j * 32 + lane;
-            float c = softmax ? __expf(x[j] - m0) * inv : rt_sigmoid(x[j]);
-            if (A.bias) c += __ldg(A.bias + RT_AT(j));
-            c = x[j] > -INFINITY && c > -INFINITY ? c : -INFINITY;
-            v[j] = A.bias ? c : x[j];
-            if (G > 1 && e < E) reinterpret_cast<float *>(s_c[warp])[e] = c;
+            for (int j = 0; j < NPL; j++) v[j] = __expf(x[j] - m0) * inv;
+        } else {
+#pragma unroll
+            for (int j = 0; j < NPL; j++) v[j] = rt_sigmoid_choice(x[j]);
+        }
+        if (A.bias) {
+#pragma unroll
+            for (int j = 0; j < NPL; j++) v[j] += __ldg(A.bias + RT_AT(j)); /* (NaN: no comparison below finds it) */
+        }
+#pragma unroll
+        for (int j = 0; j < NPL; j++) v[j] = x[j] > -INFINITY ? v[j] : -INFINITY;
+        if (G > 1) {
+#pragma unroll
+            for (int j = 0; j < NPL; j++)
+                if (j < LOW || j * 32 + lane < E) reinterpret_cast<float *>(s_c[warp])[j * 32 + lane] = v[j];
+        }
+        if (!A.bias) {
+#pragma unroll
+            for (int j = 0; j < NPL; j++) v[j] = x[j];
         }
     } else {
 #pragma unroll
         for (int j = 0; j < NPL; j++) v[j] = x[j];
     }
-    const int per = E / G;
-    uint32_t keep = 0xffffffffu;
+    uint32_t keep = 0xffffffffu, mul = 0;
+    int shift = 0;
     if (G > 1) {
+        const int per = E / G;
         __syncwarp();
-        const int shift = 5 - (32 - __clz(G - 1)); /* lanes of a group, as a power of two */
+        mul = ((1u << 20) + per - 1) / per;
+        shift = 5 - (32 - __clz(G - 1)); /* lanes of a group, as a power of two */
         const float gs = rt_group_score(reinterpret_cast<const float *>(s_c[warp]), G, per, A.cfg.group_best, shift);
         keep = rt_groups_stay(gs, G, A.cfg.topk_group, shift);
-        /* does the cut pass between two scores that are too close? */
-        const bool mine = (keep >> min(lane >> shift, 31)) & 1u;
-        bool near = false;
-        for (int h = 0; h < G; h++) {
-            const float o = __shfl_sync(FULL, gs, h << shift);
-            near |= (lane >> shift) < G && mine && !((keep >> h) & 1u) && o > -INFINITY && !(gs - o > 2.0f * RT_NEAR(gs, o));
-        }
-        if (__any_sync(FULL, near)) {
-            rt_exact_choices(A, t, shut, mx, s_c[warp]);
-            keep = rt_groups_stay(rt_group_score(s_c[warp], G, per, A.cfg.group_best, shift), G, A.cfg.topk_group, shift);
+        /* does the cut pass between two scores that are too close?  The lowest that stays and the highest that does not are
+         * the closest two; the largest of all is taken for the size that their error goes by. */
+        const bool head = (lane & ((1 << shift) - 1)) == 0 && (lane >> shift) < G, in = (keep >> lane) & 1u;
+        const uint32_t out = __reduce_max_sync(FULL, head && !in ? rt_key(gs) : 0u), low = __reduce_min_sync(FULL, head && in ? rt_key(gs) : 0xffffffffu);
+        if (out > rt_key(-INFINITY)) {
+            const float a = rt_val(low), b = rt_val(out);
+            const float size = __uint_as_float(__reduce_max_sync(FULL, head && gs > -INFINITY ? __float_as_uint(fabsf(gs)) : 0u));
+            if (!(a - b > 2.0f * RT_NEAR(size, size))) {
+                rt_exact_choices(A, t, mx, s_c[warp]);
+                keep = rt_groups_stay(rt_group_score(s_c[warp], G, per, A.cfg.group_best, shift), G, A.cfg.topk_group, shift);
+            }
         }
 #pragma unroll
-        for (int j = 0; j < NPL; j++) {
-            const int e = j * 32 + lane;
-            if (e < E && !((keep >> (e / per)) & 1u)) v[j] = -INFINITY;
-        }
+        for (int j = 0; j < NPL; j++)
+            if (!RT_STAYS(keep, j * 32 + lane, mul, shift)) v[j] = -INFINITY; /* (behind the last expert: closed already) */
     }
     float most = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NPL; j++) most = fmaxf(most, v[j]);
     uint32_t best = most > -INFINITY ? rt_key(most) : 0u;
-    float bound = -FLT_MAX; /* (all that is open; a value below it would be an infinite bias) */
+    uint32_t w = 0;
+#pragma unroll 3
     for (int r = 0; r <= K; r++) { /* (equal ones of several lanes go together: the bound is only lower for it) */
-        const uint32_t w = __reduce_max_sync(FULL, best);
-        bound = w == 0 ? -FLT_MAX : rt_val(w);
-        if (w == 0) break;
+        w = __reduce_max_sync(FULL, best);
         best = best == w ? 0u : best;
     }
+    float bound = w ? rt_val(w) : -FLT_MAX; /* (all that is open; a value below it would be an infinite bias) */
     if (A.bias) { /* and those that may be as good for all fp32 can say */
         const float low = bound - RT_NEAR(bound, bound);
         bound = low >= -FLT_MAX ? low : -FLT_MAX; /* (infinite choices: all that is open) */
@@ -265,36 +296,41 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_ops_route(const __grid_consta
         const uint32_t m = __ballot_sync(FULL, in);
         if (m) { /* (most have none) */
             const int at = n + __popc(m & ((1u << lane) - 1u));
-            if (in && at < 32) s_best[warp][at] = make_uint2(rt_key(v[j]), (uint32_t)(j * 32 + lane));
+            if (in && at < 32) s_best[warp][at] = make_uint2(__float_as_uint(v[j]), (uint32_t)(j * 32 + lane));
             n += __popc(m);
         }
     }
     __syncwarp();
     int slot = lane, id = -1; /* this lane writes slot `slot`, if there is one */
+    float lx = 0.0f;          /* the logit of `id` */
     bool exact = false;
     if (n <= 32) {
-        const uint2 own = lane < n ? s_best[warp][lane] : make_uint2(0u, 0u);
-        int rank = 0;
-        for (int i = 0; i < n; i++) {
-            const uint2 o = s_best[warp][i];
-            rank += o.x > own.x || (o.x == own.x && o.y < own.y);
+        uint32_t own = 0;
+        if (lane < n) {
+            const uint2 c = s_best[warp][lane];
+            own = rt_key(__uint_as_float(c.x));
+            id = (int)c.y;
+            lx = fminf(rt_logit(A, t, id), FLT_MAX); /* (holding all of x this far costs occupancy) */
         }
+        s_key[warp][lane] = own;
         __syncwarp();
-        if (lane < n) { /* (lanes behind the candidates keep their own slot: empty) */
-            slot = rank;
-            id = (int)own.y;
-            s_best[warp][rank] = own;
+        int rank = 0; /* (candidates lie in the order of their ids: of equal ones the earlier is the better) */
+        for (int i = 0; i < n; i += 4) {
+            const uint4 o = *reinterpret_cast<const uint4 *>(&s_key[warp][i]);
+            rank += (o.x + (i < lane) > own) + (o.y + (i + 1 < lane) > own) + (o.z + (i + 2 < lane) > own) + (o.w + (i + 3 < lane) > own);
         }
-        __syncwarp();
+        slot = lane < n ? rank : lane;
         if (A.bias) { /* neighbours among the best K + 1 that are too close? */
+            __syncwarp();
+            if (lane < n) s_key[warp][rank] = own;
+            __syncwarp();
             bool near = false;
             if (lane < K && lane + 1 < n) {
-                const float a = rt_val(s_best[warp][lane].x), b = rt_val(s_best[warp][lane + 1].x);
+                const float a = rt_val(s_key[warp][lane]), b = rt_val(s_key[warp][lane + 1]);
                 near = !(a - b > RT_NEAR(a, b));
             }
             if (__any_sync(FULL, near)) { /* rank the candidates again, by their exact choices */
-                id = lane < n ? (int)own.y : -1;
-                const double c = rt_exact_choice(A, t, shut, mx, id);
+                const double c = rt_exact_choice(A, t, mx, id);
                 rank = 0;
                 for (int i = 0; i < n; i++) {
                     const double oc = __shfl_sync(FULL, c, i);
@@ -310,20 +346,18 @@ __global__ void __launch_bounds__(32 * RT_WARPS) k_ops_route(const __grid_consta
         for (int j = 0; j < NPL; j++)
             if (j * 32 + lane < E) c[j * 32 + lane] = v[j] > -INFINITY ? rt_key(v[j]) : 0u;
         __syncwarp();
-        id = rt_top<uint32_t>(c, 0u, E, K, keep, per);
+        id = rt_top<uint32_t>(c, 0u, E, K, keep, mul, shift);
     } else {
         exact = true;
     }
     if (exact) {
-        rt_exact_choices(A, t, shut, mx, s_c[warp]);
+        rt_exact_choices(A, t, mx, s_c[warp]);
         slot = lane;
-        id = rt_top<double>(s_c[warp], (double)-INFINITY, E, K, keep, per);
+        id = rt_top<double>(s_c[warp], (double)-INFINITY, E, K, keep, mul, shift);
     }
+    if (n > 32 && id >= 0) lx = fminf(rt_logit(A, t, id), FLT_MAX);
     float p = 0.0f;
-    if (slot < K && id >= 0) {
-        const float v = fminf(rt_logit(A, t, id), FLT_MAX);
-        p = softmax ? __expf(v - mx) * inv : rt_sigmoid(v);
-    }
+    if (slot < K && id >= 0) p = softmax ? __expf(lx - mx) * inv : rt_sigmoid(lx);
     if (A.cfg.renorm) {
         float s = p;
 #pragma unroll
