@@ -182,12 +182,16 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
  * warps 0..7 are two warpgroups that each join half of the columns.  Tensor memory holds NB buffers of NT columns, so the
  * MMAs of the next block run while this one's sums are joined.
  *
- * What bounds it (4096 x 8192 x 4096, 144.5 us, 1.90 PFLOP/s): the MMAs with nothing but their barriers take 121 us -- the
- * operands of 128 x 256 tiles pass shared memory twice, 192 bytes a cycle at the tensor cores' full rate --, the joining
- * FMAs 13 us more and the way out 10 us.  Two SMs a tile of 256 x 256 (cta_group::2: two thirds of the operand bytes) came
- * to 147 us, with more padding for the experts (1.81 against 1.76 ms): its hand-overs between the SMs cost what the bytes
- * saved.  Handing the columns over in two halves (180 us) and 16 joining warps (158 us) were slower: every barrier is
- * shared-memory traffic too.
+ * F8_PAIR: two SMs work on one tile of 256 x 256 (cta_group::2).  Each loads its own 128 rows and half of the weights'
+ * rows, 32 KB a block of k instead of 48, one thread of the first issues the MMAs of both, and each joins its own rows.  Six
+ * stages leave 2 KB of staging a warp, so rows leave in runs of 64 bytes by plain stores.
+ *
+ * What bounds it (4096 x 8192 x 4096): one SM a tile 148 us, 1.86 PFLOP/s -- the MMAs with nothing but their barriers take 121
+ * us, the operands of 128 x 256 tiles pass shared memory twice, 192 bytes a cycle at the tensor cores' full rate; the joining
+ * FMAs and the way out are the rest --, pairs 136 us, 2.02 PFLOP/s (their bare MMAs 102).  Under the power cap, where a long
+ * step runs, 177 and 159 us at 1.66 GHz.  With four stages and TMA stores out pairs took 179 us there, with stores of
+ * 32 bytes from registers 172.  Handing the columns over in two halves (180 us) and 16 joining warps (158 us) were slower:
+ * every barrier is shared-memory traffic too.
  *
  *   dense    A: rows of a;                               B: rows of b;                        D to out
  *   gate/up  A: the tokens of an expert's pairs;         B: 128 gate rows, 128 up rows;       silu(g) u to FP8, 128 a block
@@ -196,6 +200,8 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
  * Every wait is bounded; when one runs out the status word is set, all roles stop waiting and the block drains, frees its
  * tensor memory and returns. */
 enum { F8_DENSE = 0, F8_GATE_UP = 1, F8_DOWN = 2 };
+/* a tile belongs to one SM, to the SMs of a cluster that share its blocks of k, or to two SMs that multiply together */
+enum { F8_ONE = 0, F8_SPLIT = 1, F8_PAIR = 2 };
 
 #define F8_THREADS 384
 #define F8_EPI_WARPS 8
@@ -279,19 +285,42 @@ __device__ __forceinline__ uint64_t f8_desc(uint32_t saddr) {
            ((uint64_t)2 << 61);
 }
 
+template <bool PAIR>
 __device__ __forceinline__ void f8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+            "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+            "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
 
-/* all MMAs so far, then an arrival at `bar` */
+/* all MMAs so far, then an arrival at `bar`, in a pair at both SMs' */
+template <bool PAIR>
 __device__ __forceinline__ void f8_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+/* the same shared-memory address in the pair's first SM */
+__device__ __forceinline__ uint32_t f8_leader(uint32_t addr) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
 }
 
 __device__ __forceinline__ uint32_t f8_cluster_size() {
@@ -311,12 +340,20 @@ __device__ __forceinline__ void f8_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-/* a box of the map to shared memory */
+/* a box of the map to this SM's shared memory; in a pair the barrier may be the first SM's */
+template <bool PAIR>
 __device__ __forceinline__ void f8_tma2(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+            "[%4];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
 }
 
 __device__ __forceinline__ void f8_tmem_ld32(uint32_t taddr, uint32_t *r) {
@@ -343,14 +380,16 @@ __device__ __forceinline__ void f8_fma2(float2 &acc, uint32_t v0, uint32_t v1, f
 
 __device__ __forceinline__ float f8_silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
-template <int MODE, int NT>
+template <int MODE, int NT, int KIND>
 struct f8_cfg {
-    static constexpr int B_BYTES = NT * 128;
+    static constexpr bool PAIR = KIND == F8_PAIR, SPLIT = KIND == F8_SPLIT;
+    static constexpr int ROWS = PAIR ? 256 : 128;              /* of a tile */
+    static constexpr int B_BYTES = (PAIR ? NT / 2 : NT) * 128; /* of one SM's share */
     static constexpr int STAGE = (int)F8_A_BYTES + B_BYTES;
-    static constexpr int STAGES = NT == 256 ? (MODE == F8_GATE_UP ? 4 : 3) : 5;
+    static constexpr int STAGES = PAIR ? 6 : NT == 256 ? (MODE == F8_GATE_UP ? 4 : 3) : 5;
     static constexpr int NB = NT == 256 ? 2 : 4;
-    static constexpr int BUFS = MODE == F8_GATE_UP ? 0 : NT == 256 ? 2 : 1; /* a warp's staging buffers of 32 rows x 128 bytes */
-    static constexpr int OUT = F8_EPI_WARPS * BUFS * 4096;
+    static constexpr int BUFS = NT == 256 ? 2 : 1; /* a warp's staging buffers of 32 rows x 128 bytes */
+    static constexpr int OUT = F8_EPI_WARPS * (MODE == F8_GATE_UP ? 0 : PAIR ? 2048 : BUFS * 4096);
     static constexpr int SMEM = STAGES * STAGE + OUT + 1024 + (int)sizeof(f8_ctl_t);
 };
 
@@ -359,14 +398,14 @@ typedef struct {
     int e, r0, rows, n0;
 } f8_tile_t;
 
-template <int MODE, int NT>
+template <int MODE, int NT, int ROWS>
 __device__ __forceinline__ f8_tile_t f8_tile(const f8_args_t &P, int it, int n_tiles) {
     f8_tile_t t;
     if (MODE == F8_DENSE) { /* rows first: tiles in flight at the same time share rows of b */
-        const int mt = (P.m + 127) / 128, nt = it / mt;
+        const int mt = (P.m + ROWS - 1) / ROWS, nt = it / mt;
         t.e = 0;
-        t.r0 = (it - nt * mt) * 128;
-        t.rows = min(128, P.m - t.r0);
+        t.r0 = (it - nt * mt) * ROWS;
+        t.rows = min(ROWS, P.m - t.r0);
         t.n0 = nt * NT;
     } else {
         const int g = it / n_tiles;
@@ -435,16 +474,56 @@ __device__ __forceinline__ void f8_st32(void *p, const uint32_t *w) {
                  : "memory");
 }
 
+/* A warp's 32 rows of BYTES bytes through 2 KB of shared memory, 64 bytes of a row at a time (the 16-byte piece q of row r at
+ * q ^ (r / 2) % 4, so that neither side has bank conflicts): they leave as runs of 64 bytes.  Arguments as f8_rows_out's; vec:
+ * rows are 16-byte aligned. */
+template <int BYTES>
+__device__ __forceinline__ void f8_runs_out(uint32_t buf, const uint32_t *w, uint8_t *row0, int64_t stride, int rows, int left, int elem, int vec) {
+    const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+    for (int c = 0; c < BYTES / 64; c++) {
+        __syncwarp();
+#pragma unroll
+        for (uint32_t q = 0; q < 4; q++)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 64u + ((q ^ ((lane >> 1) & 3u)) << 4)), "r"(w[16 * c + 4 * q]),
+                         "r"(w[16 * c + 4 * q + 1]), "r"(w[16 * c + 4 * q + 2]), "r"(w[16 * c + 4 * q + 3])
+                         : "memory");
+        __syncwarp();
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const int r = (int)(8 * i + (lane >> 2)), at = 64 * c + 16 * (int)(lane & 3);
+            const uint4 v = fb_lds128(buf + r * 64u + (((lane & 3u) ^ ((r >> 1) & 3u)) << 4));
+            if (r >= rows || at >= left) continue;
+            uint8_t *to = row0 + r * stride + at;
+            if (vec && at + 16 <= left) {
+                *reinterpret_cast<uint4 *>(to) = v;
+            } else {
+                const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (elem == 4) {
+                        if (at + 4 * k < left) *reinterpret_cast<uint32_t *>(to + 4 * k) = x[k];
+                    } else {
+                        if (at + 4 * k < left) *reinterpret_cast<uint16_t *>(to + 4 * k) = (uint16_t)x[k];
+                        if (at + 4 * k + 2 < left) *reinterpret_cast<uint16_t *>(to + 4 * k + 2) = (uint16_t)(x[k] >> 16);
+                    }
+                }
+            }
+        }
+    }
+}
+
 /* the warp's boxes have left its staging buffers */
 __device__ __forceinline__ void f8_box_wait() {
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
 }
 
-template <int MODE, int NT, bool SPLIT>
+template <int MODE, int NT, int KIND>
 __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant__ f8_args_t P) {
-    typedef f8_cfg<MODE, NT> cfg;
-    constexpr int STAGES = cfg::STAGES, NB = cfg::NB;
+    typedef f8_cfg<MODE, NT, KIND> cfg;
+    constexpr int STAGES = cfg::STAGES, NB = cfg::NB, ROWS = cfg::ROWS;
+    constexpr bool PAIR = cfg::PAIR, SPLIT = cfg::SPLIT;
     extern __shared__ uint8_t dyn_raw[];
     const uint32_t dyn_u = (fb_smem_u32(dyn_raw) + 1023u) & ~1023u;
     const uint32_t out_u = dyn_u + STAGES * cfg::STAGE;
@@ -454,10 +533,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
     const int n_tiles = (P.n + per_n - 1) / per_n;
     if (MODE != F8_DENSE) f8_next();
     /* this block's blocks of k: all, or (SPLIT) its rank's share; the cluster's blocks have one tile */
-    const uint32_t ranks = SPLIT ? f8_cluster_size() : 1, rank = SPLIT ? f8_cluster_rank() : 0;
-    const int kb_all = (P.k + 127) / 128, kb_lo = (int)(rank * kb_all / ranks), kbs = (int)((rank + 1) * kb_all / ranks) - kb_lo;
+    const uint32_t ranks = SPLIT ? f8_cluster_size() : PAIR ? 2 : 1, rank = KIND != F8_ONE ? f8_cluster_rank() : 0;
+    const int kb_all = (P.k + 127) / 128, kb_lo = SPLIT ? (int)(rank * kb_all / ranks) : 0;
+    const int kbs = SPLIT ? (int)((rank + 1) * kb_all / ranks) - kb_lo : kb_all;
     const int first = (int)(blockIdx.x / ranks), stride = (int)(gridDim.x / ranks);
-    int tiles = MODE == F8_DENSE ? (P.m + 127) / 128 * n_tiles : 0;
+    const int up = PAIR ? 128 * (int)rank : 0; /* where this SM's rows of a tile begin */
+    int tiles = MODE == F8_DENSE ? (P.m + ROWS - 1) / ROWS * n_tiles : 0;
 
     if (tid == 0) {
         for (int s = 0; s < STAGES; s++) {
@@ -466,7 +547,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
         }
         for (int b = 0; b < NB; b++) {
             fb_mbar_init(fb_smem_u32(&C->acc_full[b]), 1);
-            fb_mbar_init(fb_smem_u32(&C->acc_empty[b]), F8_EPI_WARPS);
+            fb_mbar_init(fb_smem_u32(&C->acc_empty[b]), PAIR ? 2 * F8_EPI_WARPS : F8_EPI_WARPS);
         }
         for (int g = 0; g < 2; g++) {
             fb_mbar_init(fb_smem_u32(&C->sc_full[g]), 2);
@@ -476,13 +557,21 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
         fb_mbar_init_fence();
     }
     if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fb_smem_u32(&C->tmem_base)),
-                     "r"((uint32_t)(NB * NT))
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fb_smem_u32(&C->tmem_base)),
+                         "r"((uint32_t)(NB * NT))
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fb_smem_u32(&C->tmem_base)),
+                         "r"((uint32_t)(NB * NT))
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    if (PAIR) f8_cluster_sync();
+    else __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = C->tmem_base;
     if (MODE != F8_DENSE) f8_after();
@@ -496,10 +585,11 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             uint32_t st = 0, ph = 0; /* stage, and the parity of its phase */
             bool ok = true;
             for (int it = first; it < tiles && ok; it += stride) {
-                const f8_tile_t t = f8_tile<MODE, NT>(P, it, n_tiles);
+                const f8_tile_t t = f8_tile<MODE, NT, ROWS>(P, it, n_tiles);
                 /* boxes of 32 rows, as many as the rows need; what is behind the tile's rows is never stored */
-                const int groups = (t.rows + 31) / 32, y = t.e * P.b_rec_rows + t.n0;
-                const uint32_t bytes = (uint32_t)groups * 4096u + cfg::B_BYTES;
+                const int groups = PAIR ? min(4, max(0, (t.rows - up + 31) / 32)) : (t.rows + 31) / 32;
+                const int y = t.e * P.b_rec_rows + t.n0 + (!PAIR || rank == 0 ? 0 : MODE == F8_GATE_UP ? P.n : NT / 2);
+                const uint32_t bytes = (uint32_t)((t.rows + 31) / 32) * 4096u + (PAIR ? 2u : 1u) * cfg::B_BYTES; /* of both SMs */
                 for (int kb = 0; kb < kbs; kb++) {
                     const uint32_t a_u = dyn_u + st * cfg::STAGE, b_u = a_u + F8_A_BYTES;
                     if (!f8_wait_all(fb_smem_u32(&C->empty[st]), ph ^ 1, C)) {
@@ -507,12 +597,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                         break;
                     }
                     if (f8_elect()) {
-                        const uint32_t bar = fb_smem_u32(&C->full[st]);
+                        const uint32_t own = fb_smem_u32(&C->full[st]), bar = PAIR ? f8_leader(own) : own;
                         const int x = (kb_lo + kb) * 128;
-                        fb_mbar_expect_tx(bar, bytes);
-                        f8_tma2(b_u, &P.tb, x, y, bar);
-                        if (MODE == F8_GATE_UP) f8_tma2(b_u + 16384u, &P.tb, x, y + P.n, bar);
-                        for (int g = 0; g < groups; g++) f8_tma2(a_u + g * 4096u, &P.ta, x, t.r0 + 32 * g, bar);
+                        if (!PAIR || rank == 0) fb_mbar_expect_tx(own, bytes);
+                        f8_tma2<PAIR>(b_u, &P.tb, x, y, bar);
+                        if (MODE == F8_GATE_UP && !PAIR) f8_tma2<PAIR>(b_u + 16384u, &P.tb, x, y + P.n, bar);
+                        for (int g = 0; g < groups; g++) f8_tma2<PAIR>(a_u + g * 4096u, &P.ta, x, t.r0 + up + 32 * g, bar);
                     }
                     __syncwarp();
                     if (++st == STAGES) {
@@ -529,9 +619,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     ph ^= 1;
                 }
             }
-        } else if (warp == 9) {
-            /* ---------------- MMAs: one thread */
-            const uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        } else if (warp == 9 && (!PAIR || rank == 0)) {
+            /* ---------------- MMAs: one thread, in a pair one for both SMs */
+            const uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
             uint32_t st = 0, ph = 0, b = 0, bph = 0, have_ab = 0, have_acc = 0;
             bool ok = true;
             for (int it = first; it < tiles && ok; it += stride)
@@ -546,9 +636,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     if (f8_elect()) {
 #pragma unroll
                         for (int q = 0; q < 4; q++)
-                            f8_mma(tmem + b * NT, f8_desc(a_u + 32 * q), f8_desc(b_u + 32 * q), idesc, q > 0);
-                        f8_commit(fb_smem_u32(&C->acc_full[b]));
-                        f8_commit(fb_smem_u32(&C->empty[st]));
+                            f8_mma<PAIR>(tmem + b * NT, f8_desc(a_u + 32 * q), f8_desc(b_u + 32 * q), idesc, q > 0);
+                        f8_commit<PAIR>(fb_smem_u32(&C->acc_full[b]));
+                        f8_commit<PAIR>(fb_smem_u32(&C->empty[st]));
                     }
                     __syncwarp();
                     if (++st == STAGES) {
@@ -569,9 +659,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             uint32_t g = 0;
             bool ok = true;
             for (int it = first; it < tiles && ok; it += stride) {
-                const f8_tile_t t = f8_tile<MODE, NT>(P, it, n_tiles);
-                const float *a0 = P.a_scales + (int64_t)(t.r0 + min(i, t.rows - 1)) * P.as_stride;
-                const float *a1 = P.a_scales + (int64_t)(t.r0 + min(i + 64, t.rows - 1)) * P.as_stride;
+                const f8_tile_t t = f8_tile<MODE, NT, ROWS>(P, it, n_tiles);
+                const float *a0 = P.a_scales + (int64_t)(t.r0 + min(up + i, t.rows - 1)) * P.as_stride;
+                const float *a1 = P.a_scales + (int64_t)(t.r0 + min(up + i + 64, t.rows - 1)) * P.as_stride;
                 const float *rec = P.b_scales + (int64_t)t.e * P.bs_rec;
                 const float *b0 = rec + (int64_t)(min(t.n0, P.n - 1) >> 7) * P.bs_stride;
                 const float *b1 = rec + (int64_t)((MODE == F8_GATE_UP ? P.n + t.n0 : min(t.n0 + NT / 2, P.n - 1)) >> 7) * P.bs_stride;
@@ -580,8 +670,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
 #pragma unroll
                     for (int q = 0; q < F8_SC; q++) {
                         const int k = kb_lo + min(kb + q, kbs - 1);
-                        va[0][q] = __ldcg(a0 + k); /* (the kernel before this one may have written them as this one started) */
-                        va[1][q] = __ldcg(a1 + k);
+                        va[0][q] = a0[k]; /* (no __ldg: the kernel before this one may have written them as this one started) */
+                        va[1][q] = a1[k];
                         vb[0][q] = __ldg(b0 + k);
                         vb[1][q] = __ldg(b1 + k);
                     }
@@ -609,8 +699,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
         uint32_t step = 0, cnt = 0, grp = 0, have = 0;
         bool ok = true;
         for (int it = first; it < tiles; it += stride, cnt++) {
-            const f8_tile_t t = f8_tile<MODE, NT>(P, it, n_tiles);
-            const int c0 = t.n0 + (MODE == F8_GATE_UP ? 0 : wg * W); /* first row of b of this thread's columns */
+            f8_tile_t t = f8_tile<MODE, NT, ROWS>(P, it, n_tiles);
+            t.r0 += up, t.rows -= up; /* of this SM (a pair's second may have none) */
             float2 acc[W / 2];
 #pragma unroll
             for (int i = 0; i < W / 2; i++) acc[i] = make_float2(0.0f, 0.0f);
@@ -654,7 +744,10 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     } else { /* the buffer has been read: the next block's MMAs may have it */
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) fb_mbar_arrive(fb_smem_u32(&C->acc_empty[b]));
+                        if (lane == 0) {
+                            if (PAIR) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(f8_leader(fb_smem_u32(&C->acc_empty[b]))) : "memory");
+                            else fb_mbar_arrive(fb_smem_u32(&C->acc_empty[b]));
+                        }
                         if (kb + 1 < kbs) {
                             if (!__all_sync(FULL, have)) ok = f8_wait_all(fb_smem_u32(&C->acc_full[(step + 1) % NB]), ((step + 1) / NB) & 1, C);
                             if (ok) {
@@ -673,7 +766,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     if (c == CH - 2) have = f8_look(fb_smem_u32(&C->acc_full[(step + 1) % NB]), ((step + 1) / NB) & 1);
                 }
             }
-            const uint32_t buf = out_u + warp * (uint32_t)(cfg::BUFS * 4096);
+            const uint32_t buf = out_u + warp * (uint32_t)(cfg::OUT / F8_EPI_WARPS);
             if (MODE == F8_GATE_UP) {
                 /* silu(g) u of this thread's 64 columns, and the amax over the row's 128 with the other warpgroup's */
                 float amax = 0.0f;
@@ -712,7 +805,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             } else {
                 /* rows of this warp that are the tile's; a box may only leave whole if none of its rows is another expert's */
                 const int w0 = (warp & 3) * 32, rows = ok ? max(0, min(32, t.rows - w0)) : 0, c0 = t.n0 + wg * W;
-                const bool tma = P.out_tma && (MODE == F8_DENSE ? rows > 0 : rows == 32);
+                const bool tma = !PAIR && P.out_tma && (MODE == F8_DENSE ? rows > 0 : rows == 32);
                 uint32_t w[W / 2];
                 if (MODE == F8_DOWN || P.out_bf16) {
                     if constexpr (MODE == F8_DOWN) {
@@ -738,6 +831,11 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                             w[i] = *reinterpret_cast<const uint32_t *>(&v);
                         }
                     }
+                    if (PAIR) {
+                        f8_runs_out<2 * W>(buf, w, reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + w0) * P.out_stride + c0),
+                                           2 * P.out_stride, rows, 2 * (P.n - c0), 2, P.out_tma);
+                        continue;
+                    }
                     if (MODE == F8_DOWN && !tma) { /* (61 tokens of 8 in 256 experts: 150 us by staged rows, 133 so) */
                         if (lane < rows && c0 < P.n) {
                             uint8_t *o = reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + row) * P.out_stride + c0);
@@ -759,6 +857,10 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                             f8_rows_out(buf + c * 4096u, reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + w0) * P.out_stride + x),
                                         2 * P.out_stride, rows, 2 * (P.n - x), 2);
                     }
+                } else if (PAIR) {
+                    f8_runs_out<4 * W>(buf, reinterpret_cast<const uint32_t *>(acc),
+                                       reinterpret_cast<uint8_t *>(P.out) + 4 * ((int64_t)(t.r0 + w0) * P.out_stride + c0),
+                                       4 * P.out_stride, rows, 4 * (P.n - c0), 4, P.out_tma);
                 } else {
 #pragma unroll
                     for (int c = 0; c < W / 32; c++) { /* boxes of 32 columns, through the buffers there are */
@@ -776,7 +878,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                 }
             }
         }
-        if (MODE != F8_GATE_UP && !SPLIT) f8_box_wait(); /* the staging buffers go away with the block */
+        if (MODE != F8_GATE_UP && KIND == F8_ONE) f8_box_wait(); /* the staging buffers go away with the block */
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -788,7 +890,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
     if (SPLIT) {
         /* the parts meet: rank r sums rows r, r + ranks, ... in rank order, a warp a row */
         f8_cluster_sync();
-        const f8_tile_t t = f8_tile<MODE, NT>(P, first, n_tiles);
+        const f8_tile_t t = f8_tile<MODE, NT, ROWS>(P, first, n_tiles);
         for (int row = (int)rank + (int)ranks * warp; row < t.rows; row += (int)ranks * (F8_THREADS / 32)) {
             const uint32_t at = dyn_u + row * 512u + (((uint32_t)lane ^ (row & 31u)) << 4);
             float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -828,9 +930,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
         }
         f8_cluster_sync(); /* nobody leaves while its part is being read */
     }
-    __syncthreads();
-    if (warp == 9)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(NB * NT)) : "memory");
+    if (PAIR) f8_cluster_sync(); /* neither SM goes while the other's MMAs or arrivals may reach it */
+    else __syncthreads();
+    if (warp == 9) {
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(NB * NT)) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(NB * NT)) : "memory");
+    }
 }
 
 /* ------------------------------------------------------------------ few rows: the weights' bytes are all that counts
@@ -1182,32 +1287,40 @@ static int f8_map(CUtensorMap *m, const void *p, uint64_t k, uint64_t rows, uint
                : (int)cudaErrorInvalidValue;
 }
 
-template <int MODE, int NT, bool SPLIT>
-static int f8_launch(f8_args_t &p, int64_t most_tiles, int ranks, int n_sm, int *launches, cudaStream_t st) {
+/* most_tiles: no more than this; at_once: tiles that the device works at at the same time */
+template <int MODE, int NT, int KIND>
+static int f8_launch(f8_args_t &p, int64_t most_tiles, int ranks, int at_once, int *launches, cudaStream_t st) {
     cudaLaunchConfig_t c = {};
-    cudaLaunchAttribute at[1] = {};
-    c.gridDim = dim3((unsigned)(SPLIT ? most_tiles * ranks : most_tiles < n_sm ? most_tiles : n_sm));
+    cudaLaunchAttribute at[2] = {};
+    c.gridDim = dim3((unsigned)((KIND == F8_SPLIT || most_tiles < at_once ? most_tiles : at_once) * ranks));
     c.blockDim = dim3(F8_THREADS);
-    c.dynamicSmemBytes = f8_cfg<MODE, NT>::SMEM;
+    c.dynamicSmemBytes = f8_cfg<MODE, NT, KIND>::SMEM;
     c.stream = st;
-    if (SPLIT) {
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = ranks;
-        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    } else if (MODE != F8_DENSE) {
-        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[0].val.programmaticStreamSerializationAllowed = 1;
+    if (KIND != F8_ONE) {
+        at[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        at[c.numAttrs].val.clusterDim.x = ranks;
+        at[c.numAttrs].val.clusterDim.y = at[c.numAttrs].val.clusterDim.z = 1;
+        c.numAttrs++;
+    }
+    if (MODE != F8_DENSE) {
+        at[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[c.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        c.numAttrs++;
     }
     c.attrs = at;
-    c.numAttrs = SPLIT || MODE != F8_DENSE ? 1 : 0;
     *launches += 1;
-    const cudaError_t rc = cudaLaunchKernelEx(&c, k_f8_mma<MODE, NT, SPLIT>, p);
+    const cudaError_t rc = cudaLaunchKernelEx(&c, k_f8_mma<MODE, NT, KIND>, p);
     return (int)(rc != cudaSuccess ? rc : cudaGetLastError());
 }
 
-#define F8_KB256 0.53 /* 64 x 4096 x 4096 in tiles of 256: 22.3 us, 64 x 8192 x 1024: 9.8 us */
-#define F8_KB128 0.33 /* in tiles of 128: 15.7 and 7.9 us */
-#define F8_MEET 2.2   /* 64 x 4096 x 4096 split over 2: 12.7 us, over 4: 10.7 us */
+/* Microseconds of a tile: so much a block of k and so much around them, fitted to k of 1024 and 4096 (4096 x 8192 x 4096 by
+ * pairs 136 us, by single SMs 148; 4096 x 4096 x 1024 29.5 and 28; 64 x 4096 x 4096 in tiles of 256 columns 22, of 128 15.7, of
+ * 128 split over 2 SMs 12.7, over 4 10.7; 640 x 4096 x 4096 split over 4, in five waves, 48). */
+#define F8_PAIR_US(kb) (0.517 * (kb) + 2.5)
+#define F8_256_US(kb) (0.56 * (kb) + 1.8)
+#define F8_128_US(kb) (0.33 * (kb) + 2.1)
+#define F8_SPLIT_US(kb) (0.33 * (kb) + 4.7)
+static double f8_waves(int64_t tiles, int at_once) { return (double)((tiles + at_once - 1) / at_once); }
 
 extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *status, const ops_device_t *d, int *launches,
                                     void *stream) {
@@ -1232,23 +1345,25 @@ extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *s
     p.status = status;
     cudaStream_t st = (cudaStream_t)stream;
     const int64_t m = a->m, n = a->n, mt = (m + 127) / 128;
-    /* Tiles of 256 columns read the least and take F8_KB256 a block of k, tiles of 128 columns F8_KB128 (microseconds, the
-     * serial time of the hand-overs); the blocks of k of few tiles are split over the ranks of a cluster, which costs the
-     * meeting.  The choice is the least of waves x blocks x time. */
-    const int64_t kb = (a->k + 127) / 128, t256 = mt * ((n + 255) / 256), t128 = mt * ((n + 127) / 128);
-    double best = (double)((t256 + n_sm - 1) / n_sm * kb) * F8_KB256;
-    int nt = 256, ranks = 1;
+    /* Two SMs on 256 x 256 read the least, one on 128 x 256 wastes fewer rows, tiles of 128 columns reach more SMs, and the
+     * blocks of k of few tiles are split over the SMs of a cluster: the least of waves x time of a tile. */
+    const int64_t kb = (a->k + 127) / 128, pairs = (m + 255) / 256 * ((n + 255) / 256), t256 = mt * ((n + 255) / 256), t128 = mt * ((n + 127) / 128);
+    double best = f8_waves(t256, n_sm) * F8_256_US(kb);
+    int nt = 256, ranks = 1, pair = 0;
     for (int i = 0, r = 1; i < 4 && r <= kb; i++, r *= 2) {
         if (d->clusters[i] < 1) continue;
-        const double c = (double)((t128 + d->clusters[i] - 1) / d->clusters[i] * ((kb + r - 1) / r)) * F8_KB128 + (r > 1 ? F8_MEET : 0.0);
+        const int64_t part = (kb + r - 1) / r;
+        const double c = f8_waves(t128, d->clusters[i]) * (r > 1 ? F8_SPLIT_US(part) : F8_128_US(part));
         if (c < best) best = c, nt = 128, ranks = r;
     }
-    int rc = f8_map(&p.ta, a->a, a->k, a->m, a->a_stride, 32) | f8_map(&p.tb, a->b, a->k, a->n, a->b_stride, nt);
+    if (d->clusters[1] > 0 && f8_waves(pairs, d->clusters[1]) * F8_PAIR_US(kb) < best) pair = 1, nt = 256;
+    int rc = f8_map(&p.ta, a->a, a->k, a->m, a->a_stride, 32) | f8_map(&p.tb, a->b, a->k, a->n, a->b_stride, pair ? 128 : nt);
     if (p.out_tma) rc |= f8_map(&p.to, a->out, (uint64_t)a->n * eb, a->m, (os + 15) & ~15ull, 32);
     if (rc) return rc;
-    return nt == 256    ? f8_launch<F8_DENSE, 256, false>(p, t256, 1, n_sm, launches, st)
-           : ranks == 1 ? f8_launch<F8_DENSE, 128, false>(p, t128, 1, n_sm, launches, st)
-                        : f8_launch<F8_DENSE, 128, true>(p, t128, ranks, n_sm, launches, st);
+    return pair         ? f8_launch<F8_DENSE, 256, F8_PAIR>(p, pairs, 2, d->clusters[1], launches, st)
+           : nt == 256  ? f8_launch<F8_DENSE, 256, F8_ONE>(p, t256, 1, n_sm, launches, st)
+           : ranks == 1 ? f8_launch<F8_DENSE, 128, F8_ONE>(p, t128, 1, n_sm, launches, st)
+                        : f8_launch<F8_DENSE, 128, F8_SPLIT>(p, t128, ranks, n_sm, launches, st);
 }
 
 /* ------------------------------------------------------------------ the pairs' rows of x side by side: one warp a row
@@ -1398,8 +1513,8 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     /* no more tiles than this (the device knows how many there are).  Tiles of 32 rows, with more weights in flight and a
      * joining warp of each warpgroup, were tried for few pairs an expert: 61 tokens of 8 in 256 experts 155 us as with 128. */
     const int64_t tiles = w.n_pairs / 128 + recs;
-    if (!rc) rc = f8_launch<F8_GATE_UP, 256, false>(gu, tiles * (I / 128), 1, n_sm, launches, st);
-    if (!rc) rc = f8_launch<F8_DOWN, 256, false>(dn, tiles * ((H + 255) / 256), 1, n_sm, launches, st);
+    if (!rc) rc = f8_launch<F8_GATE_UP, 256, F8_ONE>(gu, tiles * (I / 128), 1, n_sm, launches, st);
+    if (!rc) rc = f8_launch<F8_DOWN, 256, F8_ONE>(dn, tiles * ((H + 255) / 256), 1, n_sm, launches, st);
     if (rc) return rc;
     const int vec = ((uintptr_t)a->out & 15) == 0 && (a->n_tokens == 1 || a->out_stride % 8 == 0);
     /* (the grid's y goes to 65535) */
@@ -1426,14 +1541,14 @@ extern "C" int ops_f8_init(ops_device_t *d) {
         f8_encode = (f8_encode_t)fn;
     }
 #define RK(k) rc |= (int)cudaFuncGetAttributes(&f, (k))
-#define RM(MODE, NT, SPLIT)                                                                                             \
-    rc |= (int)cudaFuncSetAttribute((k_f8_mma<MODE, NT, SPLIT>), cudaFuncAttributeMaxDynamicSharedMemorySize, f8_cfg<MODE, NT>::SMEM)
+#define RM(MODE, NT, KIND)                                                                                             \
+    rc |= (int)cudaFuncSetAttribute((k_f8_mma<MODE, NT, KIND>), cudaFuncAttributeMaxDynamicSharedMemorySize, f8_cfg<MODE, NT, KIND>::SMEM)
     RK(k_ops_combine); RK(k_ops_permute);
 #define RF(k, smem) rc |= (int)cudaFuncSetAttribute((k), cudaFuncAttributeMaxDynamicSharedMemorySize, (smem))
     RF(k_f8_few<1>, FR_SMEM); RF(k_f8_few<2>, FR_SMEM); RF(k_f8_few_gate_up, FG_SMEM); RF(k_f8_few_down, FD_SMEM_MOST);
 #undef RF
-    RM(F8_DENSE, 256, false); RM(F8_DENSE, 128, false); RM(F8_DENSE, 128, true); RM(F8_GATE_UP, 256, false);
-    RM(F8_DOWN, 256, false);
+    RM(F8_DENSE, 256, F8_PAIR); RM(F8_DENSE, 256, F8_ONE); RM(F8_DENSE, 128, F8_ONE); RM(F8_DENSE, 128, F8_SPLIT);
+    RM(F8_GATE_UP, 256, F8_ONE); RM(F8_DOWN, 256, F8_ONE);
 #undef RM
 #undef RK
     d->clusters[0] = d->n_sm;
@@ -1442,13 +1557,13 @@ extern "C" int ops_f8_init(ops_device_t *d) {
         cudaLaunchAttribute at[1];
         c.gridDim = dim3(1u << i);
         c.blockDim = dim3(F8_THREADS);
-        c.dynamicSmemBytes = f8_cfg<F8_DENSE, 128>::SMEM;
+        c.dynamicSmemBytes = f8_cfg<F8_DENSE, 128, F8_SPLIT>::SMEM;
         at[0].id = cudaLaunchAttributeClusterDimension;
         at[0].val.clusterDim.x = 1u << i;
         at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
         c.attrs = at;
         c.numAttrs = 1;
-        rc |= (int)cudaOccupancyMaxActiveClusters(&d->clusters[i], k_f8_mma<F8_DENSE, 128, true>, &c);
+        rc |= (int)cudaOccupancyMaxActiveClusters(&d->clusters[i], k_f8_mma<F8_DENSE, 128, F8_SPLIT>, &c);
     }
     rc |= (int)cudaFuncSetAttribute(k_ops_bucket<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, OPS_MAX_E * (BK_WARPS + 1) * 4);
     rc |= (int)cudaFuncSetAttribute(k_ops_bucket<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, OPS_MAX_E * (BK_WARPS + 1) * 4);
