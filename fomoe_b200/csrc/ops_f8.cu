@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                 const f8_tile_t t = f8_tile<MODE, NT, ROWS>(P, it, n_tiles);
                 /* boxes of 32 rows, as many as the rows need; what is behind the tile's rows is never stored */
                 const int groups = PAIR ? min(4, max(0, (t.rows - up + 31) / 32)) : (t.rows + 31) / 32;
-                const int y = t.e * P.b_rec_rows + t.n0 + (!PAIR || rank == 0 ? 0 : MODE == F8_GATE_UP ? P.n : NT / 2);
+                const int y = t.e * P.b_rec_rows + t.n0 + (PAIR && rank ? NT / 2 : 0);
                 const uint32_t bytes = (uint32_t)((t.rows + 31) / 32) * 4096u + (PAIR ? 2u : 1u) * cfg::B_BYTES; /* of both SMs */
                 for (int kb = 0; kb < kbs; kb++) {
                     const uint32_t a_u = dyn_u + st * cfg::STAGE, b_u = a_u + F8_A_BYTES;
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                         const int x = (kb_lo + kb) * 128;
                         if (!PAIR || rank == 0) fb_mbar_expect_tx(own, bytes);
                         f8_tma2<PAIR>(b_u, &P.tb, x, y, bar);
-                        if (MODE == F8_GATE_UP && !PAIR) f8_tma2<PAIR>(b_u + 16384u, &P.tb, x, y + P.n, bar);
+                        if (MODE == F8_GATE_UP) f8_tma2<PAIR>(b_u + 16384u, &P.tb, x, y + P.n, bar);
                         for (int g = 0; g < groups; g++) f8_tma2<PAIR>(a_u + g * 4096u, &P.ta, x, t.r0 + up + 32 * g, bar);
                     }
                     __syncwarp();
@@ -1511,7 +1511,9 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
                              (const int *)counts, (const int *)pairs, n_routed, a->top_k, n_shared, ws + w.xp, (float *)(ws + w.xp_scales));
     *launches += 2;
     /* no more tiles than this (the device knows how many there are).  Tiles of 32 rows, with more weights in flight and a
-     * joining warp of each warpgroup, were tried for few pairs an expert: 61 tokens of 8 in 256 experts 155 us as with 128. */
+     * joining warp of each warpgroup, were tried for few pairs an expert: 61 tokens of 8 in 256 experts 155 us as with 128;
+     * tiles of 256 by pairs of SMs for many: 8192 tokens of 8 + 1 in 64 experts 1.59 ms under the power cap, 1.55 with 128,
+     * half a tile of every expert being padding. */
     const int64_t tiles = w.n_pairs / 128 + recs;
     if (!rc) rc = f8_launch<F8_GATE_UP, 256, F8_ONE>(gu, tiles * (I / 128), 1, n_sm, launches, st);
     if (!rc) rc = f8_launch<F8_DOWN, 256, F8_ONE>(dn, tiles * ((H + 255) / 256), 1, n_sm, launches, st);
