@@ -943,9 +943,10 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
  * (blocks of k; of all slots of a token for the down product) w, w + 8, ..., and the eight partial sums meet in shared
  * memory, in warp order.  A unit, 16 rows x 128 k, goes to the registers of mma.sync (m16n8k32, e4m3: the weight rows are
  * its 16 rows, the activations its columns) through a ring of FR_RING units a warp: each lane copies (cp.async) exactly the
- * four 16-byte pieces that it will read, so no lane waits for another, and 192 KB an SM are in flight all the time.  The k
- * inside a block come in the order that this gives: lane (g, t) holds bytes 16 t .. of rows g and g + 8, the activations
- * likewise.  16 weight rows a block spread small matrices over all SMs, and nothing has to be set up first. */
+ * four 16-byte pieces that it will read, so no lane waits for another.  The k inside a block come in the order that this
+ * gives: lane (g, t) holds bytes 16 t .. of rows g and g + 8, the activations likewise.  16 weight rows a block spread small
+ * matrices over all SMs, and nothing has to be set up first: 1 x 4096 x 4096 5.4 us (on tcgen05 11), 16 rows 7.4, 1 x 8192 x
+ * 8192 16 us, 1 x 4096 x 16,384 14.5 us, 4.6 TB/s; start and end of a block are what is left. */
 #define FR_WARPS 8
 #define FR_RING 2
 #define FR_SMEM (FR_WARPS * FR_RING * 2048)
@@ -1106,7 +1107,9 @@ __device__ __forceinline__ int fr_expert(const fr_experts_t &P, int t, int j) {
 
 /* act[pair][128 rows] = silu(gate x) (up x) in FP8; block (128 rows, slot, token) of 16 warps: warp w has rows
  * 16 (w % 8) .. of the 128 and every other block of k, both matrices.  One block holds a whole block of activations, so its
- * amax meets in shared memory; 192 KB an SM are in flight from the start to the end of a block. */
+ * amax meets in shared memory; 192 KB an SM are in flight from the start to the end of a block.  (One token with 11 experts of
+ * 4096 x 1024: 21 us, 4.3 TB/s from 88 blocks.  Blocks of 64 rows in clusters of two that tell one another their amax, 176 of
+ * them: 28 us, two share an SM.) */
 #define FG_WARPS 16
 #define FG_RING 6
 #define FG_SMEM (FG_WARPS * FG_RING * 2048)

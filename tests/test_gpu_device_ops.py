@@ -627,3 +627,30 @@ def test_handle_dropped_while_capturing(ops, fb):
     torch.cuda.synchronize()
     want = ops.f8_quantize(x)
     assert (q.view(torch.uint8) == want[0].view(torch.uint8)).all() and (s == want[1]).all()
+
+
+# sizes whose tiles two SMs share: the second without rows, with some, with all; odd columns, a last block of k that is short
+@pytest.mark.parametrize("M,N,K", [(700, 3500, 2560), (630, 4001, 4080), (513, 4000, 4080), (2049, 1025, 4096)])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_matmul_by_pairs(ops, M, N, K, out):
+    from fomoe_b200.device_ops import MatmulArgs
+    g = gen(M + N + K)
+    a, sa = ops.f8_quantize(randn(g, M, K))
+    b, sb = f8_table(g, N, K)
+    c = ops.f8_matmul(a, sa, b, sb, out=out)
+    A, B = rows64(a, sa), mat64(b, sb)
+    want, size = A @ B.T, A.abs() @ B.abs().T
+    # (test_matmul's bound)
+    tol = (K // 128 + 1 + 130) * U * size + HALF[c.dtype] * want.abs() + 1e-40
+    within(c, want, tol)
+    if out == "f32":
+        assert float((c.double() - want).norm() / want.norm()) < 2e-6
+    # inside a larger buffer whose rows are not aligned: the same values, and nothing beside them
+    big = torch.full((M + 2, N + 7), 7.0, device="cuda", dtype=c.dtype)
+    o = big[1:1 + M, 3:3 + N]
+    args = MatmulArgs(M, N, K, a.data_ptr(), K, sa.data_ptr(), sa.stride(0), b.data_ptr(), K, sb.data_ptr(), sb.stride(0),
+                      o.data_ptr(), 1 if out == "bf16" else 0, o.stride(0))
+    ops._ck(ops._l.fomoe_b200_ops_f8_matmul(ops._h, args, torch.cuda.current_stream().cuda_stream), "matmul")
+    assert (o == c).all()
+    o.fill_(7.0)
+    assert (big == 7.0).all()
