@@ -48,8 +48,7 @@ static int f8_launch_after(void (*k)(P...), dim3 grid, int threads, int smem, cu
  * over (expert, block, warp) give every warp its first place, a second walk places the pairs.  The order inside an expert is
  * the order of the pairs, so results do not depend on timing.  The shared expert's pairs (n_routed + t) come last.  With more
  * than one block a first launch (COUNT) leaves each block's counts in `block_counts`.  Eight ids a lane are in flight at
- * once.  (65,536 pairs in 64 experts: one block 150 us, eight ids
- * a lane 100 us, bound by one SM's scattered stores; by 16 blocks in two launches 19 us.) */
+ * once.  (65,536 pairs in 64 experts: one block 150 us, eight ids a lane 100 us, bound by one SM's scattered stores; by 16 blocks in two launches 19 us.) */
 #define BK_THREADS 1024
 #define BK_WARPS 32
 #define BK_AHEAD 8
@@ -186,12 +185,12 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
  * rows, 32 KB a block of k instead of 48, one thread of the first issues the MMAs of both, and each joins its own rows.  Six
  * stages leave 2 KB of staging a warp, so rows leave in runs of 64 bytes by plain stores.
  *
- * What bounds it (4096 x 8192 x 4096): one SM a tile 148 us, 1.86 PFLOP/s -- the MMAs with nothing but their barriers take 121
- * us, the operands of 128 x 256 tiles pass shared memory twice, 192 bytes a cycle at the tensor cores' full rate; the joining
- * FMAs and the way out are the rest --, pairs 136 us, 2.02 PFLOP/s (their bare MMAs 102).  Under the power cap, where a long
- * step runs, 177 and 159 us at 1.66 GHz.  With four stages and TMA stores out pairs took 179 us there, with stores of
- * 32 bytes from registers 172.  Handing the columns over in two halves (180 us) and 16 joining warps (158 us) were slower:
- * every barrier is shared-memory traffic too.
+ * What bounds it (4096 x 8192 x 4096): one SM a tile 144.5 us, 1.90 PFLOP/s -- the MMAs with nothing but their barriers take
+ * 121 us, the operands of 128 x 256 tiles pass shared memory twice, 192 bytes a cycle at the tensor cores' full rate; the
+ * joining FMAs and the way out are the rest --, pairs 136 us, 2.02 PFLOP/s (their bare MMAs 102).  Under the power cap, where a
+ * long step runs, 175 and 159 us at 1.66 GHz.  Pairs with four stages and TMA stores out took 179 us there, with stores of 32
+ * bytes from registers 172, with runs of 64 bytes 166, all three with scales read past the L1: that alone costs 7 us.  Handing
+ * the columns over in two halves (180 us) and 16 joining warps (158 us) were slower: every barrier is shared-memory traffic too.
  *
  *   dense    A: rows of a;                               B: rows of b;                        D to out
  *   gate/up  A: the tokens of an expert's pairs;         B: 128 gate rows, 128 up rows;       silu(g) u to FP8, 128 a block
@@ -1317,7 +1316,7 @@ static int f8_launch(f8_args_t &p, int64_t most_tiles, int ranks, int at_once, i
 }
 
 /* Microseconds of a tile: so much a block of k and so much around them, fitted to k of 1024 and 4096 (4096 x 8192 x 4096 by
- * pairs 136 us, by single SMs 148; 4096 x 4096 x 1024 29.5 and 28; 64 x 4096 x 4096 in tiles of 256 columns 22, of 128 15.7, of
+ * pairs 136 us, by single SMs 144.5; 4096 x 4096 x 1024 29.5 and 28; 64 x 4096 x 4096 in tiles of 256 columns 22, of 128 15.7, of
  * 128 split over 2 SMs 12.7, over 4 10.7; 640 x 4096 x 4096 split over 4, in five waves, 48). */
 #define F8_PAIR_US(kb) (0.517 * (kb) + 2.5)
 #define F8_256_US(kb) (0.56 * (kb) + 1.8)
