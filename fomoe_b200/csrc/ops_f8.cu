@@ -48,7 +48,8 @@ static int f8_launch_after(void (*k)(P...), dim3 grid, int threads, int smem, cu
  * over (expert, block, warp) give every warp its first place, a second walk places the pairs.  The order inside an expert is
  * the order of the pairs, so results do not depend on timing.  The shared expert's pairs (n_routed + t) come last.  With more
  * than one block a first launch (COUNT) leaves each block's counts in `block_counts`.  Eight ids a lane are in flight at
- * once.  (65,536 pairs in 64 experts: one block 150 us, eight ids a lane 100 us, bound by one SM's scattered stores; by 16 blocks in two launches 19 us.) */
+ * once.  (65,536 pairs in 64 experts: one block 150 us, eight ids a lane 100 us, bound by one SM's scattered stores; by 16
+ * blocks in two launches 19 us.) */
 #define BK_THREADS 1024
 #define BK_WARPS 32
 #define BK_AHEAD 8
