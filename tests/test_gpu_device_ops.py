@@ -654,3 +654,40 @@ def test_matmul_by_pairs(ops, M, N, K, out):
     assert (o == c).all()
     o.fill_(7.0)
     assert (big == 7.0).all()
+
+
+def test_matmul_on_streams_at_once(ops):
+    """Products of every kind of tile on four streams at once, and replayed from two graphs at once: the bits of calls in turn."""
+    g = gen(77)
+    cases = []
+    for M, N, K in [(700, 3500, 2560), (640, 4001, 144), (200, 1000, 512), (64, 2048, 1040), (8, 4096, 512), (2049, 1025, 4096)]:
+        a, sa = ops.f8_quantize(randn(g, M, K))
+        cases.append((a, sa, *f8_table(g, N, K)))
+    want = [ops.f8_matmul(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for r in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                for j in range(len(cases)):
+                    k = (i + j + r) % len(cases)
+                    got.append((k, ops.f8_matmul(*cases[k])))
+    torch.cuda.synchronize()
+    for k, c in got:
+        assert (c.view(torch.uint8) == want[k].view(torch.uint8)).all()
+    graphs = []
+    for i in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(streams[i]):
+            with torch.cuda.graph(gr, stream=streams[i]):
+                o = [ops.f8_matmul(*c) for c in (cases if i else cases[::-1])]
+        graphs.append((gr, o if i else o[::-1]))
+    for _ in range(3):
+        for st, (gr, _) in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                gr.replay()
+    torch.cuda.synchronize()
+    for _, o in graphs:
+        for c, w in zip(o, want):
+            assert (c.view(torch.uint8) == w.view(torch.uint8)).all()
