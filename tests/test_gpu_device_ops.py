@@ -691,3 +691,28 @@ def test_matmul_on_streams_at_once(ops):
     for _, o in graphs:
         for c, w in zip(o, want):
             assert (c.view(torch.uint8) == w.view(torch.uint8)).all()
+
+
+@pytest.mark.parametrize("ratio", [2.0 ** -10, 2.0 ** -18, 2.0 ** -30])
+def test_experts_blocks_of_very_different_scales(ops, ratio):
+    """Outputs that only small-scaled blocks of a row reach, beside a block whose scale is far larger: an expert's output is
+    held to 2^-11 of itself or 2^-38 of the bound 128 448^2 sum |sa sb|, whichever is more."""
+    T, H, I, E = 257, 256, 256, 3
+    x, ids, w, gu, gus, dn, dns = make_experts(5, T, H, I, E, 1, False)
+    dns = dns.clone()
+    dns[:, :, 1] *= ratio
+    dn.view(torch.uint8)[:, ::2, :128] = 0
+    q, s = ops.f8_quantize(x)
+    y = ops.f8_experts(q, s, ids, w, gu, gus, dn, dns)
+    want, tol = experts64(q, s, ids, w, gu, gus, dn, dns, False)
+    top = torch.zeros_like(want)
+    for e in range(E):
+        t = torch.nonzero(ids[:, 0] == e)[:, 0]
+        z = rows64(q, s)[t] @ mat64(gu[e], gus[e]).T
+        act = z[:, :I] / (1 + torch.exp(-z[:, :I])) * z[:, I:]
+        sc = act.view(-1, 2, 128).abs().amax(2).clamp(min=TINY) / 448
+        top[t] = (sc @ dns[e].double().T).repeat_interleave(128, 1) * 128 * 448 ** 2
+    within(y, want, tol + w.double() * 2.0 ** -38 * top + 2.0 ** -11 * want.abs())
+    if ratio > 2.0 ** -20:   # and so the small ones are there at all
+        even = want[:, ::2]
+        assert float((y.double()[:, ::2] - even).norm() / even.norm()) < 0.02
