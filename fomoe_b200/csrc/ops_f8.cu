@@ -4,7 +4,6 @@
  */
 #include <cuda.h>
 #include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -195,7 +194,7 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
  *
  *   dense    A: rows of a;                               B: rows of b;                        D to out
  *   gate/up  A: the tokens of an expert's pairs;         B: 128 gate rows, 128 up rows;       silu(g) u to FP8, 128 a block
- *   down     A: the activations of an expert's pairs;    B: rows of its down matrix;          D as fp16 with a scale
+ *   down     A: the activations of an expert's pairs;    B: rows of its down matrix;          D in fp32
  *
  * Every wait is bounded; when one runs out the status word is set, all roles stop waiting and the block drains, frees its
  * tensor memory and returns. */
@@ -221,7 +220,6 @@ typedef struct {
     void *out;
     int out_bf16, out_tma; /* out_tma: rows of out are 16-byte aligned, D leaves as boxes */
     int64_t out_stride;
-    float *out_scales; /* F8_DOWN: [pairs][n / 128] */
     uint8_t *act_q; /* F8_GATE_UP: [pairs][n] */
     float *act_scales;
     const int *counts, *pairs;
@@ -717,7 +715,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             grp++;                                                                                   \
         }                                                                                            \
     } while (0)
-            float n0, n1 = 0.0f, fsum = 0.0f;
+            float n0, n1 = 0.0f;
             F8_FACTORS(0);
             /* Chunks of 32 columns through two register buffers: while one is joined the next is on its way, also across
              * blocks.  (gate/up: the first half of a thread's columns are the gate's, the second the up's) */
@@ -733,7 +731,6 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
             for (int kb = 0; kb < kbs; kb++, step++) {
                 const int b = step % NB;
                 const float f0 = n0, f1 = MODE == F8_GATE_UP ? n1 : n0;
-                if (MODE == F8_DOWN) fsum += fabsf(f0);
                 if (!ok) continue;
 #pragma unroll
                 for (int c = 0; c < CH; c++) {
@@ -806,42 +803,22 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                 /* rows of this warp that are the tile's; a box may only leave whole if none of its rows is another expert's */
                 const int w0 = (warp & 3) * 32, rows = ok ? max(0, min(32, t.rows - w0)) : 0, c0 = t.n0 + wg * W;
                 const bool tma = !PAIR && P.out_tma && (MODE == F8_DENSE ? rows > 0 : rows == 32);
-                uint32_t w[W / 2];
-                if (MODE == F8_DOWN || P.out_bf16) {
-                    if constexpr (MODE == F8_DOWN) {
-                        /* fp16 relative to a power of two: 2^-11 of a value, a sixteenth of the rounding to bf16 that the sum
-                         * over the experts ends with, at half of fp32's bytes both ways.  No sum of products passes
-                         * sum |sa sb| 128 448^2 = top: with that below 2^15 nothing overflows, and only values under 2^-28 of
-                         * top have fewer bits (steps of 2^-38 top).  (Looking for the row's largest value instead cost 600 of
-                         * 11,000 cycles a tile.) */
-                        const float top = fsum * (128.0f * 448.0f * 448.0f);
-                        const uint32_t e = min(max(__float_as_uint(top) >> 23, 15u) - 14u, 253u);
-                        const float down = __uint_as_float((254u - e) << 23);
+                if (MODE == F8_DOWN && !tma) { /* (61 tokens of 8 in 256 experts, as fp16: 150 us by staged rows, 133 so) */
+                    if (lane < rows && c0 < P.n) {
+                        float *o = reinterpret_cast<float *>(P.out) + (int64_t)(t.r0 + row) * P.out_stride + c0;
 #pragma unroll
-                        for (int i = 0; i < W / 2; i++) {
-                            const __half2 v = __floats2half2_rn(acc[i].x * down, acc[i].y * down);
-                            w[i] = *reinterpret_cast<const uint32_t *>(&v);
-                        }
-                        if (lane < rows && c0 < P.n)
-                            P.out_scales[(int64_t)(t.r0 + row) * (P.n >> 7) + (c0 >> 7)] = __uint_as_float(e << 23);
-                    } else {
+                        for (int i = 0; i < W / 8; i++) f8_st32(o + 8 * i, reinterpret_cast<const uint32_t *>(acc) + 8 * i);
+                    }
+                } else if (MODE == F8_DENSE && P.out_bf16) {
+                    uint32_t w[W / 2];
 #pragma unroll
-                        for (int i = 0; i < W / 2; i++) {
-                            const __nv_bfloat162 v = __floats2bfloat162_rn(acc[i].x, acc[i].y);
-                            w[i] = *reinterpret_cast<const uint32_t *>(&v);
-                        }
+                    for (int i = 0; i < W / 2; i++) {
+                        const __nv_bfloat162 v = __floats2bfloat162_rn(acc[i].x, acc[i].y);
+                        w[i] = *reinterpret_cast<const uint32_t *>(&v);
                     }
                     if (PAIR) {
                         f8_runs_out<2 * W>(buf, w, reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + w0) * P.out_stride + c0),
                                            2 * P.out_stride, rows, 2 * (P.n - c0), 2, P.out_tma);
-                        continue;
-                    }
-                    if (MODE == F8_DOWN && !tma) { /* (61 tokens of 8 in 256 experts: 150 us by staged rows, 133 so) */
-                        if (lane < rows && c0 < P.n) {
-                            uint8_t *o = reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + row) * P.out_stride + c0);
-#pragma unroll
-                            for (int i = 0; i < W / 16; i++) f8_st32(o + 32 * i, w + 8 * i);
-                        }
                         continue;
                     }
                     f8_box_wait();
@@ -1388,9 +1365,9 @@ __global__ void __launch_bounds__(256) k_ops_permute(const uint8_t *x, int64_t x
 
 /* ------------------------------------------------------------------ out[t] = sum over the slots, in slot order
  * A thread has 8 columns; a token's rows of dots lie where its pairs were bucketed. */
-__global__ void __launch_bounds__(256) k_ops_combine(const __half *dots, const float *dot_scales, const int *pos, const int *ids,
-                                                    const float *weights, int n_embd, int n_experts, int top_k, int n_routed,
-                                                    int has_shared, __nv_bfloat16 *out, int64_t out_stride, int vec) {
+__global__ void __launch_bounds__(256) k_ops_combine(const float *dots, const int *pos, const int *ids, const float *weights,
+                                                    int n_embd, int n_experts, int top_k, int n_routed, int has_shared,
+                                                    __nv_bfloat16 *out, int64_t out_stride, int vec) {
     const int t = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 8;
     f8_after();
     if (c >= n_embd) return;
@@ -1398,16 +1375,12 @@ __global__ void __launch_bounds__(256) k_ops_combine(const __half *dots, const f
     for (int j = 0; j < top_k + has_shared; j++) {
         const int p = j < top_k ? t * top_k + j : n_routed + t;
         if (j < top_k && (unsigned)ids[p] >= (unsigned)n_experts) continue;
-        const int64_t r = pos[p];
-        const float w = (j < top_k ? weights[p] : 1.0f) * dot_scales[r * (n_embd >> 7) + (c >> 7)];
-        const uint4 u = *reinterpret_cast<const uint4 *>(dots + r * n_embd + c);
-        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+        const float w = j < top_k ? weights[p] : 1.0f;
+        const float4 *d = reinterpret_cast<const float4 *>(dots + (int64_t)pos[p] * n_embd + c);
+        const float4 a = d[0], b = d[1];
+        const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x[i]));
-            v[2 * i] = fmaf(w, f.x, v[2 * i]);
-            v[2 * i + 1] = fmaf(w, f.y, v[2 * i + 1]);
-        }
+        for (int i = 0; i < 8; i++) v[i] = fmaf(w, x[i], v[i]);
     }
     __nv_bfloat16 *o = out + t * out_stride + c;
     if (vec) {
@@ -1449,8 +1422,7 @@ extern "C" void ops_experts_layout(const fomoe_b200_f8_experts_args_t *a, ops_ex
     PART(xp_scales, np * (a->n_embd / 128) * 4);
     PART(act_q, np * a->n_inter);
     PART(act_scales, np * (a->n_inter / 128) * 4);
-    PART(dots, np * a->n_embd * 2);
-    PART(dot_scales, np * (a->n_embd / 128) * 4);
+    PART(dots, np * a->n_embd * 4);
 #undef PART
     w->bytes = at;
 }
@@ -1487,10 +1459,10 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     dn.n = H, dn.k = I;
     dn.a_scales = gu.act_scales, dn.as_stride = I / 128;
     dn.b_scales = a->down_scales, dn.bs_stride = I / 128, dn.bs_rec = (int64_t)(H / 128) * (I / 128), dn.b_rec_rows = H;
-    dn.out = ws + w.dots, dn.out_stride = H, dn.out_tma = 1, dn.out_scales = (float *)(ws + w.dot_scales);
+    dn.out = ws + w.dots, dn.out_stride = H, dn.out_tma = 1;
     int rc = f8_map(&gu.ta, ws + w.xp, H, w.n_pairs, H, 32) | f8_map(&gu.tb, a->gate_up, H, recs * 2 * I, H, 128) |
              f8_map(&dn.ta, ws + w.act_q, I, w.n_pairs, I, 32) | f8_map(&dn.tb, a->down, I, recs * H, I, 256) |
-             f8_map(&dn.to, ws + w.dots, 2ull * H, w.n_pairs, 2ull * H, 32);
+             f8_map(&dn.to, ws + w.dots, 4ull * H, w.n_pairs, 4ull * H, 32);
     if (rc) return rc;
     int run = (n_routed + BK_BLOCKS - 1) / BK_BLOCKS;
     run = run < BK_RUN ? BK_RUN : run;
@@ -1525,9 +1497,9 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     /* (the grid's y goes to 65535) */
     for (int t0 = 0; t0 < a->n_tokens; t0 += 65535) {
         const int nt = a->n_tokens - t0 < 65535 ? a->n_tokens - t0 : 65535, p0 = t0 * a->top_k;
-        rc = f8_launch_after(k_ops_combine, dim3((H / 8 + 255) / 256, nt), 256, 0, st, (const __half *)(ws + w.dots),
-                             (const float *)(ws + w.dot_scales), (const int *)pos + p0, ids + p0, a->weights + p0, H, a->n_experts,
-                             a->top_k, n_routed + t0 - p0, a->has_shared, (__nv_bfloat16 *)a->out + t0 * a->out_stride, a->out_stride, vec);
+        rc = f8_launch_after(k_ops_combine, dim3((H / 8 + 255) / 256, nt), 256, 0, st, (const float *)(ws + w.dots),
+                             (const int *)pos + p0, ids + p0, a->weights + p0, H, a->n_experts, a->top_k, n_routed + t0 - p0,
+                             a->has_shared, (__nv_bfloat16 *)a->out + t0 * a->out_stride, a->out_stride, vec);
         if (rc) return rc;
         *launches += 1;
     }

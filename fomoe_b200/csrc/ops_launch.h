@@ -37,7 +37,7 @@ int ops_launch_f8_quantize(int rows, int cols, const void *x, int x_bf16, int64_
 
 /* Where the parts of the experts' workspace lie, in bytes from its start (all 256-byte aligned). */
 typedef struct {
-    uint64_t counts, block_counts, pairs, pos, xp, xp_scales, act_q, act_scales, dots, dot_scales, bytes;
+    uint64_t counts, block_counts, pairs, pos, xp, xp_scales, act_q, act_scales, dots, bytes;
     int n_pairs; /* routed and shared pairs */
 } ops_experts_ws_t;
 

@@ -491,8 +491,7 @@ int fomoe_b200_ops_f8_matmul(fomoe_b200_ops_t *ops, const fomoe_b200_f8_matmul_a
 /* The experts of one layer on FP8 rows, routing given:
  *     z = gate_up_e x,  act = silu(z[0 .. I)) * z[I .. 2 I)  (to FP8 per 128),  y_e = down_e act
  *     out[t] = sum_j weights[t][j] y_{ids[t][j]}  (in slot order)  + y_shared   (bf16)
- * Between the experts' products and the sum each y_e is held to 2^-11 of its value, or to 2^-38 of the bound 128 448^2
- * sum |scale scale| over its blocks where that is more.
+ * The products, each y_e and the sum over the experts are fp32.
  * ids of -1 are left out (as fomoe_b200_ops_route writes them); other ids outside 0 .. n_experts - 1 too, with status 1.
  * A token with no expert at all gets zeros.  The tables hold n_experts + has_shared contiguous records, the shared
  * expert last.  workspace: fomoe_b200_ops_f8_experts_workspace bytes, 256-byte aligned; its contents do not matter
