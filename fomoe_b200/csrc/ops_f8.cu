@@ -776,7 +776,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                 C->amax[cnt & 1][wg][row] = amax;
                 asm volatile("bar.sync 1, 256;" ::: "memory"); /* the 8 warps meet once a tile, also after a wait that ran out */
                 const float sc = ops_f8_scale(ops_amax(amax, C->amax[cnt & 1][wg ^ 1][row]));
-                const float inv = __frcp_rn(sc); /* (the values carry a few roundings already: one more, of the quotient, is theirs) */
+                const float inv = __frcp_rn(sc);
                 const bool mine = row < t.rows && ok;
                 if (mine) {
                     uint4 *q = reinterpret_cast<uint4 *>(P.act_q + (int64_t)(t.r0 + row) * P.n + t.n0 + wg * 64);
@@ -785,8 +785,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                         uint32_t w[4];
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            w[k] = ops_f8_pack4(acc[8 * i + 2 * k].x * inv, acc[8 * i + 2 * k].y * inv, acc[8 * i + 2 * k + 1].x * inv,
-                                                acc[8 * i + 2 * k + 1].y * inv);
+                            w[k] = ops_f8_pack4(ops_f8_quot(acc[8 * i + 2 * k].x, sc, inv), ops_f8_quot(acc[8 * i + 2 * k].y, sc, inv),
+                                                ops_f8_quot(acc[8 * i + 2 * k + 1].x, sc, inv), ops_f8_quot(acc[8 * i + 2 * k + 1].y, sc, inv));
                         q[i] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                     if (wg == 0) P.act_scales[(int64_t)(t.r0 + row) * (P.n >> 7) + (t.n0 >> 7)] = sc;
@@ -1172,7 +1172,8 @@ __global__ void __launch_bounds__(32 * FG_WARPS) k_f8_few_gate_up(const __grid_c
         for (int s = 16; s > 0; s >>= 1) amax = ops_amax(amax, __shfl_xor_sync(FULL, amax, s));
         const float sc = ops_f8_scale(amax), inv = __frcp_rn(sc);
         const int64_t row = (int64_t)t * (P.top_k + P.has_shared) + j;
-        *reinterpret_cast<uint32_t *>(P.act_q + row * I + n0 + 4 * lane) = ops_f8_pack4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        *reinterpret_cast<uint32_t *>(P.act_q + row * I + n0 + 4 * lane) =
+            ops_f8_pack4(ops_f8_quot(v.x, sc, inv), ops_f8_quot(v.y, sc, inv), ops_f8_quot(v.z, sc, inv), ops_f8_quot(v.w, sc, inv));
         if (lane == 0) P.act_scales[row * (I / 128) + (n0 >> 7)] = sc;
     }
 }
