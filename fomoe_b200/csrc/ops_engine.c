@@ -63,11 +63,9 @@ fomoe_b200_ops_t *fomoe_b200_ops_create(int device) {
     return o;
 }
 
-void fomoe_b200_ops_destroy(fomoe_b200_ops_t *o) {
-    if (!o) return;
-    cudaFreeHost((void *)o->status);
-    free(o);
-}
+/* The status words stay for the life of the process: calls in flight and graphs that hold some of this handle's go on
+ * storing into them.  They are no later handle's either, which would hear of what is not its own. */
+void fomoe_b200_ops_destroy(fomoe_b200_ops_t *o) { free(o); }
 
 const char *fomoe_b200_ops_last_error(fomoe_b200_ops_t *o) { return o ? o->err : "no handle"; }
 

@@ -77,7 +77,7 @@ class DeviceOps:
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
     def close(self):
-        """Release the handle; none of its calls may still be in flight."""
+        """Release the handle.  Calls in flight and graphs that hold its calls may outlive it; their status is lost."""
         if getattr(self, "_h", None):
             self._l.fomoe_b200_ops_destroy(self._h)
             self._h = None

@@ -400,7 +400,9 @@ typedef struct fomoe_b200_ops fomoe_b200_ops_t;
 #define FOMOE_B200_F8 2
 
 fomoe_b200_ops_t *fomoe_b200_ops_create(int device);
-void fomoe_b200_ops_destroy(fomoe_b200_ops_t *ops); /* none of its calls may still be in flight */
+/* Calls in flight and graphs that hold the handle's calls may outlive it (nothing tells their status any more): its 64 bytes
+ * of page-locked status words are never freed, so a program makes one handle a device and keeps it. */
+void fomoe_b200_ops_destroy(fomoe_b200_ops_t *ops);
 const char *fomoe_b200_ops_last_error(fomoe_b200_ops_t *ops);
 /* What went wrong on the device since the last call of this function (as far as the device has got: synchronise first
  * for what is in flight): 0 nothing, 1 an expert id outside the table (its pair was left out), 2 a kernel gave a bounded
