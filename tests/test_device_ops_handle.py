@@ -4,6 +4,7 @@ import ctypes as C
 import gc
 import os
 import subprocess
+import types
 
 import pytest
 import torch
@@ -62,3 +63,18 @@ def test_captured_calls_outlive_their_handle(make, fake, how):
     product(after)
     fake.fake_goes_wrong(1)
     assert after.status() == 1
+
+
+def test_a_handle_goes_without_touching_the_device(make):
+    """Whoever drops it, wherever: a wait would end a capture of another thread or stream."""
+    o = make()
+    asked = []
+
+    class Cuda(types.SimpleNamespace):
+        def __getattr__(self, name):
+            asked.append(name)
+            return lambda *a: False
+    o._t = types.SimpleNamespace(cuda=Cuda())
+    del o
+    gc.collect()
+    assert asked == []
