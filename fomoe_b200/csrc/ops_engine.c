@@ -16,7 +16,7 @@
 struct fomoe_b200_ops {
     int device;
     ops_device_t dev;
-    volatile int *status; /* mapped host memory: kernels store into it, the host reads it without a copy */
+    int *status; /* OPS_STATUS_WORDS of mapped host memory: kernels store into them, the host reads them without a copy */
     int *status_dev;
     uint64_t launches;
     char err[256];
@@ -49,13 +49,13 @@ fomoe_b200_ops_t *fomoe_b200_ops_create(int device) {
              cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) == cudaSuccess && major == 10 &&
              cudaDeviceGetAttribute(&o->dev.n_sm, cudaDevAttrMultiProcessorCount, device) == cudaSuccess &&
              cudaHostAlloc((void **)&o->status, 64, cudaHostAllocMapped) == cudaSuccess &&
-             cudaHostGetDevicePointer((void **)&o->status_dev, (void *)o->status, 0) == cudaSuccess &&
+             cudaHostGetDevicePointer((void **)&o->status_dev, o->status, 0) == cudaSuccess &&
              ops_rows_init() == 0 && ops_f8_init(&o->dev) == 0;
     if (ok) {
-        *o->status = FB_ST_OK;
+        memset(o->status, 0, OPS_STATUS_WORDS * sizeof(int));
     } else {
         fprintf(stderr, "fomoe_b200_ops_create: device %d cannot be used: %s\n", device, cudaGetErrorString(cudaGetLastError()));
-        if (o->status) cudaFreeHost((void *)o->status);
+        if (o->status) cudaFreeHost(o->status);
         free(o);
         o = NULL;
     }
@@ -71,9 +71,10 @@ const char *fomoe_b200_ops_last_error(fomoe_b200_ops_t *o) { return o ? o->err :
 
 int fomoe_b200_ops_status(fomoe_b200_ops_t *o) {
     if (!o) return -1;
-    const int st = *o->status;
-    if (st) *o->status = FB_ST_OK;
-    return st;
+    /* the worse first; read and cleared in one step, so that nothing stored in between is lost */
+    for (int st = OPS_STATUS_WORDS; st > FB_ST_OK; st--)
+        if (__atomic_exchange_n(&o->status[OPS_STATUS_WORD(st)], 0, __ATOMIC_ACQ_REL)) return st;
+    return FB_ST_OK;
 }
 
 uint64_t fomoe_b200_ops_kernel_launches(fomoe_b200_ops_t *o) { return o ? o->launches : 0; }

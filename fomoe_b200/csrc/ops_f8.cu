@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(BK_THREADS) k_ops_bucket(const int *ids, int n
 #pragma unroll
         for (int u = 0; u < BK_AHEAD; u++) {
             if ((unsigned)e[u] < (unsigned)n_experts) atomicAdd(&s_cnt[e[u] * BK_WARPS + warp], 1);
-            else if (e[u] != -1) *status = FB_ST_BAD_ID;
+            else if (e[u] != -1) status[OPS_STATUS_WORD(FB_ST_BAD_ID)] = 1;
         }
     }
     __syncthreads();
@@ -861,7 +861,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (C->abort_flag) {
-        if (tid == 0) *P.status = FB_ST_WAIT_TIMEOUT;
+        if (tid == 0) P.status[OPS_STATUS_WORD(FB_ST_WAIT_TIMEOUT)] = 1;
         for (int i = 0; i < 100; i++) __nanosleep(1000); /* copies and MMAs under way land before their memory is released */
     }
     if (SPLIT) {
@@ -1100,7 +1100,7 @@ __global__ void __launch_bounds__(32 * FG_WARPS) k_f8_few_gate_up(const __grid_c
     const int e = fr_expert(P, t, j);
     f8_next(); /* (the down product's weights may be asked for while this one runs) */
     if (e < 0) {
-        if (threadIdx.x == 0 && P.ids[t * P.top_k + j] != -1) *P.status = FB_ST_BAD_ID;
+        if (threadIdx.x == 0 && P.ids[t * P.top_k + j] != -1) P.status[OPS_STATUS_WORD(FB_ST_BAD_ID)] = 1;
         return;
     }
     const uint8_t *w0 = P.gate_up + ((int64_t)e * 2 * I + n0 + r0 + g) * H;

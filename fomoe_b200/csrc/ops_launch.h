@@ -29,6 +29,10 @@ typedef struct {
     float *weights;
 } ops_route_t;
 
+/* Where kernels store 1 when FB_ST_.. `st` happens: a word each, so that neither hides the other. */
+#define OPS_STATUS_WORD(st) ((st) - 1)
+#define OPS_STATUS_WORDS 2
+
 int ops_rows_init(void); /* loads the kernels on the current device */
 int ops_launch_route(const ops_route_t *a, void *stream);
 int ops_launch_norm(const fomoe_b200_norm_args_t *a, void *stream);

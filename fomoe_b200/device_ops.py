@@ -89,7 +89,7 @@ class DeviceOps:
             pass
 
     def status(self):
-        """0 nothing, 1 an expert id outside the table, 2 a bounded wait ran out; reading clears it."""
+        """0 nothing, 1 an expert id outside the table, 2 a bounded wait ran out (first, where both happened); reading clears it."""
         return int(self._l.fomoe_b200_ops_status(self._h))
 
     def kernel_launches(self):

@@ -406,7 +406,8 @@ void fomoe_b200_ops_destroy(fomoe_b200_ops_t *ops);
 const char *fomoe_b200_ops_last_error(fomoe_b200_ops_t *ops);
 /* What went wrong on the device since the last call of this function (as far as the device has got: synchronise first
  * for what is in flight): 0 nothing, 1 an expert id outside the table (its pair was left out), 2 a kernel gave a bounded
- * wait up (what it wrote is incomplete).  Reading clears it. */
+ * wait up (what it wrote is incomplete).  Reading clears what it returns; where both happened, 2 comes first and 1 with
+ * the next call. */
 int fomoe_b200_ops_status(fomoe_b200_ops_t *ops);
 uint64_t fomoe_b200_ops_kernel_launches(fomoe_b200_ops_t *ops);
 

@@ -1,4 +1,4 @@
-"""The handle of the operators on device memory: what it leaves behind when it goes.  No GPU:
+"""The handle of the operators on device memory: what it leaves behind when it goes, and what its status tells.  No GPU:
 ops_engine.c built against stand-ins (fake_cuda_status.c)."""
 import ctypes as C
 import gc
@@ -63,6 +63,15 @@ def test_captured_calls_outlive_their_handle(make, fake, how):
     product(after)
     fake.fake_goes_wrong(1)
     assert after.status() == 1
+
+
+def test_neither_fault_hides_the_other(make, fake):
+    o = make()
+    product(o)
+    for order in ((1, 2), (2, 1)):
+        for what in order:
+            fake.fake_goes_wrong(what)
+        assert [o.status() for _ in range(3)] == [2, 1, 0]
 
 
 def test_a_handle_goes_without_touching_the_device(make):
