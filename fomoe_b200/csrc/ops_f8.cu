@@ -10,6 +10,7 @@
 #include <stdint.h>
 
 #include "launch.h"
+#include "ops_launch.cuh"
 #include "ops_launch.h"
 #include "ops_quant.cuh"
 #include "stream.cuh"
@@ -28,18 +29,10 @@ __device__ __forceinline__ void f8_next() { asm volatile("griddepcontrol.launch_
 
 template <typename... P, typename... A>
 static int f8_launch_after(void (*k)(P...), dim3 grid, int threads, int smem, cudaStream_t st, A... args) {
-    cudaLaunchConfig_t c = {};
-    cudaLaunchAttribute at[1];
-    c.gridDim = grid;
-    c.blockDim = dim3(threads);
-    c.dynamicSmemBytes = smem;
-    c.stream = st;
+    cudaLaunchAttribute at[1] = {};
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
-    c.attrs = at;
-    c.numAttrs = 1;
-    const cudaError_t rc = cudaLaunchKernelEx(&c, k, args...);
-    return (int)(rc != cudaSuccess ? rc : cudaGetLastError());
+    return ops_launch(k, grid, threads, smem, st, at, 1, args...);
 }
 
 /* ------------------------------------------------------------------ bucket: the pairs of every expert, in pair order
@@ -1271,27 +1264,22 @@ static int f8_map(CUtensorMap *m, const void *p, uint64_t k, uint64_t rows, uint
 /* most_tiles: no more than this; at_once: tiles that the device works at at the same time */
 template <int MODE, int NT, int KIND>
 static int f8_launch(f8_args_t &p, int64_t most_tiles, int ranks, int at_once, int *launches, cudaStream_t st) {
-    cudaLaunchConfig_t c = {};
     cudaLaunchAttribute at[2] = {};
-    c.gridDim = dim3((unsigned)((KIND == F8_SPLIT || most_tiles < at_once ? most_tiles : at_once) * ranks));
-    c.blockDim = dim3(F8_THREADS);
-    c.dynamicSmemBytes = f8_cfg<MODE, NT, KIND>::SMEM;
-    c.stream = st;
+    int n = 0;
     if (KIND != F8_ONE) {
-        at[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        at[c.numAttrs].val.clusterDim.x = ranks;
-        at[c.numAttrs].val.clusterDim.y = at[c.numAttrs].val.clusterDim.z = 1;
-        c.numAttrs++;
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = ranks;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        n++;
     }
     if (MODE != F8_DENSE) {
-        at[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[c.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-        c.numAttrs++;
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n].val.programmaticStreamSerializationAllowed = 1;
+        n++;
     }
-    c.attrs = at;
     *launches += 1;
-    const cudaError_t rc = cudaLaunchKernelEx(&c, k_f8_mma<MODE, NT, KIND>, p);
-    return (int)(rc != cudaSuccess ? rc : cudaGetLastError());
+    const dim3 grid((unsigned)((KIND == F8_SPLIT || most_tiles < at_once ? most_tiles : at_once) * ranks));
+    return ops_launch(k_f8_mma<MODE, NT, KIND>, grid, F8_THREADS, f8_cfg<MODE, NT, KIND>::SMEM, st, at, n, p);
 }
 
 /* Microseconds of a tile: so much a block of k and so much around them, fitted to k of 1024 and 4096 (4096 x 8192 x 4096 by
@@ -1310,10 +1298,8 @@ extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *s
         const fr_args_t f = {a->m, a->n, a->k, a->a, a->a_stride, a->a_scales, a->a_scales_stride, a->b, a->b_stride, a->b_scales,
                              a->b_scales_stride, a->out, a->out_type == FOMOE_B200_BF16, a->out_stride};
         const int grid = (a->n + 15) / 16;
-        if (a->m <= 8) k_f8_few<1><<<grid, 32 * FR_WARPS, FR_SMEM, (cudaStream_t)stream>>>(f);
-        else k_f8_few<2><<<grid, 32 * FR_WARPS, FR_SMEM, (cudaStream_t)stream>>>(f);
         *launches += 1;
-        return (int)cudaGetLastError();
+        return ops_launch(a->m <= 8 ? k_f8_few<1> : k_f8_few<2>, grid, 32 * FR_WARPS, FR_SMEM, (cudaStream_t)stream, f);
     }
     f8_args_t p = {};
     p.m = a->m, p.n = a->n, p.k = a->k;
@@ -1440,9 +1426,8 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
         const fr_experts_t f = {a->n_embd, a->n_inter, a->n_experts, a->top_k, a->has_shared ? 1 : 0, a->n_tokens * a->top_k, a->x,
                                 a->x_stride, a->x_scales, a->x_scales_stride, a->ids, a->weights, a->gate_up, a->down,
                                 a->gate_up_scales, a->down_scales, ws + w.act_q, (float *)(ws + w.act_scales), (__nv_bfloat16 *)a->out, a->out_stride, status};
-        k_f8_few_gate_up<<<dim3(a->n_inter / 128, few_slots, a->n_tokens), 32 * FG_WARPS, FG_SMEM, st>>>(f);
+        const int rc = ops_launch(k_f8_few_gate_up, dim3(a->n_inter / 128, few_slots, a->n_tokens), 32 * FG_WARPS, FG_SMEM, st, f);
         *launches += 2;
-        const int rc = (int)cudaGetLastError();
         return rc ? rc : f8_launch_after(k_f8_few_down, dim3(a->n_embd / 16, a->n_tokens), 32 * FR_WARPS, few_smem, st, f);
     }
     const int n_routed = a->n_tokens * a->top_k, n_shared = a->has_shared ? a->n_tokens : 0, H = a->n_embd, I = a->n_inter;
@@ -1470,17 +1455,15 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     const int nb = (n_routed + run - 1) / run, bk_smem = a->n_experts * (BK_WARPS + 1) * 4;
     const int *ids = a->ids;
     if (nb > 1) {
-        k_ops_bucket<true><<<nb, BK_THREADS, bk_smem, st>>>(ids, n_routed, run, a->n_tokens, a->n_experts, a->has_shared, block_counts,
-                                                          counts, pairs, pos, items, status);
-        rc = (int)cudaGetLastError();
+        rc = ops_launch(k_ops_bucket<true>, nb, BK_THREADS, bk_smem, st, ids, n_routed, run, a->n_tokens, a->n_experts, a->has_shared,
+                        block_counts, counts, pairs, pos, items, status);
         if (!rc)
             rc = f8_launch_after(k_ops_bucket<false>, dim3(nb), BK_THREADS, bk_smem, st, ids, n_routed, run, a->n_tokens, a->n_experts,
                                  a->has_shared, block_counts, counts, pairs, pos, items, status);
         *launches += 1;
     } else {
-        k_ops_bucket<false><<<nb, BK_THREADS, bk_smem, st>>>(ids, n_routed, run, a->n_tokens, a->n_experts, a->has_shared, block_counts,
-                                                           counts, pairs, pos, items, status);
-        rc = (int)cudaGetLastError();
+        rc = ops_launch(k_ops_bucket<false>, nb, BK_THREADS, bk_smem, st, ids, n_routed, run, a->n_tokens, a->n_experts, a->has_shared,
+                        block_counts, counts, pairs, pos, items, status);
     }
     if (!rc)
         rc = f8_launch_after(k_ops_permute, dim3((w.n_pairs + 7) / 8), 256, 0, st, a->x, a->x_stride, a->x_scales, a->x_scales_stride, H,

@@ -10,6 +10,7 @@
 #include <stdint.h>
 
 #include "launch.h"
+#include "ops_launch.cuh"
 #include "ops_launch.h"
 #include "ops_quant.cuh"
 #include "stream.cuh"
@@ -374,11 +375,8 @@ __global__ void __launch_bounds__(32 * RT_WARPS, RT_BLOCKS) k_ops_route(const __
 
 extern "C" int ops_launch_route(const ops_route_t *a, void *stream) {
     const int grid = (a->n_tokens + RT_WARPS - 1) / RT_WARPS, E = a->cfg.n_experts;
-#define RT_GO(N, LOW)                                                           \
-    if (E <= 32 * N) {                                                          \
-        k_ops_route<N, LOW><<<grid, 32 * RT_WARPS, 0, (cudaStream_t)stream>>>(*a); \
-        return (int)cudaGetLastError();                                         \
-    }
+#define RT_GO(N, LOW) \
+    if (E <= 32 * N) return ops_launch(k_ops_route<N, LOW>, grid, 32 * RT_WARPS, 0, (cudaStream_t)stream, *a);
     RT_SIZES(RT_GO)
 #undef RT_GO
     return (int)cudaErrorInvalidValue;
@@ -695,20 +693,20 @@ static bool nm_al(const void *p, int64_t stride, int bytes) {
 }
 
 template <bool VEC>
-static void nm_launch(const fomoe_b200_norm_args_t &a, cudaStream_t st) {
+static int nm_launch(const fomoe_b200_norm_args_t &a, cudaStream_t st) {
     const int rw = (a.n_tokens + 7) / 8, T = a.n_tokens, n = a.n;
     /* one run of columns a thread while the rows do not fill the card (1 x 4096: 3.2 us, with two runs 3.9), two and more
      * blocks to an SM when they do (8192 x 4096: 76 us, with one run 80) */
     const bool few = T <= NM_FEW;
-    if (n <= 256) k_ops_norm<VEC, 32, 1><<<rw, 256, 0, st>>>(a);
-    else if (n <= 512) k_ops_norm<VEC, 32, 2><<<rw, 256, 0, st>>>(a);
-    else if (n <= 1024) k_ops_norm<VEC, 128, 1><<<T, 128, 0, st>>>(a);
-    else if (n <= 2048) k_ops_norm<VEC, 256, 1><<<T, 256, 0, st>>>(a);
-    else if (n <= 4096 && few) k_ops_norm<VEC, 512, 1><<<T, 512, 0, st>>>(a);
-    else if (n <= 4096) k_ops_norm<VEC, 256, 2><<<T, 256, 0, st>>>(a);
-    else if (n <= 8192 && few) k_ops_norm<VEC, 1024, 1><<<T, 1024, 0, st>>>(a);
-    else if (n <= 8192) k_ops_norm<VEC, 512, 2><<<T, 512, 0, st>>>(a);
-    else k_ops_norm<VEC, 1024, 2><<<T, 1024, 0, st>>>(a);
+    return n <= 256          ? ops_launch(k_ops_norm<VEC, 32, 1>, rw, 256, 0, st, a)
+           : n <= 512         ? ops_launch(k_ops_norm<VEC, 32, 2>, rw, 256, 0, st, a)
+           : n <= 1024        ? ops_launch(k_ops_norm<VEC, 128, 1>, T, 128, 0, st, a)
+           : n <= 2048        ? ops_launch(k_ops_norm<VEC, 256, 1>, T, 256, 0, st, a)
+           : n <= 4096 && few ? ops_launch(k_ops_norm<VEC, 512, 1>, T, 512, 0, st, a)
+           : n <= 4096        ? ops_launch(k_ops_norm<VEC, 256, 2>, T, 256, 0, st, a)
+           : n <= 8192 && few ? ops_launch(k_ops_norm<VEC, 1024, 1>, T, 1024, 0, st, a)
+           : n <= 8192        ? ops_launch(k_ops_norm<VEC, 512, 2>, T, 512, 0, st, a)
+                              : ops_launch(k_ops_norm<VEC, 1024, 2>, T, 1024, 0, st, a);
 }
 
 extern "C" int ops_launch_norm(const fomoe_b200_norm_args_t *a, void *stream) {
@@ -719,9 +717,7 @@ extern "C" int ops_launch_norm(const fomoe_b200_norm_args_t *a, void *stream) {
                      nm_al(a->block, many * a->block_stride, bs) && nm_al(a->post, 0, 4) && nm_al(a->pre, 0, 4) &&
                      (!a->gate_step || nm_al(a->gate, many * a->gate_stride, bs)) &&
                      nm_al(a->pre ? a->h : nullptr, many * a->h_stride, hs);
-    if (vec) nm_launch<true>(*a, (cudaStream_t)stream);
-    else nm_launch<false>(*a, (cudaStream_t)stream);
-    return (int)cudaGetLastError();
+    return vec ? nm_launch<true>(*a, (cudaStream_t)stream) : nm_launch<false>(*a, (cudaStream_t)stream);
 }
 
 /* ------------------------------------------------------------------ rows to FP8: 8 threads per block of 128
@@ -752,14 +748,12 @@ extern "C" int ops_launch_f8_quantize(int rows, int cols, const void *x, int x_b
     for (int64_t r0 = 0; r0 < rows; r0 += at_once) {
         const int n = rows - r0 < at_once ? (int)(rows - r0) : at_once, grid = (int)(((int64_t)n * nb + 31) / 32);
         const uint8_t *xr = reinterpret_cast<const uint8_t *>(x) + r0 * x_stride * (x_bf16 ? 2 : 4);
-        if (vec)
-            k_ops_quantize<true><<<grid, 256, 0, (cudaStream_t)stream>>>(n, cols, nb, per_nb, xr, x_bf16, x_stride, q + r0 * q_stride,
-                                                                       q_stride, scales + r0 * scales_stride, scales_stride);
-        else
-            k_ops_quantize<false><<<grid, 256, 0, (cudaStream_t)stream>>>(n, cols, nb, per_nb, xr, x_bf16, x_stride, q + r0 * q_stride,
-                                                                        q_stride, scales + r0 * scales_stride, scales_stride);
+        const int rc = ops_launch(vec ? k_ops_quantize<true> : k_ops_quantize<false>, grid, 256, 0, (cudaStream_t)stream, n, cols, nb, per_nb,
+                                  (const void *)xr, x_bf16, x_stride, q + r0 * q_stride, q_stride, scales + r0 * scales_stride,
+                                  scales_stride);
+        if (rc) return rc;
     }
-    return (int)cudaGetLastError();
+    return 0;
 }
 
 /* every kernel of this file loaded on the current device, so that no call loads one inside a stream capture */

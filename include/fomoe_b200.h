@@ -385,7 +385,9 @@ void fomoe_b200_batch_synth_logits(uint64_t seed, int layer, int max_tokens, int
  *    Like fomoe_b200_matvec_noalloc they take DEVICE pointers, enqueue on the caller's stream (a cudaStream_t of the
  *    handle's device; NULL = its default stream), allocate nothing and do not synchronise, so every call can be captured
  *    into a CUDA graph; the device that is current on entry is current again on return.  Return 0, or -1 with the reason
- *    in fomoe_b200_ops_last_error (and on stderr) and nothing enqueued.  A call with no rows returns 0.
+ *    in fomoe_b200_ops_last_error (and on stderr): for arguments that are refused nothing has been enqueued then; where CUDA
+ *    refuses the launch of one of a call's kernels (the reason says so) those before it have been.  An error that an earlier
+ *    CUDA call left behind does not count and stays.  A call with no rows returns 0.
  *    A handle is used from one thread at a time; any number of streams may have its calls in flight.
  *
  *    FP8 here is e4m3 (OCP: 4 exponent bits, largest value 448) with fp32 scales: one for each block of 128 values of an
