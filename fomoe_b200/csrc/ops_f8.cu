@@ -438,7 +438,7 @@ __device__ __forceinline__ void f8_box_out(uint32_t buf, const CUtensorMap *map,
 }
 
 /* the first `rows` rows of a staged box, by the warp.  row0: where the first row's 128 bytes go, stride: bytes from row to
- * row, left: bytes of a row that are inside out, elem: bytes of a value */
+ * row, left: bytes of the box's rows that are inside out (bytes of a whole row may not fit an int), elem: bytes of a value */
 __device__ __forceinline__ void f8_rows_out(uint32_t buf, uint8_t *row0, int64_t stride, int rows, int left, int elem) {
     const int lane = threadIdx.x & 31, per = 128 / elem;
     for (int i = lane; i < rows * per; i += 32) {
@@ -811,7 +811,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                     }
                     if (PAIR) {
                         f8_runs_out<2 * W>(buf, w, reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + w0) * P.out_stride + c0),
-                                           2 * P.out_stride, rows, 2 * (P.n - c0), 2, P.out_tma);
+                                           2 * P.out_stride, rows, 2 * min(P.n - c0, W), 2, P.out_tma);
                         continue;
                     }
                     f8_box_wait();
@@ -825,12 +825,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                         if (tma) f8_box_out(buf + c * 4096u, &P.to, 2 * x, t.r0 + w0);
                         else
                             f8_rows_out(buf + c * 4096u, reinterpret_cast<uint8_t *>(P.out) + 2 * ((int64_t)(t.r0 + w0) * P.out_stride + x),
-                                        2 * P.out_stride, rows, 2 * (P.n - x), 2);
+                                        2 * P.out_stride, rows, 2 * min(P.n - x, 64), 2);
                     }
                 } else if (PAIR) {
                     f8_runs_out<4 * W>(buf, reinterpret_cast<const uint32_t *>(acc),
                                        reinterpret_cast<uint8_t *>(P.out) + 4 * ((int64_t)(t.r0 + w0) * P.out_stride + c0),
-                                       4 * P.out_stride, rows, 4 * (P.n - c0), 4, P.out_tma);
+                                       4 * P.out_stride, rows, 4 * min(P.n - c0, W), 4, P.out_tma);
                 } else {
 #pragma unroll
                     for (int c = 0; c < W / 32; c++) { /* boxes of 32 columns, through the buffers there are */
@@ -843,7 +843,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                         else
                             f8_rows_out(buf + c % cfg::BUFS * 4096u,
                                         reinterpret_cast<uint8_t *>(P.out) + 4 * ((int64_t)(t.r0 + w0) * P.out_stride + x),
-                                        4 * P.out_stride, rows, 4 * (P.n - x), 4);
+                                        4 * P.out_stride, rows, 4 * min(P.n - x, 32), 4);
                     }
                 }
             }
