@@ -7,6 +7,7 @@ the same bytes)."""
 import ctypes as C
 
 F32, BF16, F8 = 0, 1, 2
+_OVER = 1 << 31   # no C int (ctypes would keep the low 32 bits)
 
 
 class RouteConfig(C.Structure):
@@ -110,7 +111,9 @@ class DeviceOps:
                          f"{t.device} with strides {t.stride()}")
 
     def _rows(self, t, name, types, shape=None):
-        """Checks a 2-D tensor with contiguous rows; -> its row stride."""
+        """Checks a 2-D tensor with contiguous rows, whose sizes are C ints; -> its row stride."""
+        if t.numel() >= _OVER and max(t.shape) >= _OVER:
+            raise ValueError(f"{name}: less than 2^31 rows and columns are taken, got {tuple(t.shape)}")
         if (t.dim() != 2 or t.dtype not in types or t.get_device() != self.device or (t.stride(1) != 1 and t.shape[1] > 1)
                 or (shape is not None and t.shape != shape)):
             self._bad(t, name, types, shape, "a 2-D tensor with contiguous rows")
@@ -132,7 +135,10 @@ class DeviceOps:
             raise ValueError(f"score: 'softmax' or 'sigmoid' is wanted, got {score!r}")
         b = None if bias is None else self._flat(bias, "bias", self._f32, (E,))
         v = None if valid is None else self._flat(valid, "valid", self._u8, (T,))
-        k = top_k if top_k > 0 else 0
+        if (top_k | n_group | topk_group | group_best) >> 31:
+            raise ValueError("top_k, n_group, topk_group and group_best: 0 to 2^31 - 1 is wanted, got "
+                             f"{(top_k, n_group, topk_group, group_best)}")
+        k = top_k if top_k <= E else 0   # (more is refused by the call)
         ids, w = logits.new_empty((T, k), dtype=t.int32), logits.new_empty((T, k), dtype=t.float32)
         cfg = RouteConfig(E, top_k, SCORES[score], n_group, topk_group, group_best, 1 if renorm else 0, scale)
         self._ck(self._l.fomoe_b200_ops_route(self._h, cfg, T, logits.data_ptr(), self._float[logits.dtype], stride, b, v,
@@ -224,6 +230,8 @@ class DeviceOps:
         R, I2 = gate_up.shape[:2]
         I = I2 // 2
         k = ids.shape[1] if ids.dim() == 2 else 0
+        if (R | I2 | k) >> 31:
+            raise ValueError(f"records, rows of a record and slots: less than 2^31 are taken, got {(R, I2, k)}")
         if H % 128 or I2 % 256:
             raise ValueError(f"hidden size {H} and intermediate size {I2} / 2: multiples of 128 are wanted")
         hb, ib = H // 128, I // 128
@@ -247,5 +255,7 @@ class DeviceOps:
 
     def f8_experts_workspace(self, n_tokens, n_embd, n_inter, n_experts, top_k, shared=False):
         """Bytes of workspace a call of f8_experts of these sizes needs (0: sizes that it refuses)."""
+        if (n_tokens | n_embd | n_inter | n_experts | top_k) >> 31:
+            return 0
         return int(self._l.fomoe_b200_ops_f8_experts_workspace(
             ExpertsArgs(n_tokens, n_embd, n_inter, n_experts, top_k, int(bool(shared)))))
