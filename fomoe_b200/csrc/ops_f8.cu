@@ -215,7 +215,7 @@ typedef struct {
     int64_t out_stride;
     uint8_t *act_q; /* F8_GATE_UP: [pairs][n] */
     float *act_scales;
-    const int *counts, *pairs;
+    const int *counts;
     const int4 *items;
     int *status;
 } f8_args_t;
@@ -796,7 +796,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
                 /* rows of this warp that are the tile's; a box may only leave whole if none of its rows is another expert's */
                 const int w0 = (warp & 3) * 32, rows = ok ? max(0, min(32, t.rows - w0)) : 0, c0 = t.n0 + wg * W;
                 const bool tma = !PAIR && P.out_tma && (MODE == F8_DENSE ? rows > 0 : rows == 32);
-                if (MODE == F8_DOWN && !tma) { /* (61 tokens of 8 in 256 experts, as fp16: 150 us by staged rows, 133 so) */
+                if (MODE == F8_DOWN && !tma) { /* (61 tokens of 8 in 256 experts: 156 us by staged rows, 143 so) */
                     if (lane < rows && c0 < P.n) {
                         float *o = reinterpret_cast<float *>(P.out) + (int64_t)(t.r0 + row) * P.out_stride + c0;
 #pragma unroll
@@ -1052,7 +1052,7 @@ __global__ void __launch_bounds__(32 * FR_WARPS) k_f8_few(const fr_args_t P) {
 }
 
 typedef struct {
-    int n_embd, n_inter, n_experts, top_k, has_shared, n_routed;
+    int n_embd, n_inter, n_experts, top_k, has_shared;
     const uint8_t *x;
     int64_t x_stride;
     const float *x_scales;
@@ -1307,8 +1307,8 @@ extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *s
     p.b_scales = a->b_scales, p.bs_stride = a->b_scales_stride;
     p.out = a->out, p.out_bf16 = a->out_type == FOMOE_B200_BF16, p.out_stride = a->out_stride;
     const int eb = p.out_bf16 ? 2 : 4;
-    const int64_t os = a->m == 1 ? (int64_t)a->n * eb : a->out_stride * eb;
-    p.out_tma = ((uintptr_t)a->out & 15) == 0 && (a->m == 1 ? 1 : os % 16 == 0);
+    const int64_t os = a->out_stride * eb;
+    p.out_tma = ((uintptr_t)a->out & 15) == 0 && os % 16 == 0;
     p.status = status;
     cudaStream_t st = (cudaStream_t)stream;
     const int64_t m = a->m, n = a->n, mt = (m + 127) / 128;
@@ -1325,7 +1325,7 @@ extern "C" int ops_launch_f8_matmul(const fomoe_b200_f8_matmul_args_t *a, int *s
     }
     if (d->clusters[1] > 0 && f8_waves(pairs, d->clusters[1]) * F8_PAIR_US(kb) < best) pair = 1, nt = 256;
     int rc = f8_map(&p.ta, a->a, a->k, a->m, a->a_stride, 32) | f8_map(&p.tb, a->b, a->k, a->n, a->b_stride, pair ? 128 : nt);
-    if (p.out_tma) rc |= f8_map(&p.to, a->out, (uint64_t)a->n * eb, a->m, (os + 15) & ~15ull, 32);
+    if (p.out_tma) rc |= f8_map(&p.to, a->out, (uint64_t)a->n * eb, a->m, os, 32);
     if (rc) return rc;
     return pair         ? f8_launch<F8_DENSE, 256, F8_PAIR>(p, pairs, 2, d->clusters[1], launches, st)
            : nt == 256  ? f8_launch<F8_DENSE, 256, F8_ONE>(p, t256, 1, n_sm, launches, st)
@@ -1423,7 +1423,7 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     const int few_slots = a->top_k + (a->has_shared ? 1 : 0);
     const int few_smem = FD_SMEM + few_slots * a->n_inter + few_slots * (a->n_inter / 128) * 4; /* of the down product */
     if (experts_few(a, w.n_pairs) && few_smem <= FD_SMEM_MOST) {
-        const fr_experts_t f = {a->n_embd, a->n_inter, a->n_experts, a->top_k, a->has_shared ? 1 : 0, a->n_tokens * a->top_k, a->x,
+        const fr_experts_t f = {a->n_embd, a->n_inter, a->n_experts, a->top_k, a->has_shared ? 1 : 0, a->x,
                                 a->x_stride, a->x_scales, a->x_scales_stride, a->ids, a->weights, a->gate_up, a->down,
                                 a->gate_up_scales, a->down_scales, ws + w.act_q, (float *)(ws + w.act_scales), (__nv_bfloat16 *)a->out, a->out_stride, status};
         const int rc = ops_launch(k_f8_few_gate_up, dim3(a->n_inter / 128, few_slots, a->n_tokens), 32 * FG_WARPS, FG_SMEM, st, f);
@@ -1436,7 +1436,7 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     int *block_counts = (int *)(ws + w.block_counts);
     int4 *items = (int4 *)(ws + w.counts + 256);
     f8_args_t gu = {}, dn;
-    gu.counts = counts, gu.pairs = pairs, gu.items = items, gu.status = status;
+    gu.counts = counts, gu.items = items, gu.status = status;
     dn = gu;
     gu.n = I, gu.k = H;
     gu.a_scales = (const float *)(ws + w.xp_scales), gu.as_stride = H / 128;
