@@ -916,7 +916,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_f8_mma(const __grid_constant_
  * four 16-byte pieces that it will read, so no lane waits for another.  The k inside a block come in the order that this
  * gives: lane (g, t) holds bytes 16 t .. of rows g and g + 8, the activations likewise.  16 weight rows a block spread small
  * matrices over all SMs, and nothing has to be set up first: 1 x 4096 x 4096 5.4 us (on tcgen05 11), 16 rows 7.4, 1 x 8192 x
- * 8192 16 us, 1 x 4096 x 16,384 14.5 us, 4.6 TB/s; start and end of a block are what is left. */
+ * 8192 16 us, 1 x 4096 x 16,384 14.5 us, 4.6 TB/s; what is left are start and end of a block, and of large matrices that 256
+ * or 512 equal blocks do not come out even on 148 SMs. */
 #define FR_WARPS 8
 #define FR_RING 2
 #define FR_SMEM (FR_WARPS * FR_RING * 2048)
@@ -1386,8 +1387,8 @@ __global__ void __launch_bounds__(256) k_ops_combine(const float *dots, const in
 
 /* Each pair by itself, or bucketed by expert: microseconds of either.  Few pairs stream their experts' weights once a pair, at
  * 5.3 TB/s and with 8 us around it and a block's start a pair; bucketed they are read once an expert, but five kernels and
- * their tiles come first.  (By themselves | bucketed: one token with 11 experts of 4096 x 1024 34.8 | 56 us, 27 pairs of it
- * 74 | 86, 45 pairs 114 | 94; 2048 x 768, 32 pairs 39 | 46, 64 pairs 67 | 64; 192 pairs in 17 experts of 512 x 256 30 | 23.)
+ * their tiles come first.  (By themselves | bucketed: one token with 11 experts of 4096 x 1024 36 | 57 us, 27 pairs of it
+ * 77 | 90, 45 pairs 117 | 101; 2048 x 768, 32 pairs 40 | 59, 64 pairs 65 | 66; 192 pairs in 17 experts of 512 x 256 30 | 24.)
  * How many different experts there will be is known on the device only: the expectation of equally likely ones stands for it. */
 static int experts_few(const fomoe_b200_f8_experts_args_t *a, int n_pairs) {
     const double bytes = 3.0 * a->n_embd * a->n_inter, routed = (double)a->n_tokens * a->top_k;
@@ -1472,7 +1473,8 @@ extern "C" int ops_launch_f8_experts(const fomoe_b200_f8_experts_args_t *a, uint
     /* no more tiles than this (the device knows how many there are).  Tiles of 32 rows, with more weights in flight and a
      * joining warp of each warpgroup, were tried for few pairs an expert: 61 tokens of 8 in 256 experts 155 us as with 128;
      * tiles of 256 by pairs of SMs for many: 8192 tokens of 8 + 1 in 64 experts 1.59 ms under the power cap, 1.55 with 128,
-     * half a tile of every expert being padding. */
+     * half a tile of every expert being padding (all of these with an expert's output in fp16, which saves 10 % of the last but
+     * rounds what the sum over the experts may cancel). */
     const int64_t tiles = w.n_pairs / 128 + recs;
     if (!rc) rc = f8_launch<F8_GATE_UP, 256, F8_ONE>(gu, tiles * (I / 128), 1, n_sm, launches, st);
     if (!rc) rc = f8_launch<F8_DOWN, 256, F8_ONE>(dn, tiles * ((H + 255) / 256), 1, n_sm, launches, st);

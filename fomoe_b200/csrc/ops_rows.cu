@@ -31,7 +31,11 @@
  * The best K + 1 keys: each lane's best key first; the (K + 1)-th best of those is a bound that every one of the best K + 1
  * keys reaches, and few others do.  The keys that reach it are put side by side in shared memory, one to a lane, and each
  * counts how many are better.  (16,384 tokens x 384 experts, sigmoid + bias, top 8: 87 us in 64 bits with a round over all
- * keys for every slot, 18 us so; bound by its instructions, 810 a token at 69 % of the issue slots) */
+ * keys for every slot, 18 us so: 810 instructions a token at 66 % of the issue slots, 28 of 64 warps on an SM; 256 experts in 8
+ * groups 25 us, 1060 at 70 %)
+ *
+ * How often 64 bits are needed goes by the logits.  16,384 x 256 in 8 groups, logits of 1.5, 5, 8, 16 x normal: softmax 25, 27,
+ * 32, 46 us, sigmoid 24, 32, 51, 50 us (groups' scores that saturate); with a bias of 0.1 x normal 25 to 27 us throughout. */
 #define RT_WARPS 4
 #define RT_BLOCKS 8 /* an SM: registers for so many (16,384 x 512, bias, top 16: 35 us, unbounded 36, for ten 44) */
 #define RT_NEAR(a, b) (8e-6f + 1e-6f * (fabsf(a) + fabsf(b)))
@@ -393,7 +397,9 @@ extern "C" int ops_launch_route(const ops_route_t *a, void *stream) {
  * sums over the block, two square roots, the scale of a block -- is long, so it takes many rows at once on an SM: blocks of 256
  * threads whose registers let five share one, and the next rows asked into L2.  Rings of rows in shared memory under persistent
  * blocks (108 us and more: they take the L1 that holds the weights) and 128 threads with four runs each (85 us) were slower;
- * values in pairs (fma.rn.f32x2) saved 2 us, one scale for 16 values a thread the quantiser a quarter of its time. */
+ * values in pairs (fma.rn.f32x2) saved 2 us, one scale for 16 values a thread the quantiser a quarter of its time.
+ * Rows without alignment (8192 x 4095: 160 us) take twice the instructions, 91 M for 43 M, from three blocks an SM (72
+ * registers for 48): narrow accesses and the exchange in shared memory. */
 #define NM_THREADS(G) ((G) == 32 ? 256 : (G))
 #define NM_AHEAD 148 /* rows: what a later block reads is asked into L2 (8192 x 4096: 74 us, without 82, 296 rows ahead 74) */
 #define NM_BLOCKS 5  /* of 256 threads, an SM (8192 x 4096: 68 us, with 4 74, with 6 and spills 93) */

@@ -3,7 +3,8 @@
 Every call enqueues on torch's current stream of the handle's device, allocates its results (and the experts' workspace)
 through torch on that stream, and neither copies to the host nor synchronises: calls can be captured into a CUDA graph.
 Rows may be strided; the last axis of a tensor is contiguous.  FP8 tensors are ``torch.float8_e4m3fn`` (or ``uint8`` with
-the same bytes)."""
+the same bytes).  The operators serve: autograd does not see them (results carry no gradient, and ``norm(inplace=True)``
+writes x without its version counter)."""
 import ctypes as C
 
 F32, BF16, F8 = 0, 1, 2

@@ -495,8 +495,8 @@ int fomoe_b200_ops_f8_matmul(fomoe_b200_ops_t *ops, const fomoe_b200_f8_matmul_a
 
 /* The experts of one layer on FP8 rows, routing given:
  *     z = gate_up_e x,  act = silu(z[0 .. I)) * z[I .. 2 I)  (to FP8 per 128),  y_e = down_e act
- *     out[t] = sum_j weights[t][j] y_{ids[t][j]}  (in slot order)  + y_shared   (bf16)
- * The products, each y_e and the sum over the experts are fp32.
+ *     out[t] = sum_j weights[t][j] y_{ids[t][j]} + y_shared   (bf16)
+ * The products, each y_e and the sum over the experts are fp32; the order of the sums goes by the call's sizes alone.
  * ids of -1 are left out (as fomoe_b200_ops_route writes them); other ids outside 0 .. n_experts - 1 too, with status 1.
  * A token with no expert at all gets zeros.  The tables hold n_experts + has_shared contiguous records, the shared
  * expert last.  workspace: fomoe_b200_ops_f8_experts_workspace bytes, 256-byte aligned; its contents do not matter
